@@ -481,6 +481,69 @@ int loom_b200_decoder_set_stack_embeddings(loom_b200_decoder* dec, const void* t
  * Ternary decoders take it too, with want empty or the last place only. */
 int loom_b200_decoder_extend(loom_b200_decoder* dec, const int32_t* tokens, int n, const int32_t* want, int n_want, float* logits_host);
 
+/* ---- serving several requests on one decoder ------------------------------------------------------
+ * No counterpart in the reference, which decodes greedily, keeps float32 rings and has one set of weights for every request.
+ * All buffers are device memory; the calls may be recorded between graph_begin and graph_end. */
+
+/* The next token of every row of logits [rows, vocab] (`stride` floats from one row to the next) by temperature, top-k, top-p and
+ * min-p, from random numbers that the caller gives.  Per row, arrays [rows], each but `uniform` may be NULL (= 1, 0, 1, 0):
+ *   order  larger logits first, equal ones by index; weight w_i = exp((l_i - largest) / temperature)
+ *   kept   the first top_k (0 or less: all); of those the shortest run from the front that holds top_p of their weight (1 or more: all;
+ *          one token at least); of those the ones with w_i >= min_p (0 or less: all)
+ *   token  the first kept one by index at which the kept weight up to it exceeds uniform (0 <= uniform < 1; else the last one, or the
+ *          first) times all of it
+ * temperature 0 or less: the first largest logit.  Not-a-numbers and minus infinity are never chosen; plus infinities share alike; a row
+ * with nothing to choose gives -1.  logprob [rows] or NULL: logarithm of the chosen token's share of the kept weight (not a number for -1).
+ * Sums are integers and repeat bit for bit.  vocab <= 737,280. */
+int loom_b200_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logits, long long stride, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* tokens, float* logprob);
+
+/* The same for a decoder, from the logits that its last forward left on the device: of one sequence (seq), or of every one (seq -1; all need a
+ * prompt behind them).  Host arrays, one entry for each of them; the tokens are the caller's to feed to the next forward, extend or step_batch. */
+int loom_b200_decoder_sample(loom_b200_decoder* dec, int seq, const float* temperature, const int32_t* top_k, const float* top_p,
+                             const float* min_p, const float* uniform, int32_t* tokens, float* logprob);
+
+/* Low-rank adapters of several requests beside a projection that they share (loom_b200_ternary_linear, loom_b200_ternary_gemm):
+ * `slots` adapters for a matrix [rows, cols], each of a rank of its own up to max_rank (<= 256), bf16 or float32.  put fills a slot
+ * from down [rank, cols] and up [rows, rank], row-major values of either type (host memory, or device memory with src_on_device; the call
+ * returns when they have been read); rank 0 empties it. */
+typedef struct loom_b200_adapters loom_b200_adapters;
+int loom_b200_adapters_create(loom_b200_ctx* ctx, int slots, int rows, int cols, int max_rank, int dtype, loom_b200_adapters** out);
+int loom_b200_adapters_put(loom_b200_ctx* ctx, loom_b200_adapters* a, int slot, int rank, float scale, const void* down, const void* up,
+                           int src_dtype, int src_on_device);
+int loom_b200_adapters_info(const loom_b200_adapters* a, int* slots, int* rows, int* cols, int* max_rank, int* dtype);
+void loom_b200_adapters_free(loom_b200_ctx* ctx, loom_b200_adapters* a);
+/* out[t] = base[t] + scale_s * up_s (down_s x[t]) with s = slot[t]; a token whose slot is outside [0, slots) or empty gets base[t].
+ * x [tokens, cols] with ldx floats from one row to the next, slot [tokens], base [tokens, rows] or NULL (zeros), out [tokens, rows]; base may
+ * be out.  Products and sums as float32 operands would give them, whatever the adapters' type; a row of x
+ * that is not finite gives not-a-numbers. */
+int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, int tokens, const int32_t* slot, const float* x, long long ldx,
+                             const float* base, float* out);
+
+/* A cache of keys and values in 8 bits for `sequences` sequences of up to max_len positions, head_dim <= 256.  Positions go by blocks of
+ * 64: a whole block is held as int8 codes with one scale for each KV head, for keys and for values (largest |x| / 127; codes rounded half
+ * away from zero, as loom_b200_quantize_activation does); the positions behind a sequence's last whole block are held as they came.  A
+ * block with a value that is not finite reads as not-a-numbers.
+ * The caller keeps the lengths: every call takes the device array lengths [sequences], the positions that each sequence holds in front of
+ * this call's rows, and starts [sequences + 1]: rows starts[s] .. starts[s+1]-1 belong to sequence s and have the positions
+ * lengths[s], lengths[s] + 1, ... (no rows: the sequence takes no part); rows behind starts[sequences] are left as they are.  starts NULL: one row each
+ * of the first `rows` sequences, a decode step.  A sequence is cut back by giving a smaller length, not further than to the beginning of the block in
+ * front of the one its last position lies in.  Rows that a sequence has no room for are not taken (attention: zeros), which loom_b200_sync
+ * reports as LOOM_B200_ERR_INVALID. */
+typedef struct loom_b200_kv8 loom_b200_kv8;
+int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_heads, int head_dim, loom_b200_kv8** out);
+void loom_b200_kv8_free(loom_b200_ctx* ctx, loom_b200_kv8* cache);
+/* k, v [rows, kv_heads, head_dim] with ld floats from one row to the next */
+int loom_b200_kv8_append(loom_b200_ctx* ctx, loom_b200_kv8* cache, int rows, const int32_t* starts, const int32_t* lengths, const float* k,
+                         const float* v, long long ld);
+/* the rows of an append with the same starts and lengths, as the cache holds them: k, v [rows, kv_heads, head_dim] */
+int loom_b200_kv8_read(loom_b200_ctx* ctx, loom_b200_kv8* cache, int rows, const int32_t* starts, const int32_t* lengths, float* k, float* v);
+/* Causal attention of the rows of an append with the same starts and lengths: row j of sequence s sees positions 0 .. lengths[s] + j, in the
+ * state that the cache has behind that append.  q [rows, heads, head_dim] with ldq floats from one row to the next, head H reads KV head
+ * H / (heads / kv_heads); scale: factor of the scores, 0 or less means 1 / sqrt(head_dim); out [rows, heads, head_dim]. */
+int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* cache, int rows, int heads, const int32_t* starts, const int32_t* lengths,
+                         const float* q, long long ldq, double scale, float* out);
+
 /* ---- tensor parallelism over the GPUs of one box --------------------------------------------------
  * The reference has no multi-device path (its only sharding notion is the per-layer tile size,
  * poly/wgpu_context.go).  The split used here is the one the integer arithmetic allows without changing a bit

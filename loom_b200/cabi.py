@@ -40,6 +40,7 @@ _i = C.c_int
 _f = C.c_float
 _d = C.c_double
 _sz = C.c_size_t
+_ll = C.c_longlong
 
 # name -> (restype, argtypes); kept in one table so that the symbol-export test can walk it
 SIGNATURES = {
@@ -121,6 +122,18 @@ SIGNATURES = {
     "loom_b200_decoder_set_layer": (_i, [_vp, _i, _vp, _vp]),
     "loom_b200_decoder_set_stack_embeddings": (_i, [_vp, _vp, _f, _vp, _f, _vp]),
     "loom_b200_decoder_extend": (_i, [_vp, _vp, _i, _vp, _i, _vp]),
+    "loom_b200_sample": (_i, [_vp, _i, _i, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "loom_b200_decoder_sample": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "loom_b200_adapters_create": (_i, [_vp, _i, _i, _i, _i, _i, C.POINTER(_vp)]),
+    "loom_b200_adapters_put": (_i, [_vp, _vp, _i, _i, _f, _vp, _vp, _i, _i]),
+    "loom_b200_adapters_info": (_i, [_vp, C.POINTER(_i), C.POINTER(_i), C.POINTER(_i), C.POINTER(_i), C.POINTER(_i)]),
+    "loom_b200_adapters_free": (None, [_vp, _vp]),
+    "loom_b200_adapters_apply": (_i, [_vp, _vp, _i, _vp, _vp, _ll, _vp, _vp]),
+    "loom_b200_kv8_create": (_i, [_vp, _i, _i, _i, _i, C.POINTER(_vp)]),
+    "loom_b200_kv8_free": (None, [_vp, _vp]),
+    "loom_b200_kv8_append": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _ll]),
+    "loom_b200_kv8_read": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "loom_b200_kv8_attend": (_i, [_vp, _vp, _i, _i, _vp, _vp, _vp, _ll, _d, _vp]),
     "loom_b200_tp_unique_id": (_i, [_vp]),
     "loom_b200_tp_init": (_i, [_vp, _i, _i, _vp]),
     "loom_b200_tp_peer_handle": (_i, [_vp, _vp]),
@@ -374,6 +387,11 @@ class Context:
         self._check(lib().loom_b200_ternary_gemm(self.h, w.h, tokens, _ptr(x), _ptr(bias), _ptr(residual), act, _ptr(out),
                                                  _ptr(acc_out), _ptr(amax_out)))
 
+    def sample(self, rows, vocab, logits, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None, stride=None):
+        """The next token of every row of logits (device buffers; one entry a row in every array)."""
+        self._check(lib().loom_b200_sample(self.h, rows, vocab, _ptr(logits), vocab if stride is None else stride, _ptr(temperature), _ptr(top_k), _ptr(top_p),
+                                           _ptr(min_p), _ptr(uniform), _ptr(tokens), _ptr(logprob)))
+
     # ---- tensor parallelism: one process per GPU, one context per process ----
     @staticmethod
     def tp_unique_id() -> bytes:
@@ -545,6 +563,82 @@ class Matrix:
             pass
 
 
+class Adapters:
+    """Low-rank adapters of several requests for one matrix [rows, cols]: `slots` places, each of a rank of its own."""
+
+    def __init__(self, ctx: "Context", slots: int, rows: int, cols: int, max_rank: int, dtype: int = DTYPE_BF16):
+        self.ctx, self.h = ctx, None
+        self.slots, self.rows, self.cols, self.max_rank, self.dtype = slots, rows, cols, max_rank, dtype
+        h = _vp()
+        ctx._check(lib().loom_b200_adapters_create(ctx.h, slots, rows, cols, max_rank, dtype, C.byref(h)))
+        self.h = h
+
+    def put(self, slot: int, down, up, scale: float = 1.0, dtype: int = DTYPE_F32):
+        """down [rank, cols] and up [rows, rank]: host arrays (float32, or uint16 bit patterns with DTYPE_BF16) or device tensors; None
+        for both empties the slot."""
+        rank, on_device = 0 if down is None else down.shape[0], hasattr(down, "data_ptr")
+        if rank and not on_device:
+            down, up = np.ascontiguousarray(down), np.ascontiguousarray(up)
+        if rank and (tuple(down.shape) != (rank, self.cols) or tuple(up.shape) != (self.rows, rank)):
+            raise ValueError("adapter of %s and %s for a matrix %dx%d" % (tuple(down.shape), tuple(up.shape), self.rows, self.cols))
+        self.ctx._check(lib().loom_b200_adapters_put(self.ctx.h, self.h, slot, rank, float(scale), _ptr(down), _ptr(up), dtype, 1 if on_device else 0))
+
+    def apply(self, tokens, slot, x, out, base=None, ldx=None):
+        """out[t] = base[t] + scale up (down x[t]) with the adapter in slot[t] (device buffers; base may be out)."""
+        self.ctx._check(lib().loom_b200_adapters_apply(self.ctx.h, self.h, tokens, _ptr(slot), _ptr(x), self.cols if ldx is None else ldx, _ptr(base), _ptr(out)))
+
+    def free(self):
+        if self.h:
+            if self.ctx.h:
+                lib().loom_b200_adapters_free(self.ctx.h, self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+class KV8:
+    """Keys and values of several sequences in 8 bits, one scale for each block of 64 positions and KV head.  `lengths` (device, int32):
+    the positions that every sequence holds in front of a call's rows; `starts` (device, int32, one more than sequences): which rows are whose,
+    None for one row a sequence."""
+
+    BLOCK = 64
+
+    def __init__(self, ctx: "Context", sequences: int, max_len: int, kv_heads: int, head_dim: int):
+        self.ctx, self.h = ctx, None
+        self.sequences, self.max_len, self.kv_heads, self.head_dim = sequences, max_len, kv_heads, head_dim
+        h = _vp()
+        ctx._check(lib().loom_b200_kv8_create(ctx.h, sequences, max_len, kv_heads, head_dim, C.byref(h)))
+        self.h = h
+
+    def append(self, rows, lengths, k, v, starts=None, ld=None):
+        self.ctx._check(lib().loom_b200_kv8_append(self.ctx.h, self.h, rows, _ptr(starts), _ptr(lengths), _ptr(k), _ptr(v), self.kv_heads * self.head_dim if ld is None else ld))
+
+    def read(self, rows, lengths, k, v, starts=None):
+        """The rows of that append as the cache holds them, into k and v."""
+        self.ctx._check(lib().loom_b200_kv8_read(self.ctx.h, self.h, rows, _ptr(starts), _ptr(lengths), _ptr(k), _ptr(v)))
+
+    def attend(self, rows, heads, lengths, q, out, starts=None, scale=0.0, ldq=None):
+        """Causal attention of the rows that an append with the same starts and lengths has added."""
+        self.ctx._check(lib().loom_b200_kv8_attend(self.ctx.h, self.h, rows, heads, _ptr(starts), _ptr(lengths), _ptr(q), heads * self.head_dim if ldq is None else ldq,
+                                                   float(scale), _ptr(out)))
+
+    def free(self):
+        if self.h:
+            if self.ctx.h:
+                lib().loom_b200_kv8_free(self.ctx.h, self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class Decoder:
     """A decoder on the device: the ternary stack (InitHFDecoderBlocks + Transformer stand-in), or with `Decoder.stack` layers that
     are given one by one (`set_layer`)."""
@@ -678,6 +772,16 @@ class Decoder:
         out = np.zeros((self.batch, n), np.int32)
         self.ctx._check(lib().loom_b200_decoder_read_tokens_batch(self.h, out.ctypes.data, n))
         return out
+
+    def sample(self, uniform, temperature=None, top_k=None, top_p=None, min_p=None, seq: int = -1):
+        """Draws from the logits of the last forward, with random numbers 0 <= uniform < 1: (tokens, log probabilities), of one sequence or
+        (seq -1) of every one.  Settings are one number for all, or one a sequence."""
+        n = 1 if seq >= 0 else self.batch
+        full = lambda v, kind: None if v is None else np.ascontiguousarray(np.broadcast_to(np.asarray(v, kind), (n,)))  # noqa: E731
+        u, t, k, p, m = full(uniform, np.float32), full(temperature, np.float32), full(top_k, np.int32), full(top_p, np.float32), full(min_p, np.float32)
+        tokens, logprob = np.empty(n, np.int32), np.empty(n, np.float32)
+        self.ctx._check(lib().loom_b200_decoder_sample(self.h, seq, _hp(t), _hp(k), _hp(p), _hp(m), _hp(u), tokens.ctypes.data, logprob.ctypes.data))
+        return tokens, logprob
 
     def set_kv_offset(self, kv_offset: int):
         """Cuts the sequence back to its first kv_offset positions."""

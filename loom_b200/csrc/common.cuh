@@ -133,6 +133,9 @@ void lb_free_idle_slots();
 // Faults the pages of a pageable buffer in by one call (their contents stay); nothing for memory that CUDA knows.
 void lb_touch_pages(void* p, size_t bytes);
 int lb_ensure_quant_scratch(loom_b200_ctx* ctx, size_t bytes);
+// loom_b200_sample without its checks (sample.cu)
+int lb_launch_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logits, long long stride, const float* temperature, const int32_t* top_k,
+                     const float* top_p, const float* min_p, const float* uniform, int32_t* tokens, float* logprob);
 
 #define LB_CUDA(ctx, expr)                                                                          \
     do {                                                                                            \

@@ -80,6 +80,8 @@ struct loom_b200_decoder {
     int* h_tok_all = nullptr;           // pinned [batch]
     cudaEvent_t read_done[kReadEvents] = {};  // pieces of a logits row on their way to the host; passes of several sequences
     cudaStream_t read_stream = nullptr;  // several sequences: a pass's logits cross the bus beside the next pass
+    uint32_t *draw = nullptr, *h_draw = nullptr;  // sampling: seven words a sequence (settings, random numbers, tokens, logarithms), and their pinned twin
+    int draw_cap = 0;
 };
 
 namespace {
@@ -929,6 +931,8 @@ void loom_b200_decoder_destroy(loom_b200_decoder* dec) {
     if (dec->h_tok) cudaFreeHost(dec->h_tok);
     if (dec->h_tok_all) cudaFreeHost(dec->h_tok_all);
     if (dec->h_logits) cudaFreeHost(dec->h_logits);
+    if (dec->draw) cudaFree(dec->draw);
+    if (dec->h_draw) cudaFreeHost(dec->h_draw);
     for (cudaEvent_t ev : dec->read_done)
         if (ev) cudaEventDestroy(ev);
     if (dec->read_stream) cudaStreamDestroy(dec->read_stream);
@@ -1241,6 +1245,44 @@ int loom_b200_decoder_step_batch(loom_b200_decoder* dec, const int32_t* tokens, 
         LB_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
         return lb_status_result(ctx);
     }
+    return 0;
+}
+
+int loom_b200_decoder_sample(loom_b200_decoder* dec, int seq, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                             const float* uniform, int32_t* tokens, float* logprob) {
+    if (!dec) return lb_fail(nullptr, LOOM_B200_ERR_INVALID, "decoder_sample: decoder is NULL");
+    loom_b200_ctx* ctx = dec->ctx;
+    LB_REQUIRE(ctx, seq >= -1 && seq < dec->batch, "decoder_sample: sequence %d of %d", seq, dec->batch);
+    LB_REQUIRE(ctx, uniform && tokens, "decoder_sample: NULL buffer");
+    if (ctx->capturing) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "decoder_sample takes host buffers and cannot be recorded");
+    const int first = seq < 0 ? 0 : seq, n = seq < 0 ? dec->batch : 1;
+    for (int i = first; i < first + n; ++i)
+        LB_REQUIRE(ctx, (i == dec->lane ? dec->kv_offset : dec->kv_offsets[i]) > 0, "decoder_sample: sequence %d has no prompt behind it", i);
+    if (int rc = lb_set_device(ctx)) return rc;
+    if (n > dec->draw_cap) {
+        if (dec->draw) cudaFree(dec->draw);
+        if (dec->h_draw) cudaFreeHost(dec->h_draw);
+        dec->draw = dec->h_draw = nullptr;
+        dec->draw_cap = 0;
+        LB_CUDA(ctx, cudaMalloc((void**)&dec->draw, (size_t)n * 28));
+        LB_CUDA(ctx, cudaMallocHost((void**)&dec->h_draw, (size_t)n * 28));
+        dec->draw_cap = n;
+    }
+    for (int i = first; i < first + n; ++i)
+        if (int rc = dec_gather_logits(dec, dec->logits_all + (size_t)i * dec->d.vocab)) return rc;
+    uint32_t *h = dec->h_draw, *d = dec->draw;
+    const void* given[] = {uniform, temperature, top_k, top_p, min_p};
+    for (int k = 0; k < 5; ++k)
+        if (given[k]) memcpy(h + (size_t)k * n, given[k], (size_t)n * 4);
+    LB_CUDA(ctx, cudaMemcpyAsync(d, h, (size_t)n * 20, cudaMemcpyHostToDevice, ctx->stream));
+    const auto at = [&](int k) { return given[k] ? (const float*)(d + (size_t)k * n) : nullptr; };
+    if (int rc = lb_launch_sample(ctx, n, dec->d.vocab, dec->logits_all + (size_t)first * dec->d.vocab, dec->d.vocab, at(1), (const int32_t*)at(2), at(3), at(4),
+                                  at(0), (int32_t*)(d + (size_t)5 * n), (float*)(d + (size_t)6 * n)))
+        return rc;
+    LB_CUDA(ctx, cudaMemcpyAsync(h + (size_t)5 * n, d + (size_t)5 * n, (size_t)n * 8, cudaMemcpyDeviceToHost, ctx->stream));
+    if (int rc = lb_sync_checked(ctx)) return rc;
+    memcpy(tokens, h + (size_t)5 * n, (size_t)n * 4);
+    if (logprob) memcpy(logprob, h + (size_t)6 * n, (size_t)n * 4);
     return 0;
 }
 

@@ -1,0 +1,355 @@
+"""The 8-bit cache: what it holds bit for bit, however the rows came, and attention over it against the plain form in 64 bits."""
+import numpy as np
+import pytest
+
+import loom_b200
+import servingkit as kit
+from loom_b200 import LoomB200Error, cabi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = loom_b200.Context(0)
+    yield c
+    c.close()
+
+
+class Cache:
+    """A cache and, on the host, every row that each sequence was given."""
+
+    def __init__(self, ctx, seqs, max_len, kv_heads, dim):
+        self.ctx, self.kv, self.dim, self.heads, self.seqs = ctx, cabi.KV8(ctx, seqs, max_len, kv_heads, dim), dim, kv_heads, seqs
+        self.k = [np.zeros((0, kv_heads, dim), np.float32) for _ in range(seqs)]
+        self.v = [np.zeros((0, kv_heads, dim), np.float32) for _ in range(seqs)]
+        self.held = []
+
+    def dev(self, a):
+        self.held.append(self.ctx.to_device(a))
+        return self.held[-1]
+
+    def drop(self):
+        self.ctx.sync()
+        for b in self.held:
+            self.ctx.free(b)
+        self.held = []
+
+    def lengths(self):
+        return np.array([len(k) for k in self.k], np.int32)
+
+    def append(self, rng, counts, spread=1.0, change=None, step=False, pad=0):
+        """counts[s] random rows to every sequence.  step: one row each without starts; pad: floats between rows.  Returns starts and lengths on
+        the device and the number of rows, for the calls that follow."""
+        counts = np.asarray(counts)
+        rows, width = int(counts.sum()), self.heads * self.dim
+        k, v = rng.standard_normal((rows, self.heads, self.dim)).astype(np.float32) * np.float32(spread), rng.standard_normal((rows, self.heads, self.dim)).astype(np.float32)
+        if change:
+            change(k, v)
+        lengths = self.dev(self.lengths())
+        starts = None if step else self.dev(np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+        wide = [np.full((rows, width + pad), np.nan, np.float32) for _ in "kv"]
+        wide[0][:, :width], wide[1][:, :width] = k.reshape(rows, -1), v.reshape(rows, -1)
+        self.kv.append(rows, lengths, self.dev(wide[0]), self.dev(wide[1]), starts=starts, ld=width + pad)
+        at = 0
+        for s, n in enumerate(counts):
+            self.k[s], self.v[s] = np.concatenate([self.k[s], k[at:at + n]]), np.concatenate([self.v[s], v[at:at + n]])
+            at += n
+        return starts, lengths, rows
+
+    def read(self, starts, lengths, rows):
+        out = [self.dev(np.full((rows, self.heads, self.dim), 9.5, np.float32)) for _ in "kv"]
+        self.kv.read(rows, lengths, *out, starts=starts)
+        return [self.ctx.download(o, (rows, self.heads, self.dim), np.float32) for o in out]
+
+    def check_rows(self, call, counts):
+        got = self.read(*call)
+        at = 0
+        for s, n in enumerate(counts):
+            for g, mine in zip(got, (self.k[s], self.v[s])):
+                want = kit.held(mine, exact=False)[len(mine) - n:]
+                assert np.array_equal(g[at:at + n], want, equal_nan=True), (s, n)
+            at += n
+
+    def attend(self, rng, call, heads, scale=0.0, q=None, pad=0):
+        starts, lengths, rows = call
+        width = heads * self.dim
+        q = rng.standard_normal((rows, heads, self.dim)).astype(np.float32) if q is None else q
+        wide = np.full((rows, width + pad), np.nan, np.float32)
+        wide[:, :width] = q.reshape(rows, -1)
+        out = self.dev(np.full((rows + 1, heads, self.dim), 3.5, np.float32))
+        self.kv.attend(rows, heads, lengths, self.dev(wide), out, starts=starts, scale=scale, ldq=width + pad)
+        got = self.ctx.download(out, (rows + 1, heads, self.dim), np.float32)
+        assert (got[rows] == 3.5).all()
+        return q, got[:rows]
+
+    def check(self, rng, call, counts, heads, scale=0.0, pad=0, want_rows=None):
+        q, got = self.attend(rng, call, heads, scale, pad=pad)
+        at = 0
+        for s, n in enumerate(counts):
+            if n:
+                want, tol = kit.attend(q[at:at + n], kit.held(self.k[s]), kit.held(self.v[s]), len(self.k[s]) - n, scale or None)
+                off = np.abs(got[at:at + n] - want)
+                assert (off <= tol).all(), (s, n, len(self.k[s]), off.max(), (off / tol).max())
+            at += n
+        self.drop()
+        return q, got
+
+
+@pytest.mark.parametrize("dim", [1, 8, 20, 32, 40, 64, 72, 80, 96, 128, 160, 200, 224, 256])
+def test_head_dimensions(ctx, dim):
+    rng = np.random.default_rng(dim)
+    c = Cache(ctx, 3, 400, 2, dim)
+    counts = [130, 64, 7]
+    call = c.append(rng, counts)
+    c.check_rows(call, counts)
+    c.check(rng, call, counts, 6)
+    call = c.append(rng, [1, 1, 1], step=True)
+    c.check_rows(call, [1, 1, 1])
+    c.check(rng, call, [1, 1, 1], 6)
+    call = c.append(rng, [0, 63, 60])
+    c.check_rows(call, [0, 63, 60])
+    c.check(rng, call, [0, 63, 60], 2)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 7, 8, 9, 12, 16, 20])
+def test_query_heads(ctx, group):
+    rng = np.random.default_rng(group)
+    c = Cache(ctx, 2, 600, 3, 64)
+    c.append(rng, [300, 129])
+    c.drop()
+    call = c.append(rng, [1, 1], step=True)
+    c.check(rng, call, [1, 1], 3 * group)
+    call = c.append(rng, [5, 37])
+    c.check(rng, call, [5, 37], 3 * group)
+
+
+@pytest.mark.parametrize("length", [0, 1, 2, 31, 62, 63, 64, 65, 127, 128, 129, 191, 192, 1000])
+def test_lengths(ctx, length):
+    """One row, a step and portions at every place of a block."""
+    rng = np.random.default_rng(length)
+    for counts in ([1], [2], [63], [64], [65], [130]):
+        c = Cache(ctx, 1, length + 140, 2, 32)
+        if length:
+            c.append(rng, [length])
+            c.drop()
+        call = c.append(rng, counts)
+        c.check_rows(call, counts)
+        c.check(rng, call, counts, 4)
+
+
+def test_a_long_sequence(ctx):
+    rng = np.random.default_rng(1)
+    c = Cache(ctx, 1, 20000, 1, 128)
+    c.append(rng, [19000])
+    c.drop()
+    call = c.append(rng, [1], step=True)
+    c.check(rng, call, [1], 4)
+    call = c.append(rng, [40])
+    c.check(rng, call, [40], 4)
+
+
+def test_many_sequences_of_all_lengths(ctx):
+    rng = np.random.default_rng(2)
+    n = 200
+    c = Cache(ctx, n, 700, 2, 40)
+    counts = np.where(rng.random(n) < 0.2, 0, rng.integers(1, 300, n))
+    call = c.append(rng, counts)
+    c.check_rows(call, counts)
+    c.check(rng, call, counts[:0], 2)
+    call = c.append(rng, np.ones(n, int), step=True)
+    c.check_rows(call, np.ones(n, int))
+    c.check(rng, call, np.ones(n, int), 8)
+
+
+def test_however_the_rows_came(ctx):
+    """Row by row, in portions or at once: the same cache bit for bit, and the same attention of the last row."""
+    rng = np.random.default_rng(3)
+    k, v = rng.standard_normal((333, 2, 48)).astype(np.float32), rng.standard_normal((333, 2, 48)).astype(np.float32)
+    q = rng.standard_normal((1, 4, 48)).astype(np.float32)
+    results = []
+    for cuts in (list(range(334)), [0, 333], [0, 1, 64, 65, 190, 192, 300, 333], [0, 63, 127, 128, 332, 333], [0, 332, 333]):
+        c = Cache(ctx, 1, 333, 2, 48)
+        for a, b in zip(cuts, cuts[1:]):
+            def put(kk, vv, a=a, b=b):
+                kk[:], vv[:] = k[a:b], v[a:b]
+            c.append(rng, [b - a], change=put)
+            c.drop()
+        whole = [c.dev(np.array(x, np.int32)) for x in ([0, 333], [0])]
+        rows = c.read(whole[0], whole[1], 333)
+        last = [c.dev(np.array(x, np.int32)) for x in ([0, 1], [332])]
+        results.append((rows[0].view(np.uint32), rows[1].view(np.uint32), c.attend(rng, (last[0], last[1], 1), 4, q=q)[1].view(np.uint32)))
+        c.drop()
+    for r in results[1:]:
+        assert all(np.array_equal(x, y) for x, y in zip(r, results[0]))
+
+
+def test_cut_back_and_go_on(ctx):
+    """A sequence cut back into the block in front of its last one, then given other rows (what a rejected draft does)."""
+    rng = np.random.default_rng(4)
+    for length, back in ((200, 190), (200, 128), (195, 130), (130, 64), (64, 63), (64, 1), (128, 65), (70, 3)):
+        c = Cache(ctx, 1, 400, 2, 32)
+        c.append(rng, [length])
+        c.drop()
+        c.k[0], c.v[0] = c.k[0][:back], c.v[0][:back]
+        call = c.append(rng, [1], step=True)
+        c.check(rng, call, [1], 2)
+        call = c.append(rng, [100])
+        c.check_rows(call, [100])
+        c.check(rng, call, [100], 2)
+
+
+def test_strides_and_scale(ctx):
+    rng = np.random.default_rng(5)
+    for pad in (1, 3, 4, 96):
+        c = Cache(ctx, 2, 300, 2, 24)
+        counts = [150, 70]
+        call = c.append(rng, counts, pad=pad)
+        c.check_rows(call, counts)
+        c.check(rng, call, counts, 4, scale=0.7, pad=pad)
+
+
+def test_values_at_their_ends(ctx):
+    rng = np.random.default_rng(6)
+
+    def change(k, v):
+        k[:64] = 0.0                       # a block of zeros
+        k[64:128, 0] *= np.float32(1e30)   # large, small and tiny blocks
+        v[64:128, 1] *= np.float32(1e-30)
+        v[128:192, 0] = np.float32(1e-42)
+        k[130, 0, 3] = np.float32(50.0)    # an outlier
+        v[192:256] = np.where(v[192:256] > 0, np.float32(1.0), np.float32(-1.0))
+        k[200, 1] = np.float32(0.5) * k[192:256, 1].max() / 127  # half a step
+    c = Cache(ctx, 1, 300, 2, 16)
+    call = c.append(rng, [290], change=change)
+    c.check_rows(call, [290])
+
+
+def test_what_is_not_finite_stays_in_its_block_and_head(ctx):
+    rng = np.random.default_rng(7)
+
+    def change(k, v):
+        k[70, 0, 3] = np.nan    # block 1 of head 0
+        v[130, 1, 2] = np.inf   # block 2 of head 1
+        k[200, 1, 0] = -np.inf  # block 3 of head 1, open
+    c = Cache(ctx, 1, 300, 2, 16)
+    call = c.append(rng, [205], change=change)
+    got_k, got_v = c.read(*call)
+    assert np.isnan(got_k[64:128, 0]).all() and np.isfinite(got_k[64:128, 1]).all() and np.isfinite(got_k[:64]).all() and np.isfinite(got_k[128:192]).all()
+    assert np.isnan(got_v[128:192, 1]).all() and np.isfinite(got_v[128:192, 0]).all()
+    _, out = c.attend(rng, call, 4)
+    bad = ~np.isfinite(out).all(2)  # heads 0, 1 read head 0
+    assert not bad[:64].any()
+    assert bad[64:, :2].all()
+    assert not bad[:128, 2:].any() and bad[128:, 2:].all()
+    c.drop()
+    # a query that is not finite: its own row alone
+    c = Cache(ctx, 1, 300, 2, 16)
+    call = c.append(rng, [100])
+    q = rng.standard_normal((100, 4, 16)).astype(np.float32)
+    q[50, 1, 3], q[60, 2, 0] = np.nan, np.inf
+    _, out = c.attend(rng, call, 4, q=q)
+    bad = ~np.isfinite(out).all(2)
+    assert bad[50, 1] and bad[60, 2] and bad.sum() == 2
+    c.drop()
+
+
+def test_zero_and_large_queries(ctx):
+    rng = np.random.default_rng(8)
+    c = Cache(ctx, 1, 300, 1, 16)
+    call = c.append(rng, [200])
+    q = rng.standard_normal((200, 2, 16)).astype(np.float32)
+    q[:50] = 0.0
+    q[50:100] *= np.float32(1e-30)
+    q[100:150] *= np.float32(30.0)
+    _, out = c.attend(rng, call, 2, q=q)
+    want, tol = kit.attend(q, kit.held(c.k[0]), kit.held(c.v[0]), 0)
+    assert (np.abs(out - want) <= tol).all(), (np.abs(out - want) / tol).max()
+    c.drop()
+
+
+def test_rows_without_room(ctx):
+    """Rows past max_len are not taken, the call's other sequences are; sync says so once."""
+    rng = np.random.default_rng(9)
+    c = Cache(ctx, 3, 100, 1, 16)
+    c.append(rng, [90, 90, 90])
+    c.drop()
+    counts = [10, 11, 5]
+    k = rng.standard_normal((26, 1, 16)).astype(np.float32)
+    starts, lengths = c.dev(np.array([0, 10, 21, 26], np.int32)), c.dev(c.lengths())
+    c.kv.append(26, lengths, c.dev(k), c.dev(k), starts=starts)
+    with pytest.raises(LoomB200Error) as e:
+        ctx.sync()
+    assert e.value.code == cabi.ERR_INVALID and "8-bit cache" in str(e.value)
+    ctx.sync()
+    for s in (0, 2):
+        at = [0, 10, 21][s]
+        c.k[s], c.v[s] = np.concatenate([c.k[s], k[at:at + counts[s]]]), np.concatenate([c.v[s], k[at:at + counts[s]]])
+    q = rng.standard_normal((26, 2, 16)).astype(np.float32)
+    out = c.dev(np.full((26, 2, 16), 3.5, np.float32))
+    c.kv.attend(26, 2, lengths, c.dev(q), out, starts=starts)
+    got = ctx.download(out, (26, 2, 16), np.float32)
+    with pytest.raises(LoomB200Error):
+        ctx.sync()
+    assert (got[10:21] == 0).all()
+    for s, a in ((0, 0), (2, 21)):
+        want, tol = kit.attend(q[a:a + counts[s]], kit.held(c.k[s]), kit.held(c.v[s]), 90)
+        assert (np.abs(got[a:a + counts[s]] - want) <= tol).all()
+    c.drop()
+
+
+def test_starts_that_do_not_ascend_or_pass_the_rows(ctx):
+    rng = np.random.default_rng(10)
+    c = Cache(ctx, 4, 100, 1, 8)
+    k = rng.standard_normal((20, 1, 8)).astype(np.float32)
+    starts, lengths = c.dev(np.array([-3, 5, 2, 8, 99], np.int32)), c.dev(np.zeros(4, np.int32))  # sequences: rows 0-4, none, 2-7, 8-19
+    c.kv.append(20, lengths, c.dev(k), c.dev(k), starts=starts)
+    ctx.sync()
+    out = c.dev(np.zeros((20, 1, 8), np.float32))
+    c.kv.attend(20, 1, lengths, c.dev(k), out, starts=starts)
+    got = ctx.download(out, (20, 1, 8), np.float32)
+    want, tol = kit.attend(k[8:], k[8:].astype(np.float64), k[8:].astype(np.float64), 0)
+    assert (np.abs(got[8:] - want) <= tol).all()
+    ctx.sync()
+    c.drop()
+
+
+def test_frames_and_repeats():
+    """A recorded step replayed with new lengths, beside another frame of the same cache: the same bits as eager calls."""
+    rng = np.random.default_rng(11)
+    ctx = loom_b200.Context(0)
+    try:
+        runs = []
+        for recorded in (False, True):
+            r2 = np.random.default_rng(12)
+            c = Cache(ctx, 5, 2000, 2, 128)
+            c.append(r2, [1500, 3, 700, 64, 1])
+            c.drop()
+            base = c.lengths()
+            steps = [[r2.standard_normal((5, 2, 128)).astype(np.float32) for _ in "kv"] + [r2.standard_normal((5, 8, 128)).astype(np.float32)] for _ in range(6)]
+            lengths, k, v, q, out = c.dev(base), c.dev(steps[0][0]), c.dev(steps[0][1]), c.dev(steps[0][2]), c.dev(np.zeros((5, 8, 128), np.float32))
+
+            def call():
+                c.kv.append(5, lengths, k, v)
+                c.kv.attend(5, 8, lengths, q, out)
+            frames = []
+            if recorded:
+                for _ in range(2):
+                    ctx.graph_begin()
+                    call()
+                    frames.append(ctx.graph_end())
+            got = []
+            for i, (kk, vv, qq) in enumerate(steps):
+                for buf, a in ((lengths, base + i), (k, kk), (v, vv), (q, qq)):
+                    ctx.upload(buf, a.astype(np.int32) if buf == lengths else a)
+                for _ in range(2):  # (a step again is the same step)
+                    ctx.graph_launch(frames[i % 2]) if recorded else call()
+                got.append(ctx.download(out, (5, 8, 128), np.uint32))
+            runs.append(got)
+            for f in frames:
+                ctx.graph_free(f)
+            c.drop()
+            c.kv.free()
+        assert all(np.array_equal(a, b) for a, b in zip(*runs))
+    finally:
+        ctx.close()
