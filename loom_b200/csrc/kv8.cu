@@ -22,14 +22,14 @@
 namespace {
 
 struct Kv8 {
-    int seqs, max_len, heads, dim, blocks, dim_k, dim_v;
+    int seqs, max_len, heads, dim, blocks, dim_k, dim_v, dim_o;
     uint8_t *k, *v;
     float *k_top, *v_top, *k_open, *v_open;
     int* status;
 
     __host__ __device__ size_t head_of(int s, int h) const { return (size_t)s * heads + h; }
     __device__ __forceinline__ float* open_row(float* base, int s, int h, int pos) const {
-        return base + ((head_of(s, h) * 2 + (pos / kKvBlock & 1)) * kKvBlock + pos % kKvBlock) * dim;
+        return base + ((head_of(s, h) * 2 + (pos / kKvBlock & 1)) * kKvBlock + pos % kKvBlock) * dim_o;
     }
 };
 
@@ -177,16 +177,22 @@ __global__ void __launch_bounds__(kApThreads) lb_kv8_read_kernel(const ReadParam
 // Row j of sequence s (head H of the KV head's group) sees positions 0 .. pos + j:  softmax(scale q k) v, the running maximum and
 // sum in one pass, everything but the codes in 32 bits.
 //
-// The products run on the 8-bit integer matrix instruction, codes as they are, exactly: a query row becomes integers q' = round(q 8355711 /
+// The products run on the 8-bit integer matrix instruction, codes as they are, exactly: a query row becomes integers q' = round(q 8355584 /
 // max |q|), written as q' = d0 + 256 d1 + 65536 d2 with digits in -128 .. 127, and a row of softmax weights, relative to the block's
 // own largest score, p' = round(p 16777215) with digits in 0 .. 255.  Three products, one for each digit, make what float32 operands would have
-// given (error 2^-24 of the row's largest), and nothing has to be converted on the side of the cache.
+// given (error 2^-24 of the row's largest), and nothing has to be converted on the side of the cache.  Of the lowest digit's sum the
+// last eight bits are rounded off before the sum becomes a float32, 2^-26 of the largest possible one.
 //
-// Work is a list: sequences, their KV heads, tiles of up to 16 (token, head) rows, blocks.  Every CTA takes an equal stretch of it, so
-// long and short sequences share the device evenly; its four warps take every fourth block.  A tile whose blocks lie in
-// several CTAs' stretches is put together by the one that comes last, in the stretches' order, so results repeat bit for bit.
+// Work is a list: sequences, their KV heads, tiles of (token, head) rows, blocks.  Every CTA takes an equal stretch of it, so long and
+// short sequences share the device evenly.  A tile is either the rows of one warp's MMAs, and the four warps take every fourth block, each
+// through a ring of its own (one token and a few: the cache is read once); or four times that, and the warps share the blocks (portions
+// of a prompt, where reading a block from L2 for every 16 rows would be the bound).  A tile whose blocks lie in several CTAs' stretches
+// is put together by the one that comes last, in the stretches' order, so results repeat bit for bit.
 constexpr int kAtThreads = 128;
 constexpr int kAtWarps = kAtThreads / 32;
+constexpr int kAtSlots = 12;      // of 64 keys or values each: three a warp, or six stages that all share
+constexpr int kAtWideRows = 48;   // rows of a sequence beyond which its tiles are wide
+constexpr int kAtOpenRows = 16;   // rows that go through the open block together
 
 struct AttendParams {
     Kv8 c;
@@ -196,7 +202,8 @@ struct AttendParams {
     long long ldq;
     float* out;
     float scale;    // with log2(e)
-    float* part;    // [ctas][2][tile rows][dim + 2]
+    float* part;    // [ctas][2][largest tile][part_ld]
+    int part_ld;    // dimensions, rounded up to four, largest score, sum, two more
     unsigned* cnt;  // [ctas]
 };
 
@@ -210,8 +217,21 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
                  : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void copy16(void* smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(lb_smem_u32(smem)), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
-constexpr float kQueryMax = 8355711.f;   // 127 (1 + 256 + 65536)
+constexpr float kQueryMax = 8355584.f;  // (three digits reach 127 (1 + 256 + 65536) = 8355711; a product with the row's scale may round up)
 constexpr float kWeightMax = 16777215.f;
 
 // bytes k of four integers as a word
@@ -221,434 +241,657 @@ __device__ __forceinline__ void digit_words(uint32_t x0, uint32_t x1, uint32_t x
     w[1] = __byte_perm(a, b, 0x7632);
     w[2] = __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410);
 }
+// d0 + 256 d1 + 65536 d2, over 256
+__device__ __forceinline__ float digits_sum(int d0, int d1, int d2) { return (float)(d2 * 256 + d1 + ((d0 + 128) >> 8)); }
 
-// HALF: tiles of eight rows (rows 8 .. 15 of the MMAs are zero); NK: 32 dimensions each
-template <int NK, bool HALF>
-struct Shape {
-    static constexpr int kRows = HALF ? 8 : 16;
-    static constexpr int kSets = HALF ? 1 : 2;  // rows g, and g + 8
-    static constexpr int kDimTiles = 4 * NK;
+// SETS: rows of a warp's tile / 8 (with one, rows 8 .. 15 of the MMAs are zero); NK: 32 dimensions each
+template <int NK, int SETS>
+struct AttendShape {
+    static constexpr int kRows = 8 * SETS;              // of a warp
+    static constexpr int kTile = kAtWarps * kRows;      // of a wide tile
+    static constexpr int kSlot = kKvBlock * 32 * NK;    // bytes
+    static constexpr int kLd = 32 * NK + 8;             // floats of a row of partial results (the eight spread rows over banks)
+    static constexpr size_t kMerge = ((size_t)2 * kTile * kLd + (size_t)kAtOpenRows * (kLd + 64)) * 4;
+    static constexpr size_t kSmem = kMerge > (size_t)kAtSlots * kSlot ? kMerge : (size_t)kAtSlots * kSlot;
 };
 
-template <int NK, bool HALF>
+template <int NK, int SETS>
 __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendParams p) {
-    using S = Shape<NK, HALF>;
-    constexpr int R = S::kRows, SETS = S::kSets, NT = S::kDimTiles;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    using S = AttendShape<NK, SETS>;
+    constexpr int RW = S::kRows, NT = 4 * NK, LD = S::kLd, D4 = 8 * NK, STAGES = kAtSlots / 2;
+    extern __shared__ __align__(16) uint8_t ring[];
+    // over the ring, once a tile's blocks are through
+    float* pieces = reinterpret_cast<float*>(ring);  // [4 warps][RW][LD], or [4 RW][LD] of a wide tile
+    float* open_o = pieces + S::kTile * LD;          // [RW or 4 RW][LD] the open block's part
+    float* open_q = open_o + S::kTile * LD;          // [16][LD]
+    float* open_w = open_q + kAtOpenRows * LD;       // [64][16] scores, then weights
+    __shared__ float s_m[kAtWarps + 1][S::kTile], s_l[kAtWarps + 1][S::kTile];
+    __shared__ unsigned s_scan[kAtWarps], s_at;
+    __shared__ int s_seq, s_last;
     const Kv8& c = p.c;
-    const int hd = c.dim;
-    float* qs = reinterpret_cast<float*>(smem_raw);       // [R][32 NK] the tile's query rows, zeros behind the dimension
-    float* acc = qs + R * 32 * NK;                        // [R][32 NK] the tile's result as it is put together
-    float* tail = acc + R * 32 * NK;                      // [R][64] weights of the open block
-    float* st_m = tail + R * 64;                          // [warps + 1][R] largest score (log2) and sum
-    float* st_l = st_m + (kAtWarps + 1) * R;
-    float* qmax = st_l + (kAtWarps + 1) * R;              // [R]
-    long long* work = reinterpret_cast<long long*>(qmax + R);  // [seqs + 1] work in front of every sequence
-    __shared__ long long s_scan[kAtWarps];
-    __shared__ int s_last;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int hd = c.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    lb_pdl_launch_dependents();
+    lb_pdl_wait();
 
-    // blocks (the open one included) that the last row of sequence s sees, and its tiles
-    const auto blocks_of = [&](const Span& a) { return (a.pos + a.count - 1) / kKvBlock + 1; };
-    const auto tiles_of = [&](const Span& a) { return (int)(((long long)a.count * p.group + R - 1) / R); };
-    {
-        long long before = 0;
+    // ---- the list of work ----
+    struct Seq {
+        Span a;
+        int blocks, tiles;  // blocks (the open one included) that its last row sees
+        int cost;           // of a block of a tile: 2^cost
+        unsigned work;
+    };
+    const auto seq_of = [&](int s) {
+        Seq q;
+        q.a = span_of(p.starts, p.lengths, p.rows, s);
+        q.work = 0;
+        if (q.a.count > 0 && fits(c, q.a)) {
+            const int rows = q.a.count * p.group;
+            q.cost = rows > kAtWideRows ? 2 : 0;  // (all four warps work on it)
+            const int per = q.cost ? S::kTile : RW;
+            q.blocks = (q.a.pos + q.a.count - 1) / kKvBlock + 1;
+            q.tiles = (rows + per - 1) / per;
+            q.work = (unsigned)(c.heads * q.tiles * q.blocks) << q.cost;
+        }
+        return q;
+    };
+    unsigned total = 0, before = 0;
+    int s = 0;
+    unsigned first = 0;  // work in front of sequence s
+    unsigned at = 0, stop = 0, share = 0, more = 0;
+    const int me = blockIdx.x;
+    const auto begin_of = [&](int cta) { return share * cta + min((unsigned)cta, more); };
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {  // how much there is, then where this CTA's stretch begins
+        before = 0;
+#pragma unroll 1
         for (int s0 = 0; s0 < c.seqs; s0 += kAtThreads) {
-            const int s = s0 + tid;
-            long long w = 0;
-            if (s < c.seqs) {
-                const Span a = span_of(p.starts, p.lengths, p.rows, s);
-                if (a.count > 0) {
-                    if (fits(c, a)) {
-                        w = (long long)c.heads * tiles_of(a) * blocks_of(a);
-                    } else if (blockIdx.x == 0) {
-                        atomicExch(c.status, 7);
-                        for (long long i = 0; i < (long long)a.count * p.q_heads * hd; ++i) p.out[(size_t)a.row * p.q_heads * hd + i] = 0.f;
-                    }
+            const int i = s0 + tid;
+            unsigned mine = 0;
+            if (i < c.seqs) {
+                const Seq q = seq_of(i);
+                mine = q.work;
+                if (mine == 0 && q.a.count > 0 && pass == 0 && me == 0) {
+                    atomicExch(c.status, 7);
+#pragma unroll 1
+                    for (long long j = 0; j < (long long)q.a.count * p.q_heads * hd; ++j) p.out[(size_t)q.a.row * p.q_heads * hd + j] = 0.f;
                 }
             }
-            long long sum = w;
+            unsigned sum = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const long long u = __shfl_up_sync(0xffffffffu, sum, o);
+                const unsigned u = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += u;
             }
+            __syncthreads();
             if (lane == 31) s_scan[warp] = sum;
             __syncthreads();
-            for (int w2 = 0; w2 < kAtWarps; ++w2) {
-                if (w2 < warp) sum += s_scan[w2];
+            unsigned all = 0;
+#pragma unroll
+            for (int w = 0; w < kAtWarps; ++w) {
+                if (w < warp) sum += s_scan[w];
+                all += s_scan[w];
             }
-            if (s < c.seqs) work[s + 1] = before + sum;
-            for (int w2 = 0; w2 < kAtWarps; ++w2) before += s_scan[w2];
-            __syncthreads();
+            sum += before;
+            if (pass == 1 && mine > 0 && at >= sum - mine && at < sum) {
+                s_seq = i;
+                s_at = sum - mine;
+            }
+            before += all;
+            if (pass == 1 && before > at) break;
         }
-        if (tid == 0) work[0] = 0;
-        __syncthreads();
-    }
-    const long long total = work[c.seqs];
-    const auto begin_of = [&](int cta) { return total * cta / p.ctas; };
-    const int me = blockIdx.x;
-    long long at = begin_of(me);
-    const long long stop = begin_of(me + 1);
-    int s = 0;
-    {
-        int hi = c.seqs;  // the last sequence whose work begins at or in front of `at`
-        while (hi - s > 1) {
-            const int mid = (s + hi) / 2;
-            if (work[mid] <= at) s = mid;
-            else hi = mid;
+        if (pass == 0) {
+            total = before;
+            // stretches of at least a block for every warp
+            const unsigned ctas = min((unsigned)p.ctas, max(1u, total / kAtWarps));
+            share = total / ctas;
+            more = total - share * ctas;
+            at = begin_of(me);
+            stop = begin_of(me + 1);
+            if (me >= (int)ctas || at >= stop) return;
         }
     }
-    while (at < stop) {
-        while (work[s + 1] <= at) ++s;
-        const Span a = span_of(p.starts, p.lengths, p.rows, s);
-        const int blocks = blocks_of(a), tiles = tiles_of(a);
-        const long long unit = (at - work[s]) / blocks, unit0 = work[s] + unit * blocks;
-        const int b0 = (int)(at - unit0), b1 = (int)min((long long)blocks, stop - unit0);
-        const int h = (int)(unit / tiles), tile = (int)(unit % tiles);
-        const int r0 = tile * R, nr = min(R, a.count * p.group - r0);  // rows i = token * group + head
-        const int closed = (a.pos + a.count) / kKvBlock;               // whole blocks
-        const auto pos_of = [&](int r) { return a.pos + (r0 + r) / p.group; };
+    __syncthreads();
+    s = s_seq;
+    first = s_at;
 
-        // query rows
-        __syncthreads();
-        for (int i = tid; i < R * 32 * NK; i += kAtThreads) {
-            const int r = i / (32 * NK), d = i % (32 * NK);
-            float f = 0.f;
-            if (r < nr && d < hd) f = p.q[(size_t)(a.row + (r0 + r) / p.group) * p.ldq + (size_t)(h * p.group + (r0 + r) % p.group) * hd + d];
-            qs[i] = f;
-            acc[i] = 0.f;
+#pragma unroll 1
+    while (true) {
+        const Seq sq = seq_of(s);
+        if (sq.work == 0 || at >= first + sq.work) {
+            first += sq.work;
+            ++s;
+            continue;
         }
-        __syncthreads();
-        for (int r = warp; r < R; r += kAtWarps) {
-            float m = 0.f, odd = 0.f;
-            for (int d = lane; d < 32 * NK; d += 32) {
-                m = fmaxf(m, fabsf(qs[r * 32 * NK + d]));
-                odd += qs[r * 32 * NK + d] * 0.f;  // (not a number, from one or an infinity)
+        const Span& a = sq.a;
+        const bool wide = sq.cost != 0;
+        const int blocks = sq.blocks;
+        const unsigned unit_work = (unsigned)blocks << sq.cost;
+        const int unit = (int)((at - first) / unit_work);
+        const unsigned unit0 = first + unit * unit_work;
+        // a block is the stretch's that its first bit of work lies in
+        const auto block_at = [&](unsigned x) { return (int)((x - unit0 + (1u << sq.cost) - 1) >> sq.cost); };
+        const int b0 = block_at(at), b1 = min(blocks, block_at(min(stop, unit0 + unit_work)));
+        at = min(stop, unit0 + unit_work);
+        const int h = unit / sq.tiles, r0 = (unit - h * sq.tiles) * (wide ? S::kTile : RW);
+        const int nr = min(wide ? S::kTile : RW, a.count * p.group - r0);  // rows i = token * group + head
+        const int closed = (a.pos + a.count) / kKvBlock;                   // whole blocks
+        const auto pos_of = [&](int r) { return a.pos + (r0 + r) / p.group; };
+        // a row of queries or of the result: its first value, rows `ld` apart
+        const auto row_at = [&](int r, long long ld) { return (size_t)(a.row + (r0 + r) / p.group) * ld + (size_t)(h * p.group + (r0 + r) % p.group) * hd; };
+        const bool q_wide = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)p.ldq * 4 | (uintptr_t)hd * 4) & 15) == 0;
+        // `n` rows of queries from the tile's row r on, zeros behind their ends, by threads from, from + step, ...
+        const auto stage_queries = [&](float* to, int ld, int r, int n, int from, int step) {
+#pragma unroll 1
+            for (int i = from; i < n * D4; i += step) {
+                const int k = i / D4, d = (i - k * D4) * 4;
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r + k < nr) {
+                    const float* src = p.q + row_at(r + k, p.ldq) + d;
+                    if (q_wide) {
+                        if (d < hd) f = __ldg(reinterpret_cast<const float4*>(src));
+                    } else {
+                        if (d < hd) f.x = __ldg(src);
+                        if (d + 1 < hd) f.y = __ldg(src + 1);
+                        if (d + 2 < hd) f.z = __ldg(src + 2);
+                        if (d + 3 < hd) f.w = __ldg(src + 3);
+                    }
+                }
+                *reinterpret_cast<float4*>(to + k * ld + d) = f;
             }
-            m = lb_warp_max(m);
+        };
+        const size_t head = c.head_of(s, h) * c.blocks;
+        const int bend = min(min(b1, closed), pos_of(nr - 1) / kKvBlock + 1);
+        const bool open = b1 == blocks && b0 < b1 && closed < blocks && pos_of(nr - 1) >= closed * kKvBlock;
+        const int n_open = open ? a.pos + a.count - closed * kKvBlock : 0;
+
+        if (b0 < b1) {
+            // ---- copies on their way ----
+            const int vbytes = kKvBlock * c.dim_v;
+            const auto copy_block = [&](uint8_t* to, bool values, int b, int from, int step) {
+                const int bytes = values ? vbytes : S::kSlot;
+                const uint8_t* src = (values ? c.v : c.k) + (head + b) * bytes;
+#pragma unroll 4
+                for (int i = from * 16; i < bytes; i += step * 16) copy16(to + i, src + i);
+            };
+            uint8_t* mine_ring = ring + warp * 3 * S::kSlot;
+            const int bstep = wide ? 1 : kAtWarps, bfirst = wide ? b0 : b0 + warp;
+            // split: keys, values, keys, ... of this warp's blocks into its three slots; wide: a block into the next two of twelve
+            int ask_b = bfirst, ask_slot = 0;
+            bool ask_v = false;
+            const auto ask = [&]() {
+                if (ask_b < bend) {
+                    if (wide) copy_block(ring + ask_slot * S::kSlot, false, ask_b, tid, kAtThreads);
+                    copy_block(wide ? ring + (ask_slot + 1) * S::kSlot : mine_ring + ask_slot * S::kSlot, wide || ask_v, ask_b, wide ? tid : lane, wide ? kAtThreads : 32);
+                }
+                copies_commit();
+                if (wide || ask_v) ask_b += bstep;
+                ask_v = !ask_v;
+                ask_slot += wide ? 2 : 1;
+                if (ask_slot == (wide ? kAtSlots : 3)) ask_slot = 0;
+            };
+            __syncthreads();  // (the ring is free)
+#pragma unroll 1
+            for (int i = 0; i < (wide ? STAGES - 2 : 2); ++i) ask();
+            if (open)
+#pragma unroll 1
+                for (int i = tid; i * 32 < n_open * c.dim_o; i += kAtThreads) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(c.open_row(c.k_open, s, h, closed * kKvBlock) + i * 32));
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(c.open_row(c.v_open, s, h, closed * kKvBlock) + i * 32));
+                }
+
+            // ---- query rows as digits, by way of the slots that are asked for last ----
+            const int row0 = wide ? warp * RW : 0;  // this warp's rows in the tile
+            float* mine_q = reinterpret_cast<float*>(wide ? ring + (kAtSlots - 4 + warp) * S::kSlot : mine_ring + 2 * S::kSlot);
+            static_assert(RW * 32 * NK * 4 <= S::kSlot, "a warp's query rows in a slot");
+            stage_queries(mine_q, 32 * NK, row0, RW, lane, 32);
+            __syncwarp();
+            uint32_t qd[3][NK][2 * SETS];
+            float cr[SETS];
+            int see[SETS];  // the row's last position, -1: no row
+            float o[SETS][NT][2], m[SETS], l[SETS];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) odd += __shfl_xor_sync(0xffffffffu, odd, o);
-            if (lane == 0) qmax[r] = m + odd;
-        }
-        __syncthreads();
-        uint32_t qd[3][NK][2 * SETS];
-        float cr[SETS];
-        int see[SETS];  // the row's last position, -1: no row
+            for (int z = 0; z < SETS; ++z) {
+                const int r = g + 8 * z;
+                see[z] = row0 + r < nr ? pos_of(row0 + r) : -1;
+                float top = 0.f, odd = 0.f;
 #pragma unroll
-        for (int z = 0; z < SETS; ++z) {
-            const int r = g + 8 * z;
-            const float top = qmax[r], div = top > 0.f ? top : 1.f;
-            cr[z] = p.scale * top / (kQueryMax * 127.f);
-            see[z] = r < nr ? pos_of(r) : -1;
+                for (int i = 0; i < 2 * NK; ++i) {
+                    const float4 f = *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + 16 * i + 4 * t);
+                    top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
+                    odd += (f.x + f.y) * 0.f + (f.z + f.w) * 0.f;  // (not a number, from one or an infinity)
+                }
 #pragma unroll
-            for (int kk = 0; kk < NK; ++kk) {
-                const int d0 = (kk >> 1) * 64 + ((NK & 1) && kk == NK - 1 ? 8 * t : 16 * t + 8 * (kk & 1));
+                for (int x = 1; x < 4; x <<= 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    odd += __shfl_xor_sync(0xffffffffu, odd, x);
+                }
+                // two factors: one alone would overflow for the smallest rows
+                const float half_mul = top > 0.f ? exp2f(-floorf(log2f(top))) : 1.f, mul = __fdiv_rn(kQueryMax, top > 0.f ? top * half_mul : 1.f);
+                cr[z] = p.scale * top * 256.f / (kQueryMax * 127.f);
+                m[z] = -CUDART_INF_F;
+                l[z] = odd;  // 0, or not a number
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t digits[4];
+                for (int i = 0; i < 2 * NK; ++i) {
+                    const int d = (i >> 2) * 64 + ((NK & 1) && i >= 2 * NK - 2 ? 8 * t + 4 * (i & 1) : 16 * t + 4 * (i & 3));
+                    const float4 f = *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + d);
+                    const float e4[4] = {f.x, f.y, f.z, f.w};
+                    uint32_t digits[4], w[3];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        int v = __float2int_rn(__fdiv_rn(qs[r * 32 * NK + d0 + 4 * half + e], div) * kQueryMax);
-                        const int l0 = ((v + 128) & 255) - 128;
-                        v = (v - l0) >> 8;
-                        const int l1 = ((v + 128) & 255) - 128;
-                        v = (v - l1) >> 8;
-                        digits[e] = (l0 & 255) | (l1 & 255) << 8 | (v & 255) << 16;
+                        // v = d0 + 256 d1 + 65536 d2 with bytes of either sign: each but the last takes what it is over 127 into the next
+                        const int v = __float2int_rn(e4[e] * half_mul * mul);
+                        digits[e] = (uint32_t)(v + 0x8080) ^ 0x8080u;
                     }
-                    uint32_t w[3];
                     digit_words(digits[0], digits[1], digits[2], digits[3], w);
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) qd[k][kk][2 * z + half] = w[k];
+                    for (int k = 0; k < 3; ++k) qd[k][i >> 1][2 * z + (i & 1)] = w[k];
                 }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) o[z][n][0] = o[z][n][1] = 0.f;
             }
-        }
+            const int first_seen = pos_of(min(row0, nr - 1));
+            const int warp_last = row0 < nr ? pos_of(min(row0 + RW, nr) - 1) : -1;
+            if (wide) __syncthreads();  // (another warp's copies may go where this one's queries were)
+            __syncwarp();
+            ask();
 
-        float o[SETS][NT][2], m[SETS], l[SETS];
-#pragma unroll
-        for (int z = 0; z < SETS; ++z) {
-            m[z] = -CUDART_INF_F;
-            l[z] = 0.f;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[z][n][0] = o[z][n][1] = 0.f;
-        }
-        const size_t head = c.head_of(s, h) * c.blocks;
-        const int last_seen = pos_of(nr - 1);
-        const int bend = min(min(b1, closed), last_seen / kKvBlock + 1);
-        for (int b = b0 + warp; b < bend; b += kAtWarps) {
-            const uint8_t* kb = c.k + (head + b) * kKvBlock * c.dim_k;
-            const uint8_t* vb = c.v + (head + b) * kKvBlock * c.dim_v;
-            const float kt = c.k_top[head + b], vt = c.v_top[head + b];
-            float sc[SETS][8][2];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                int d[3][4] = {};
-                const uint8_t* kj = kb + j * 8 * c.dim_k;
-#pragma unroll
-                for (int ch = 0; ch < NK / 2; ++ch) {
-                    const uint4 f = __ldg(reinterpret_cast<const uint4*>(kj + ch * 512 + lane * 16));
-#pragma unroll
-                    for (int k = 0; k < 3; ++k) {
-                        mma_s8(d[k], qd[k][2 * ch][0], SETS == 2 ? qd[k][2 * ch][SETS == 2 ? 2 : 0] : 0u, qd[k][2 * ch][1], SETS == 2 ? qd[k][2 * ch][SETS == 2 ? 3 : 0] : 0u, f.x, f.y);
-                        mma_s8(d[k], qd[k][2 * ch + 1][0], SETS == 2 ? qd[k][2 * ch + 1][SETS == 2 ? 2 : 0] : 0u, qd[k][2 * ch + 1][1],
-                               SETS == 2 ? qd[k][2 * ch + 1][SETS == 2 ? 3 : 0] : 0u, f.z, f.w);
-                    }
-                }
-                if (NK & 1) {
-                    const uint2 f = __ldg(reinterpret_cast<const uint2*>(kj + (NK / 2) * 512 + lane * 8));
-#pragma unroll
-                    for (int k = 0; k < 3; ++k)
-                        mma_s8(d[k], qd[k][NK - 1][0], SETS == 2 ? qd[k][NK - 1][SETS == 2 ? 2 : 0] : 0u, qd[k][NK - 1][1], SETS == 2 ? qd[k][NK - 1][SETS == 2 ? 3 : 0] : 0u, f.x, f.y);
-                }
-#pragma unroll
-                for (int z = 0; z < SETS; ++z)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int i = 2 * z + e;
-                        const float dot = fmaf((float)d[2][i], 65536.f, (float)(d[1][i] * 256 + d[0][i]));
-                        sc[z][j][e] = dot * (cr[z] * kt);
-                    }
+            // ---- block by block: scores and their weights, then the weighted values ----
+            const auto hi = [](const auto& x, int i) -> uint32_t { return SETS == 2 ? x[SETS == 2 ? i : 0] : 0u; };
+            float kt = 0.f, vt = 0.f;
+            if (bfirst < bend) {
+                kt = __ldg(c.k_top + head + bfirst);
+                vt = __ldg(c.v_top + head + bfirst);
             }
-            float mul[SETS];
-            uint32_t pd[3][2][2 * SETS];  // [digit][k step][a0, a2 of rows g, then of rows g + 8]
-            const bool edge = (b + 1) * kKvBlock - 1 > pos_of(0);
+            int slot_at = 0;
+#pragma unroll 1
+            for (int b = bfirst; b < bend; b += bstep) {
+                float kt1 = 0.f, vt1 = 0.f;
+                if (b + bstep < bend) {
+                    kt1 = __ldg(c.k_top + head + b + bstep);
+                    vt1 = __ldg(c.v_top + head + b + bstep);
+                }
+                const uint8_t *kb, *vb;
+                if (wide) {
+                    copies_wait<STAGES - 2>();
+                    __syncthreads();  // block b is there, and nobody reads block b - 1 any more
+                    ask();
+                    kb = ring + slot_at * S::kSlot;
+                    vb = kb + S::kSlot;
+                    slot_at = slot_at == kAtSlots - 2 ? 0 : slot_at + 2;
+                } else {
+                    copies_wait<2>();
+                    __syncwarp();
+                    kb = mine_ring + slot_at * S::kSlot;
+                    slot_at = slot_at == 2 ? 0 : slot_at + 1;
+                    vb = mine_ring + slot_at * S::kSlot;
+                    slot_at = slot_at == 2 ? 0 : slot_at + 1;
+                }
+                const bool works = warp_last >= b * kKvBlock;
+                uint32_t pd[3][2][2 * SETS];  // [digit][k step][a0, a2 of rows g, then of rows g + 8]
+                float mul[SETS];
+                if (works) {
+                    float sc[SETS][8][2];
 #pragma unroll
-            for (int z = 0; z < SETS; ++z) {
-                float mb = -CUDART_INF_F;
+                    for (int j = 0; j < 8; ++j) {
+                        int d[3][4] = {};
+                        const uint8_t* kj = kb + j * (256 * NK);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                        for (int ch = 0; ch < NK / 2; ++ch) {
+                            const uint4 f = *reinterpret_cast<const uint4*>(kj + ch * 512 + lane * 16);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if (edge && b * kKvBlock + 8 * j + 2 * t + e > see[z]) sc[z][j][e] = -CUDART_INF_F;
-                        mb = fmaxf(mb, sc[z][j][e]);
-                    }
-                mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
-                mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
-                const bool any = see[z] >= b * kKvBlock;  // the row sees a part of the block
-                uint32_t sum = 0;
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t q4[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float w = exp2f(sc[z][4 * ks + 2 * half + (e >> 1)][e & 1] - mb);
-                            q4[e] = any ? __float2uint_rn(w * kWeightMax) : 0u;
-                            sum += q4[e];
+                            for (int k = 0; k < 3; ++k) {
+                                mma_s8(d[k], qd[k][2 * ch][0], hi(qd[k][2 * ch], 2), qd[k][2 * ch][1], hi(qd[k][2 * ch], 3), f.x, f.y);
+                                mma_s8(d[k], qd[k][2 * ch + 1][0], hi(qd[k][2 * ch + 1], 2), qd[k][2 * ch + 1][1], hi(qd[k][2 * ch + 1], 3), f.z, f.w);
+                            }
                         }
-                        uint32_t w[3];
-                        digit_words(q4[0], q4[1], q4[2], q4[3], w);
+                        if (NK & 1) {
+                            const uint2 f = *reinterpret_cast<const uint2*>(kj + (NK / 2) * 512 + lane * 8);
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) pd[k][ks][2 * z + half] = w[k];
+                            for (int k = 0; k < 3; ++k) mma_s8(d[k], qd[k][NK - 1][0], hi(qd[k][NK - 1], 2), qd[k][NK - 1][1], hi(qd[k][NK - 1], 3), f.x, f.y);
+                        }
+#pragma unroll
+                        for (int z = 0; z < SETS; ++z)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) sc[z][j][e] = digits_sum(d[0][2 * z + e], d[1][2 * z + e], d[2][2 * z + e]);
                     }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                mul[z] = 0.f;
-                if (any) {
-                    const float mn = fmaxf(m[z], mb);
-                    const float old = exp2f(m[z] - mn);
-                    mul[z] = exp2f(mb - mn) / kWeightMax;
-                    l[z] = fmaf(l[z], old, (float)sum * mul[z]);
-                    if (!(fabsf(kt) <= CUDART_MAX_NORMAL_F)) l[z] = CUDART_NAN_F;
-                    m[z] = mn;
+                    const bool edge = (b + 1) * kKvBlock - 1 > first_seen;
+                    bool same = true;
+                    float old[SETS];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        o[z][n][0] *= old;
-                        o[z][n][1] *= old;
-                    }
-                    mul[z] *= __fdiv_rn(vt, 127.f);
-                }
-            }
+                    for (int z = 0; z < SETS; ++z) {
+                        const float cs = cr[z] * kt;
+                        float mb = -CUDART_INF_F;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (8 * n >= hd) break;
-                const uint4 f = __ldg(reinterpret_cast<const uint4*>(vb + n * 512 + lane * 16));
-                int d[3][4] = {};
-#pragma unroll
-                for (int k = 0; k < 3; ++k) {
-                    mma_u8s8(d[k], pd[k][0][0], SETS == 2 ? pd[k][0][SETS == 2 ? 2 : 0] : 0u, pd[k][0][1], SETS == 2 ? pd[k][0][SETS == 2 ? 3 : 0] : 0u, f.x, f.y);
-                    mma_u8s8(d[k], pd[k][1][0], SETS == 2 ? pd[k][1][SETS == 2 ? 2 : 0] : 0u, pd[k][1][1], SETS == 2 ? pd[k][1][SETS == 2 ? 3 : 0] : 0u, f.z, f.w);
-                }
-#pragma unroll
-                for (int z = 0; z < SETS; ++z)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int i = 2 * z + e;
-                        const float sum = fmaf((float)d[2][i], 65536.f, (float)(d[1][i] * 256 + d[0][i]));
-                        if (see[z] >= b * kKvBlock) o[z][n][e] = fmaf(sum, mul[z], o[z][n][e]);
-                    }
-            }
-        }
-        if (t == 0)
-#pragma unroll
-            for (int z = 0; z < SETS; ++z) {
-                st_m[warp * R + g + 8 * z] = m[z];
-                st_l[warp * R + g + 8 * z] = l[z];
-            }
-
-        // the open block: float32 rows, plain multiply-adds
-        const bool open = b1 == blocks && closed < blocks;
-        const int n_open = open ? a.pos + a.count - closed * kKvBlock : 0;
-        float* om = st_m + kAtWarps * R;
-        float* ol = st_l + kAtWarps * R;
-        if (open) {
-            for (int i = warp; i < n_open; i += kAtWarps) {
-                const float* kr = c.open_row(c.k_open, s, h, closed * kKvBlock + i);
-                for (int r = 0; r < nr; ++r) {
-                    float dot = 0.f;
-                    for (int d = lane; d < hd; d += 32) dot = fmaf(qs[r * 32 * NK + d], kr[d], dot);
-#pragma unroll
-                    for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, x);
-                    if (lane == 0) tail[r * 64 + i] = dot * p.scale;
-                }
-            }
-            __syncthreads();
-            for (int r = warp; r < nr; r += kAtWarps) {
-                const int vis = min(n_open, pos_of(r) - closed * kKvBlock + 1);  // (0 or less: none)
-                const float s0 = lane < vis ? tail[r * 64 + lane] : -CUDART_INF_F, s1 = lane + 32 < vis ? tail[r * 64 + lane + 32] : -CUDART_INF_F;
-                const float top = lb_warp_max(fmaxf(s0, s1));
-                const float w0 = lane < vis ? exp2f(s0 - top) : 0.f, w1 = lane + 32 < vis ? exp2f(s1 - top) : 0.f;
-                float sum = w0 + w1;
-#pragma unroll
-                for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                tail[r * 64 + lane] = w0;
-                tail[r * 64 + lane + 32] = w1;
-                if (lane == 0) {
-                    om[r] = vis > 0 ? top : -CUDART_INF_F;
-                    ol[r] = sum;
-                }
-            }
-            __syncthreads();
-            for (int i = tid; i < nr * hd; i += kAtThreads) {
-                const int r = i / hd, d = i % hd;
-                const int vis = min(n_open, pos_of(r) - closed * kKvBlock + 1);
-                float sum = 0.f;
-                for (int j = 0; j < vis; ++j) sum = fmaf(tail[r * 64 + j], c.open_row(c.v_open, s, h, closed * kKvBlock + j)[d], sum);
-                acc[r * 32 * NK + d] = sum;
-            }
-        } else if (tid < R) {
-            om[tid] = -CUDART_INF_F;
-            ol[tid] = 0.f;
-        }
-        __syncthreads();
-
-        // five partial results of a row into one: acc = sum of o 2^(m - largest m)
-        const auto largest = [&](int r) {
-            float top = om[r];
-            for (int w = 0; w < kAtWarps; ++w) top = fmaxf(top, st_m[w * R + r]);
-            return top;
-        };
-        const auto factor = [](float mine, float top) { return mine == -CUDART_INF_F ? 0.f : exp2f(mine - top); };
-        if (open)
-            for (int i = tid; i < nr * hd; i += kAtThreads) {
-                const int r = i / hd, d = i % hd;
-                const float f = factor(om[r], largest(r));
-                if (om[r] != -CUDART_INF_F) acc[r * 32 * NK + d] *= f;
-            }
-        __syncthreads();
-        for (int w = 0; w < kAtWarps; ++w) {
-            if (w == warp) {
-#pragma unroll
-                for (int z = 0; z < SETS; ++z) {
-                    const int r = g + 8 * z;
-                    if (r < nr && m[z] != -CUDART_INF_F) {
-                        const float f = factor(m[z], largest(r));
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                        for (int j = 0; j < 8; ++j)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                float& x = acc[r * 32 * NK + 8 * n + 2 * t + e];
-                                x = fmaf(o[z][n][e], f, x);
+                                sc[z][j][e] *= cs;
+                                if (edge && b * kKvBlock + 8 * j + 2 * t + e > see[z]) sc[z][j][e] = -CUDART_INF_F;
+                                mb = fmaxf(mb, sc[z][j][e]);
+                            }
+                        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 1));
+                        mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, 2));
+                        const bool any = see[z] >= b * kKvBlock;  // the row sees a part of the block
+                        const float wm = any ? kWeightMax : 0.f;
+                        uint32_t sum = 0;
+#pragma unroll
+                        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                uint32_t q4[4], w[3];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    q4[e] = __float2uint_rn(exp2_of(sc[z][4 * ks + 2 * half + (e >> 1)][e & 1] - mb) * wm);
+                                    sum += q4[e];
+                                }
+                                digit_words(q4[0], q4[1], q4[2], q4[3], w);
+#pragma unroll
+                                for (int k = 0; k < 3; ++k) pd[k][ks][2 * z + half] = w[k];
+                            }
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                        mul[z] = 0.f;
+                        old[z] = 1.f;
+                        if (any) {
+                            const float mn = fmaxf(m[z], mb);
+                            old[z] = m[z] == mn ? 1.f : exp2_of(m[z] - mn);
+                            const float now = exp2_of(mb - mn) * (1.f / kWeightMax);
+                            l[z] = fmaf(l[z], old[z], (float)sum * now);
+                            if (!(fabsf(kt) <= CUDART_MAX_NORMAL_F)) l[z] = CUDART_NAN_F;
+                            m[z] = mn;
+                            mul[z] = now * (256.f / 127.f) * vt;
+                            same = same && old[z] == 1.f;
+                        }
+                    }
+                    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+                        for (int z = 0; z < SETS; ++z)
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                o[z][n][0] *= old[z];
+                                o[z][n][1] *= old[z];
                             }
                     }
                 }
-            }
-            __syncthreads();
-        }
-        const auto sum_of = [&](int r) {
-            const float top = largest(r);
-            float sum = om[r] == -CUDART_INF_F && ol[r] == 0.f ? 0.f : ol[r] * factor(om[r], top);
-            for (int w = 0; w < kAtWarps; ++w)
-                if (st_m[w * R + r] != -CUDART_INF_F || st_l[w * R + r] != 0.f) sum = fmaf(st_l[w * R + r], factor(st_m[w * R + r], top), sum);
-            return sum;
-        };
-        const auto odd_row = [&](int r) { return qmax[r] != qmax[r]; };
-        const auto out_of = [&](int r) { return p.out + ((size_t)(a.row + (r0 + r) / p.group) * p.q_heads + (size_t)h * p.group + (r0 + r) % p.group) * hd; };
-        if (b0 == 0 && b1 == blocks) {
-            for (int i = tid; i < nr * hd; i += kAtThreads) {
-                const int r = i / hd, d = i % hd;
-                out_of(r)[d] = odd_row(r) ? CUDART_NAN_F : __fdiv_rn(acc[r * 32 * NK + d], sum_of(r));
-            }
-        } else {
-            const size_t row_floats = (size_t)hd + 2;
-            const auto slot = [&](int cta, int k) { return p.part + ((size_t)cta * 2 + k) * R * row_floats; };
-            float* mine = slot(me, b0 == 0 ? 1 : 0);  // a stretch begins with a tile's end or middle, and ends with a beginning
-            for (int i = tid; i < nr * (hd + 2); i += kAtThreads) {
-                const int r = i / (hd + 2), d = i % (hd + 2);
-                const float f = d == hd ? largest(r) : d == hd + 1 ? sum_of(r) : acc[r * 32 * NK + d];
-                __stcg(mine + i, f);
-            }
-            __threadfence();
-            __syncthreads();
-            // the CTAs whose stretches this tile lies in
-            int lo = (int)(unit0 * p.ctas / total);
-            while (begin_of(lo + 1) <= unit0) ++lo;
-            while (begin_of(lo) > unit0) --lo;
-            const long long end = unit0 + blocks;
-            int hi = (int)((end - 1) * p.ctas / total);
-            while (begin_of(hi + 1) <= end - 1) ++hi;
-            while (begin_of(hi) > end - 1) --hi;
-            int parts = 0;  // (stretches may be empty)
-            for (int q = lo; q <= hi; ++q) parts += begin_of(q + 1) > begin_of(q);
-            if (tid == 0) {
-                const unsigned old = atomicAdd(p.cnt + lo, 1u);
-                s_last = old + 1 == (unsigned)parts;
-                if (s_last) p.cnt[lo] = 0;
-            }
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                for (int i = tid; i < nr * hd; i += kAtThreads) {
-                    const int r = i / hd, d = i % hd;
-                    float top = -CUDART_INF_F;
-                    for (int q = lo; q <= hi; ++q)
-                        if (begin_of(q + 1) > begin_of(q)) top = fmaxf(top, __ldcg(slot(q, begin_of(q) <= unit0 ? 1 : 0) + r * row_floats + hd));
-                    float x = 0.f, sum = 0.f;
-                    for (int q = lo; q <= hi; ++q) {
-                        if (begin_of(q + 1) <= begin_of(q)) continue;
-                        const float* from = slot(q, begin_of(q) <= unit0 ? 1 : 0) + r * row_floats;
-                        const float mm = __ldcg(from + hd);
-                        if (mm == -CUDART_INF_F && __ldcg(from + hd + 1) == 0.f) continue;
-                        const float f = factor(mm, top);
-                        x = fmaf(__ldcg(from + d), f, x);
-                        sum = fmaf(__ldcg(from + hd + 1), f, sum);
+                if (!wide) {
+                    __syncwarp();
+                    ask();
+                    copies_wait<2>();
+                    __syncwarp();
+                }
+                if (works) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if (8 * n >= hd) break;
+                        const uint4 f = *reinterpret_cast<const uint4*>(vb + n * 512 + lane * 16);
+                        int d[3][4] = {};
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) {
+                            mma_u8s8(d[k], pd[k][0][0], hi(pd[k][0], 2), pd[k][0][1], hi(pd[k][0], 3), f.x, f.y);
+                            mma_u8s8(d[k], pd[k][1][0], hi(pd[k][1], 2), pd[k][1][1], hi(pd[k][1], 3), f.z, f.w);
+                        }
+#pragma unroll
+                        for (int z = 0; z < SETS; ++z)
+                            if (see[z] >= b * kKvBlock) {  // (a scale that is not a number must not meet rows that do not see the block)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) o[z][n][e] = fmaf(digits_sum(d[0][2 * z + e], d[1][2 * z + e], d[2][2 * z + e]), mul[z], o[z][n][e]);
+                            }
                     }
-                    out_of(r)[d] = odd_row(r) ? CUDART_NAN_F : __fdiv_rn(x, sum);
+                }
+                if (!wide) {
+                    __syncwarp();
+                    ask();
+                }
+                kt = kt1;
+                vt = vt1;
+            }
+            copies_wait<0>();
+            __syncthreads();  // the ring is free: partial results take its place
+
+#pragma unroll
+            for (int z = 0; z < SETS; ++z) {
+                const int r = g + 8 * z;
+                float* to = pieces + (size_t)(warp * RW + r) * LD + 2 * t;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(to + 8 * n) = make_float2(o[z][n][0], o[z][n][1]);
+                if (t == 0) {
+                    s_m[wide ? 0 : warp][row0 + r] = m[z];
+                    s_l[wide ? 0 : warp][row0 + r] = l[z];
                 }
             }
+
+            // ---- the open block: float32 rows, plain multiply-adds, 16 rows at a time ----
+            if (open) {
+                const float* ko = c.open_row(c.k_open, s, h, closed * kKvBlock);
+                const float* vo = c.open_row(c.v_open, s, h, closed * kKvBlock);
+#pragma unroll 1
+                for (int g0 = 0; g0 < nr; g0 += kAtOpenRows) {
+                    const int gn = min(kAtOpenRows, nr - g0);
+                    __syncthreads();
+                    stage_queries(open_q, LD, g0, gn, tid, kAtThreads);
+                    __syncthreads();
+#pragma unroll 1
+                    for (int j0 = warp * 8; j0 < n_open; j0 += kAtWarps * 8) {  // a lane: a position (g) and every fourth four dimensions
+                        const float* row = ko + (size_t)min(j0 + g, n_open - 1) * c.dim_o;
+                        float4 f[2 * NK];
+#pragma unroll
+                        for (int i = 0; i < 2 * NK; ++i)
+                            f[i] = 16 * i + 4 * t < c.dim_o ? __ldg(reinterpret_cast<const float4*>(row + 16 * i + 4 * t)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                        for (int r = 0; r < gn; ++r) {
+                            float dot = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 2 * NK; ++i) {
+                                const float4 q = *reinterpret_cast<const float4*>(open_q + r * LD + 16 * i + 4 * t);
+                                dot = fmaf(q.x, f[i].x, fmaf(q.y, f[i].y, fmaf(q.z, f[i].z, fmaf(q.w, f[i].w, dot))));
+                            }
+                            dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+                            dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+                            if (t == 0 && j0 + g < n_open) open_w[(j0 + g) * kAtOpenRows + r] = dot * p.scale;
+                        }
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int r = warp; r < gn; r += kAtWarps) {
+                        const int vis = min(n_open, pos_of(g0 + r) - closed * kKvBlock + 1);  // (0 or less: none)
+                        const float s0 = lane < vis ? open_w[lane * kAtOpenRows + r] : -CUDART_INF_F;
+                        const float s1 = lane + 32 < vis ? open_w[(lane + 32) * kAtOpenRows + r] : -CUDART_INF_F;
+                        const float top = lb_warp_max(fmaxf(s0, s1));
+                        const float w0 = lane < vis ? exp2_of(s0 - top) : 0.f, w1 = lane + 32 < vis ? exp2_of(s1 - top) : 0.f;
+                        float sum = w0 + w1;
+#pragma unroll
+                        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                        open_w[lane * kAtOpenRows + r] = w0;
+                        open_w[(lane + 32) * kAtOpenRows + r] = w1;
+                        if (lane == 0) {
+                            s_m[kAtWarps][g0 + r] = vis > 0 ? top : -CUDART_INF_F;
+                            s_l[kAtWarps][g0 + r] = sum;
+                        }
+                    }
+                    __syncthreads();
+                    const int seen = min(n_open, pos_of(g0 + gn - 1) - closed * kKvBlock + 1);
+#pragma unroll 1
+                    for (int d = tid; d < hd; d += kAtThreads) {
+#pragma unroll 1
+                        for (int r = 0; r < gn; r += 4) {
+                            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                            for (int j = 0; j < seen; ++j) {
+                                const float v = __ldg(vo + (size_t)j * c.dim_o + d);
+                                const float4 w = *reinterpret_cast<const float4*>(open_w + j * kAtOpenRows + r);
+                                // (a row that does not see position j must not meet what is there)
+                                sum.x = w.x != 0.f ? fmaf(w.x, v, sum.x) : sum.x;
+                                sum.y = w.y != 0.f ? fmaf(w.y, v, sum.y) : sum.y;
+                                sum.z = w.z != 0.f ? fmaf(w.z, v, sum.z) : sum.z;
+                                sum.w = w.w != 0.f ? fmaf(w.w, v, sum.w) : sum.w;
+                            }
+                            float* to = open_o + (g0 + r) * LD + d;
+                            to[0] = sum.x;
+                            if (r + 1 < gn) to[LD] = sum.y;
+                            if (r + 2 < gn) to[2 * LD] = sum.z;
+                            if (r + 3 < gn) to[3 * LD] = sum.w;
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+
+            // ---- the pieces into one, and out ----
+            const bool o_wide = (hd & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+            const auto put = [&](int r, int d, float4 x, float sum) {
+                const float inv = __fdiv_rn(1.f, sum);
+                x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+                float* to = p.out + row_at(r, (long long)p.q_heads * hd) + d;
+                if (o_wide) {
+                    *reinterpret_cast<float4*>(to) = x;
+                } else {
+                    to[0] = x.x;
+                    if (d + 1 < hd) to[1] = x.y;
+                    if (d + 2 < hd) to[2] = x.z;
+                    if (d + 3 < hd) to[3] = x.w;
+                }
+            };
+            const auto factor = [](float one, float top) { return one == -CUDART_INF_F ? 0.f : exp2_of(one - top); };
+            const bool done = b0 == 0 && b1 == blocks;
+            const int d4s = (hd + 3) / 4, pieces_n = wide ? 1 : kAtWarps;
+            const auto slot = [&](int cta, int k) { return p.part + ((size_t)cta * 2 + k) * S::kTile * p.part_ld; };
+            float* part = slot(me, b0 == 0 ? 1 : 0);  // a stretch begins with a tile's end or middle, and ends with a beginning
+#pragma unroll 1
+            for (int i = tid; i < nr * d4s; i += kAtThreads) {
+                const int r = i / d4s, d = (i - r * d4s) * 4;
+                float top = open ? s_m[kAtWarps][r] : -CUDART_INF_F;
+#pragma unroll 1
+                for (int w = 0; w < pieces_n; ++w) top = fmaxf(top, s_m[w][r]);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                float sum = 0.f;
+#pragma unroll 1
+                for (int w = 0; w < pieces_n + (open ? 1 : 0); ++w) {
+                    const int which = w < pieces_n ? w : kAtWarps;
+                    const float mm = s_m[which][r], f = factor(mm, top);
+                    sum = fmaf(s_l[which][r], f, sum);
+                    if (mm == -CUDART_INF_F) continue;
+                    const float4 v = *reinterpret_cast<const float4*>((w < pieces_n ? pieces + w * RW * LD : open_o) + r * LD + d);
+                    x.x = fmaf(v.x, f, x.x);
+                    x.y = fmaf(v.y, f, x.y);
+                    x.z = fmaf(v.z, f, x.z);
+                    x.w = fmaf(v.w, f, x.w);
+                }
+                if (done) {
+                    put(r, d, x, sum);
+                } else {
+                    __stcg(reinterpret_cast<float4*>(part + (size_t)r * p.part_ld + d), x);
+                    if (d == 0) __stcg(reinterpret_cast<float2*>(part + (size_t)r * p.part_ld + 4 * d4s), make_float2(top, sum));
+                }
+            }
+            if (!done) {
+                __threadfence();
+                __syncthreads();
+                // the CTAs whose stretches hold blocks of this tile: this one, and its neighbours as far as the tile goes
+                const auto takes = [&](int q) { return block_at(max(begin_of(q), unit0)) < min(blocks, block_at(min(begin_of(q + 1), unit0 + unit_work))); };
+                int lo = me, last = me;
+#pragma unroll 1
+                while (begin_of(lo) > unit0) --lo;
+#pragma unroll 1
+                while (begin_of(last + 1) < unit0 + unit_work) ++last;
+                if (warp == 0) {
+                    unsigned parts = 0;
+#pragma unroll 1
+                    for (int q = lo + lane; q <= last; q += 32) parts += takes(q);
+                    parts = __reduce_add_sync(0xffffffffu, parts);
+                    if (lane == 0) {
+                        s_last = atomicAdd(p.cnt + lo, 1u) + 1 == parts;
+                        if (s_last) p.cnt[lo] = 0;
+                    }
+                }
+                __syncthreads();
+                if (s_last) {
+                    __threadfence();
+                    float* fs = pieces;  // [lo .. last][nr] largest scores, then factors
+                    const auto stat = [&](int q, int r, int k) { return __ldcg(slot(q, q == lo ? 1 : 0) + (size_t)r * p.part_ld + 4 * d4s + k); };
+#pragma unroll 1
+                    for (int i = tid; i < (last - lo + 1) * nr; i += kAtThreads) {
+                        const int q = lo + i / nr, r = i - (q - lo) * nr;
+                        fs[i] = takes(q) ? stat(q, r, 0) : -CUDART_INF_F;
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int r = warp; r < nr; r += kAtWarps) {
+                        float top = -CUDART_INF_F, sum = 0.f;
+#pragma unroll 1
+                        for (int q = lane; q <= last - lo; q += 32) top = fmaxf(top, fs[q * nr + r]);
+                        top = lb_warp_max(top);
+#pragma unroll 1
+                        for (int q = lane; q <= last - lo; q += 32) {
+                            const float f = factor(fs[q * nr + r], top);
+                            fs[q * nr + r] = f;
+                            if (takes(lo + q)) sum = fmaf(stat(lo + q, r, 1), f, sum);
+                        }
+#pragma unroll
+                        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                        if (lane == 0) s_l[0][r] = sum;
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int i = tid; i < nr * d4s; i += kAtThreads) {
+                        const int r = i / d4s, d = (i - r * d4s) * 4;
+                        const float* from = slot(lo, 0) + (size_t)r * p.part_ld + d;
+                        const size_t step = (size_t)2 * S::kTile * p.part_ld;
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                        for (int q = 0; q <= last - lo; ++q) {
+                            const float f = fs[q * nr + r];
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(q == 0 ? from + step / 2 : from + q * step));
+                            // (what a CTA without blocks of the tile, or a row that sees none of them, has left there does not count)
+                            x.x = f != 0.f ? fmaf(v.x, f, x.x) : x.x;
+                            x.y = f != 0.f ? fmaf(v.y, f, x.y) : x.y;
+                            x.z = f != 0.f ? fmaf(v.z, f, x.z) : x.z;
+                            x.w = f != 0.f ? fmaf(v.w, f, x.w) : x.w;
+                        }
+                        put(r, d, x, s_l[0][r]);
+                    }
+                }
+                __syncthreads();
+            }
         }
-        at = unit0 + b1;
+        if (at >= stop) break;
     }
 }
 
 Kv8 view(const loom_b200_kv8* c) {
-    return {c->seqs, c->max_len, c->heads, c->dim, c->blocks, c->dim_k, c->dim_v, c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->ctx->status_dev};
+    return {c->seqs, c->max_len, c->heads, c->dim, c->blocks, c->dim_k, c->dim_v, c->dim_o, c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->ctx->status_dev};
 }
 
 }  // namespace
 
-template <int NK, bool HALF>
-static int launch_attend(loom_b200_ctx* ctx, const AttendParams& p) {
-    using S = Shape<NK, HALF>;
-    const size_t smem = (size_t)S::kRows * (2 * 32 * NK + 64 + 2 * (kAtWarps + 1) + 1) * 4 + (size_t)(p.c.seqs + 1) * 8;
-    LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_attend_kernel<NK, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    lb_kv8_attend_kernel<NK, HALF><<<p.ctas, kAtThreads, smem, ctx->stream>>>(p);
-    LB_CHECK_LAUNCH(ctx, "lb_kv8_attend_kernel");
+template <typename P>
+static cudaError_t launch_pdl(loom_b200_ctx* ctx, void (*kern)(P), dim3 grid, int threads, size_t smem, const P& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->opt_pdl ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+constexpr int kAtMostCtasPerSm = 2;
+
+template <int NK, int SETS>
+static int launch_attend(loom_b200_ctx* ctx, AttendParams p) {
+    using S = AttendShape<NK, SETS>;
+    p.ctas = ctx->sm_count * (S::kSmem <= 110 * 1024 ? kAtMostCtasPerSm : 1);
+    p.part = (float*)((uint8_t*)p.cnt + (size_t)ctx->sm_count * kAtMostCtasPerSm * 4 / 16 * 16 + 16);
+    const size_t factors = (size_t)p.ctas * S::kTile * 4, smem = factors > S::kSmem ? factors : S::kSmem;
+    LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_attend_kernel<NK, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    LB_CUDA(ctx, launch_pdl(ctx, lb_kv8_attend_kernel<NK, SETS>, dim3(p.ctas), kAtThreads, smem, p));
+    ctx->launches++;
     return 0;
 }
 
-constexpr int kAtCtasPerSm = 2;
 constexpr int kKvMaxSeqs = 4096;
 
 extern "C" {
@@ -671,9 +914,10 @@ int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_
     c->blocks = max_len / kKvBlock > 0 ? max_len / kKvBlock : 1;
     c->dim_k = (head_dim + 31) / 32 * 32;
     c->dim_v = (head_dim + 7) / 8 * 8;
-    const size_t blocks = (size_t)sequences * kv_heads * c->blocks, open = (size_t)sequences * kv_heads * 2 * kKvBlock * head_dim * 4;
-    const size_t ctas = (size_t)ctx->sm_count * kAtCtasPerSm;
-    c->work_bytes = ctas * 2 * 16 * (head_dim + 2) * 4 + ctas * 4;
+    c->dim_o = (head_dim + 3) / 4 * 4;
+    const size_t blocks = (size_t)sequences * kv_heads * c->blocks, open = (size_t)sequences * kv_heads * 2 * kKvBlock * c->dim_o * 4;
+    const size_t ctas = (size_t)ctx->sm_count * kAtMostCtasPerSm;
+    c->work_bytes = ctas * 4 + 32 + ctas * 2 * AttendShape<4, 2>::kTile * ((head_dim + 3) / 4 * 4 + 4) * 4;
     cudaError_t e = cudaSuccess;
     const auto get = [&](void** p, size_t bytes) {
         if (e == cudaSuccess) e = cudaMalloc(p, bytes);
@@ -686,6 +930,8 @@ int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_
     get((void**)&c->v_open, open);
     get(&c->work, c->work_bytes);
     if (e == cudaSuccess) e = cudaMemsetAsync(c->work, 0, c->work_bytes, ctx->stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->k_open, 0, open, ctx->stream);  // (what rounds a row's dimensions up stays zero)
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->v_open, 0, open, ctx->stream);
     if (e != cudaSuccess) {
         loom_b200_kv8_free(ctx, c);
         return lb_fail(ctx, LOOM_B200_ERR_CUDA, "kv8_create: %d sequences of %d positions: %s", sequences, max_len, cudaGetErrorString(e));
@@ -750,26 +996,29 @@ int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, int hea
     p.q_heads = heads;
     p.group = heads / c->heads;
     LB_REQUIRE(ctx, (long long)rows * p.group < (1 << 30), "kv8_attend: %d rows of %d heads", rows, heads);
+    // the list of work is counted in 32 bits: blocks of tiles of eight rows, as if every sequence were full
+    if ((double)c->heads * (c->blocks + 1) * ((double)rows * p.group / 8 + 8.0 * c->seqs) >= 4294967296.0)
+        return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_attend: %d rows of %d heads over sequences of up to %d positions: fewer rows a call", rows, heads, c->max_len);
     if (int rc = lb_set_device(ctx)) return rc;
-    p.ctas = ctx->sm_count * kAtCtasPerSm;
     p.starts = starts;
     p.lengths = lengths;
     p.q = q;
     p.ldq = ldq;
     p.out = out;
     p.scale = (float)((scale > 0 ? scale : 1.0 / sqrt((double)c->dim)) * 1.4426950408889634);
-    p.part = (float*)c->work;
-    p.cnt = (unsigned*)(p.part + (size_t)p.ctas * 2 * 16 * (c->dim + 2));
-    const bool half = !starts && p.group <= 8;
+    p.cnt = (unsigned*)c->work;
+    p.part_ld = (c->dim + 3) / 4 * 4 + 4;
+    // tiles of eight rows a warp where sequences have no more on the average (any number is right with either)
+    const bool few = (long long)rows * p.group <= 8LL * (starts ? c->seqs : rows);
     switch (c->dim_k / 32) {
-        case 1: return half ? launch_attend<1, true>(ctx, p) : launch_attend<1, false>(ctx, p);
-        case 2: return half ? launch_attend<2, true>(ctx, p) : launch_attend<2, false>(ctx, p);
-        case 3: return half ? launch_attend<3, true>(ctx, p) : launch_attend<3, false>(ctx, p);
-        case 4: return half ? launch_attend<4, true>(ctx, p) : launch_attend<4, false>(ctx, p);
-        case 5: return launch_attend<5, true>(ctx, p);
-        case 6: return launch_attend<6, true>(ctx, p);
-        case 7: return launch_attend<7, true>(ctx, p);
-        default: return launch_attend<8, true>(ctx, p);
+        case 1: return few ? launch_attend<1, 1>(ctx, p) : launch_attend<1, 2>(ctx, p);
+        case 2: return few ? launch_attend<2, 1>(ctx, p) : launch_attend<2, 2>(ctx, p);
+        case 3: return few ? launch_attend<3, 1>(ctx, p) : launch_attend<3, 2>(ctx, p);
+        case 4: return few ? launch_attend<4, 1>(ctx, p) : launch_attend<4, 2>(ctx, p);
+        case 5: return launch_attend<5, 1>(ctx, p);
+        case 6: return launch_attend<6, 1>(ctx, p);
+        case 7: return launch_attend<7, 1>(ctx, p);
+        default: return launch_attend<8, 1>(ctx, p);
     }
 }
 

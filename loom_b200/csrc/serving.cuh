@@ -9,9 +9,10 @@ struct loom_b200_kv8 {
     int seqs = 0, max_len = 0, heads = 0, dim = 0;
     int blocks = 0;               // per sequence: whole ones that max_len positions can have
     int dim_k = 0, dim_v = 0;     // dimensions of the codes: multiples of 32 and of 8
+    int dim_o = 0;                // of the open rows: a multiple of 4
     uint8_t *k = nullptr, *v = nullptr;      // [seqs][heads][blocks][64 * dim_k or dim_v]
     float *k_top = nullptr, *v_top = nullptr;  // [seqs][heads][blocks] largest |x|
-    float *k_open = nullptr, *v_open = nullptr;  // [seqs][heads][2][64][dim]: rows of the open block and of the one in front, by the block's parity
+    float *k_open = nullptr, *v_open = nullptr;  // [seqs][heads][2][64][dim_o]: rows of the open block and of the one in front, by the block's parity
     void* work = nullptr;         // partial results of attention that several CTAs share, and arrival counters (zero between launches)
     size_t work_bytes = 0;
 };
