@@ -180,31 +180,35 @@ __global__ void __launch_bounds__(kApThreads) lb_kv8_read_kernel(const ReadParam
 // The products run on the 8-bit integer matrix instruction, codes as they are, exactly: a query row becomes integers q' = round(q 8355584 /
 // max |q|), written as q' = d0 + 256 d1 + 65536 d2 with digits in -128 .. 127, and a row of softmax weights, relative to the block's
 // own largest score, p' = round(p 16777215) with digits in 0 .. 255.  Three products, one for each digit, make what float32 operands would have
-// given (error 2^-24 of the row's largest), and nothing has to be converted on the side of the cache.  Of the lowest digit's sum the
-// last eight bits are rounded off before the sum becomes a float32, 2^-26 of the largest possible one.
+// given (error 2^-24 of the row's largest), and nothing has to be converted on the side of the cache.  Put together in float32 they lose what
+// the lowest digit's sum has below 256, 2^-25 of the largest possible sum.
 //
-// Work is a list: sequences, their KV heads, tiles of (token, head) rows, blocks.  Every CTA takes an equal stretch of it, so long and
-// short sequences share the device evenly.  A tile is either the rows of one warp's MMAs, and the four warps take every fourth block, each
-// through a ring of its own (one token and a few: the cache is read once); or four times that, and the warps share the blocks (portions
-// of a prompt, where reading a block from L2 for every 16 rows would be the bound).  A tile whose blocks lie in several CTAs' stretches
-// is put together by the one that comes last, in the stretches' order, so results repeat bit for bit.
+// Work is a list: sequences, their KV heads, tiles of (token, head) rows, blocks.  A tile is either the rows of one warp's MMAs, and the four
+// warps take every fourth block, each through a ring of its own (one token and a few: the cache is read once); or four times that,
+// and the warps share the blocks (portions of a prompt, where reading a block from L2 for every 16 rows would be the bound).  Every CTA
+// finds its place in the list by itself: tiles are cut into parts of nearly equal work, the smallest size with no more parts than CTAs
+// (a part's fixed cost is that of six blocks, so no CTA should have two); where there are more tiles than CTAs, each takes those that
+// begin in its stretch of the work.  The parts of a tile are put together by the CTA that comes last, in their order, so results repeat bit
+// for bit.
 constexpr int kAtThreads = 128;
 constexpr int kAtWarps = kAtThreads / 32;
 constexpr int kAtSlots = 12;      // of 64 keys or values each: three a warp, or six stages that all share
 constexpr int kAtWideRows = 48;   // rows of a sequence beyond which its tiles are wide
+constexpr int kAtSizes = 8;       // sizes of parts that are tried: 1, 1 + 1/8, 1 + 2/8 and so on of an equal share
 constexpr int kAtOpenRows = 16;   // rows that go through the open block together
 
 struct AttendParams {
     Kv8 c;
     int rows, q_heads, group, ctas;
+    unsigned group_inv;  // 2^32 / group, rounded up, for quotients of numbers below 2^16; 0: one head a group
     const int32_t *starts, *lengths;
     const float* q;
     long long ldq;
     float* out;
     float scale;    // with log2(e)
-    float* part;    // [ctas][2][largest tile][part_ld]
+    float* part;    // [2 ctas + 1][largest tile][part_ld]
     int part_ld;    // dimensions, rounded up to four, largest score, sum, two more
-    unsigned* cnt;  // [ctas]
+    unsigned* cnt;  // [2 ctas + 1]
 };
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -241,8 +245,22 @@ __device__ __forceinline__ void digit_words(uint32_t x0, uint32_t x1, uint32_t x
     w[1] = __byte_perm(a, b, 0x7632);
     w[2] = __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410);
 }
-// d0 + 256 d1 + 65536 d2, over 256
-__device__ __forceinline__ float digits_sum(int d0, int d1, int d2) { return (float)(d2 * 256 + d1 + ((d0 + 128) >> 8)); }
+// Accumulators start at the bit pattern of 1.5 2^23, so that a sum of up to 2^22 comes out as the float32 that is larger by as much (the
+// largest here is 256 dimensions x 128 x 127): no conversion, whose pipe takes sixteen values a clock and SM.
+constexpr int kSumBits = 0x4b400000;
+constexpr float kSumFrom = 12582912.f;
+// d0 + 256 d1 + 65536 d2, over 256, of three such sums
+__device__ __forceinline__ float digits_sum(int d0, int d1, int d2) {
+    const float low = fmaf(__int_as_float(d0), 1.f / 256.f, __int_as_float(d1));
+    return fmaf(__int_as_float(d2) - kSumFrom, 256.f, low) - (kSumFrom + kSumFrom / 256.f);
+}
+
+__device__ __forceinline__ void sums_begin(int (&d)[3][4]) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[k][i] = kSumBits;
+}
 
 // SETS: rows of a warp's tile / 8 (with one, rows 8 .. 15 of the MMAs are zero); NK: 32 dimensions each
 template <int NK, int SETS>
@@ -266,7 +284,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
     float* open_q = open_o + S::kTile * LD;          // [16][LD]
     float* open_w = open_q + kAtOpenRows * LD;       // [64][16] scores, then weights
     __shared__ float s_m[kAtWarps + 1][S::kTile], s_l[kAtWarps + 1][S::kTile];
-    __shared__ unsigned s_scan[kAtWarps], s_at;
+    __shared__ unsigned s_scan[kAtWarps][kAtSizes], s_at;
     __shared__ int s_seq, s_last;
     const Kv8& c = p.c;
     const int hd = c.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -294,117 +312,149 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
         }
         return q;
     };
-    unsigned total = 0, before = 0;
-    int s = 0;
-    unsigned first = 0;  // work in front of sequence s
-    unsigned at = 0, stop = 0, share = 0, more = 0;
-    const int me = blockIdx.x;
-    const auto begin_of = [&](int cta) { return share * cta + min((unsigned)cta, more); };
+    const int me = blockIdx.x, chunks = (c.seqs + kAtThreads - 1) / kAtThreads;
+    // all the work, then the number of parts for every size: a lane takes one size and every fourth of its warp's sequences
+    const int my_size = lane % kAtSizes;
+    unsigned total = 0, share = 0, size = 0;
+    bool each = false;  // a part for every CTA, at most
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {  // how much there is, then where this CTA's stretch begins
-        before = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        unsigned v = 0;
 #pragma unroll 1
-        for (int s0 = 0; s0 < c.seqs; s0 += kAtThreads) {
-            const int i = s0 + tid;
-            unsigned mine = 0;
-            if (i < c.seqs) {
-                const Seq q = seq_of(i);
-                mine = q.work;
-                if (mine == 0 && q.a.count > 0 && pass == 0 && me == 0) {
-                    atomicExch(c.status, 7);
+        for (int i = warp * (32 / kAtSizes) + lane / kAtSizes; i < c.seqs; i += kAtThreads / kAtSizes) {
+            const Seq q = seq_of(i);
+            if (pass == 1) {
+                if (q.work) v += c.heads * q.tiles * ((((unsigned)q.blocks << q.cost) + size - 1) / size);
+                continue;
+            }
+            v += q.work;
+            if (q.work == 0 && q.a.count > 0 && me == 0 && my_size == 0) {
+                atomicExch(c.status, 7);
 #pragma unroll 1
-                    for (long long j = 0; j < (long long)q.a.count * p.q_heads * hd; ++j) p.out[(size_t)q.a.row * p.q_heads * hd + j] = 0.f;
-                }
+                for (long long j = 0; j < (long long)q.a.count * p.q_heads * hd; ++j) p.out[(size_t)q.a.row * p.q_heads * hd + j] = 0.f;
             }
-            unsigned sum = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned u = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += u;
-            }
-            __syncthreads();
-            if (lane == 31) s_scan[warp] = sum;
-            __syncthreads();
-            unsigned all = 0;
-#pragma unroll
-            for (int w = 0; w < kAtWarps; ++w) {
-                if (w < warp) sum += s_scan[w];
-                all += s_scan[w];
-            }
-            sum += before;
-            if (pass == 1 && mine > 0 && at >= sum - mine && at < sum) {
-                s_seq = i;
-                s_at = sum - mine;
-            }
-            before += all;
-            if (pass == 1 && before > at) break;
         }
+#pragma unroll
+        for (int o = kAtSizes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        __syncthreads();
+        if (lane < kAtSizes) s_scan[warp][lane] = v;
+        __syncthreads();
+        v = s_scan[0][my_size] + s_scan[1][my_size] + s_scan[2][my_size] + s_scan[3][my_size];
         if (pass == 0) {
-            total = before;
-            // stretches of at least a block for every warp
-            const unsigned ctas = min((unsigned)p.ctas, max(1u, total / kAtWarps));
-            share = total / ctas;
-            more = total - share * ctas;
-            at = begin_of(me);
-            stop = begin_of(me + 1);
-            if (me >= (int)ctas || at >= stop) return;
+            total = v;
+            share = total / p.ctas + 1;
+            size = max((unsigned)kAtWarps, share + (unsigned)((unsigned long long)share * my_size / kAtSizes));
+        } else {
+            const unsigned fits_in = __ballot_sync(0xffffffffu, v <= (unsigned)p.ctas);
+            each = fits_in != 0;
+            size = __shfl_sync(0xffffffffu, size, each ? __ffs(fits_in) - 1 : 0);
+            if (!each) size = (share + 7) / 8 * 8;  // (parts of a cut tile are half of it at least, which their places in p.part go by)
+        }
+    }
+    const auto parts_of = [&](const Seq& q) { return (int)((((unsigned)q.blocks << q.cost) + size - 1) / size); };  // of a tile
+    // the sequence in which this CTA's first part lies, counted in parts (each) or in work
+    const unsigned at = each ? me : (unsigned)((unsigned long long)total * me / p.ctas);
+    const unsigned stop = each ? me + 1 : (unsigned)((unsigned long long)total * (me + 1) / p.ctas);
+    if (tid == 0) s_seq = -1;
+    unsigned before = 0;
+#pragma unroll 1
+    for (int k = 0; k < chunks; ++k) {
+        const int i = k * kAtThreads + tid;
+        unsigned mine = 0;
+        if (i < c.seqs) {
+            const Seq q = seq_of(i);
+            if (q.work) mine = each ? c.heads * q.tiles * parts_of(q) : q.work;
+        }
+        unsigned sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned u = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += u;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp][0] = sum;
+        __syncthreads();
+        unsigned all = 0;
+#pragma unroll
+        for (int w = 0; w < kAtWarps; ++w) {
+            if (w < warp) sum += s_scan[w][0];
+            all += s_scan[w][0];
+        }
+        sum += before;
+        before += all;
+        if (mine > 0 && at >= sum - mine && at < sum) {
+            s_seq = i;
+            s_at = sum - mine;
         }
     }
     __syncthreads();
-    s = s_seq;
-    first = s_at;
+    int s = s_seq;
+    if (s < 0 || at >= stop) return;
+    unsigned first = s_at;  // parts or work in front of sequence s
+    int part_at = -1;       // the part of that sequence, once it is known
 
 #pragma unroll 1
-    while (true) {
+    while (s < c.seqs) {
         const Seq sq = seq_of(s);
-        if (sq.work == 0 || at >= first + sq.work) {
+        const int blocks = sq.blocks, cuts = sq.work ? parts_of(sq) : 1;
+        const unsigned unit_work = (unsigned)blocks << sq.cost;
+        // a tile's blocks from which on a part is the part's
+        const auto block_at = [&](int cut) { return (int)((unsigned)blocks * cut / cuts); };
+        const auto work_at = [&](int part) { return (unsigned)(part / cuts) * unit_work + ((unsigned)block_at(part % cuts) << sq.cost); };
+        if (sq.work && part_at < 0) {
+            part_at = each ? at - first : max(0, (int)((at - first) / unit_work) * cuts);
+#pragma unroll 1
+            while (!each && first + work_at(part_at) < at) ++part_at;
+        }
+        if (sq.work == 0 || part_at >= c.heads * sq.tiles * cuts) {
+            if (each) break;
             first += sq.work;
             ++s;
+            part_at = 0;
             continue;
         }
+        if (!each && first + work_at(part_at) >= stop) break;
         const Span& a = sq.a;
         const bool wide = sq.cost != 0;
-        const int blocks = sq.blocks;
-        const unsigned unit_work = (unsigned)blocks << sq.cost;
-        const int unit = (int)((at - first) / unit_work);
-        const unsigned unit0 = first + unit * unit_work;
-        // a block is the stretch's that its first bit of work lies in
-        const auto block_at = [&](unsigned x) { return (int)((x - unit0 + (1u << sq.cost) - 1) >> sq.cost); };
-        const int b0 = block_at(at), b1 = min(blocks, block_at(min(stop, unit0 + unit_work)));
-        at = min(stop, unit0 + unit_work);
+        const int unit = part_at / cuts, cut = part_at - unit * cuts;
+        const int b0 = block_at(cut), b1 = block_at(cut + 1);
+        // this part's place among the partial results, and the first one's of its tile
+        const auto place_of = [&](int k) { return each ? me - cut + k : (int)(2ull * (first + work_at(unit * cuts + k)) / size); };
+        ++part_at;
         const int h = unit / sq.tiles, r0 = (unit - h * sq.tiles) * (wide ? S::kTile : RW);
         const int nr = min(wide ? S::kTile : RW, a.count * p.group - r0);  // rows i = token * group + head
         const int closed = (a.pos + a.count) / kKvBlock;                   // whole blocks
-        const auto pos_of = [&](int r) { return a.pos + (r0 + r) / p.group; };
+        const int token0 = r0 / p.group, head0 = r0 - token0 * p.group;
+        const auto token_of = [&](int r) { return token0 + (p.group_inv ? (int)__umulhi((unsigned)(head0 + r), p.group_inv) : r); };
+        const auto pos_of = [&](int r) { return a.pos + token_of(r); };
         // a row of queries or of the result: its first value, rows `ld` apart
-        const auto row_at = [&](int r, long long ld) { return (size_t)(a.row + (r0 + r) / p.group) * ld + (size_t)(h * p.group + (r0 + r) % p.group) * hd; };
+        const auto row_at = [&](int r, long long ld) {
+            const int token = token_of(r);
+            return (size_t)(a.row + token) * ld + (size_t)(h * p.group + r0 + r - token * p.group) * hd;
+        };
         const bool q_wide = ((reinterpret_cast<uintptr_t>(p.q) | (uintptr_t)p.ldq * 4 | (uintptr_t)hd * 4) & 15) == 0;
-        // `n` rows of queries from the tile's row r on, zeros behind their ends, by threads from, from + step, ...
+        // `n` rows of queries from the tile's row r on, zeros behind their ends, by threads from, from + step, ...: a group of copies
         const auto stage_queries = [&](float* to, int ld, int r, int n, int from, int step) {
 #pragma unroll 1
             for (int i = from; i < n * D4; i += step) {
                 const int k = i / D4, d = (i - k * D4) * 4;
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r + k < nr) {
-                    const float* src = p.q + row_at(r + k, p.ldq) + d;
-                    if (q_wide) {
-                        if (d < hd) f = __ldg(reinterpret_cast<const float4*>(src));
-                    } else {
-                        if (d < hd) f.x = __ldg(src);
-                        if (d + 1 < hd) f.y = __ldg(src + 1);
-                        if (d + 2 < hd) f.z = __ldg(src + 2);
-                        if (d + 3 < hd) f.w = __ldg(src + 3);
-                    }
+                float* dst = to + k * ld + d;
+                const float* src = p.q + row_at(r + k, p.ldq) + d;
+                if (q_wide && d < hd) {
+                    copy16(dst, src);
+                } else {
+#pragma unroll 1
+                    for (int e = 0; e < 4; ++e) dst[e] = d + e < hd ? __ldg(src + e) : 0.f;
                 }
-                *reinterpret_cast<float4*>(to + k * ld + d) = f;
             }
+            copies_commit();
         };
         const size_t head = c.head_of(s, h) * c.blocks;
         const int bend = min(min(b1, closed), pos_of(nr - 1) / kKvBlock + 1);
-        const bool open = b1 == blocks && b0 < b1 && closed < blocks && pos_of(nr - 1) >= closed * kKvBlock;
+        const bool open = b1 == blocks && closed < blocks && pos_of(nr - 1) >= closed * kKvBlock;
         const int n_open = open ? a.pos + a.count - closed * kKvBlock : 0;
 
-        if (b0 < b1) {
+        {
             // ---- copies on their way ----
             const int vbytes = kKvBlock * c.dim_v;
             const auto copy_block = [&](uint8_t* to, bool values, int b, int from, int step) {
@@ -429,7 +479,11 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 ask_slot += wide ? 2 : 1;
                 if (ask_slot == (wide ? kAtSlots : 3)) ask_slot = 0;
             };
+            const int row0 = wide ? warp * RW : 0;  // this warp's rows in the tile
+            float* mine_q = reinterpret_cast<float*>(wide ? ring + (kAtSlots - 4 + warp) * S::kSlot : mine_ring + 2 * S::kSlot);
+            static_assert(RW * 32 * NK * 4 <= S::kSlot, "a warp's query rows in a slot");
             __syncthreads();  // (the ring is free)
+            stage_queries(mine_q, 32 * NK, row0, min(RW, nr - row0), lane, 32);  // (none, if that is negative)
 #pragma unroll 1
             for (int i = 0; i < (wide ? STAGES - 2 : 2); ++i) ask();
             if (open)
@@ -440,10 +494,8 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 }
 
             // ---- query rows as digits, by way of the slots that are asked for last ----
-            const int row0 = wide ? warp * RW : 0;  // this warp's rows in the tile
-            float* mine_q = reinterpret_cast<float*>(wide ? ring + (kAtSlots - 4 + warp) * S::kSlot : mine_ring + 2 * S::kSlot);
-            static_assert(RW * 32 * NK * 4 <= S::kSlot, "a warp's query rows in a slot");
-            stage_queries(mine_q, 32 * NK, row0, RW, lane, 32);
+            if (wide) copies_wait<STAGES - 2>();
+            else copies_wait<2>();
             __syncwarp();
             uint32_t qd[3][NK][2 * SETS];
             float cr[SETS];
@@ -452,11 +504,13 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
 #pragma unroll
             for (int z = 0; z < SETS; ++z) {
                 const int r = g + 8 * z;
-                see[z] = row0 + r < nr ? pos_of(row0 + r) : -1;
+                const bool is = row0 + r < nr;
+                see[z] = is ? pos_of(row0 + r) : -1;
+                const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
                 float top = 0.f, odd = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * NK; ++i) {
-                    const float4 f = *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + 16 * i + 4 * t);
+                    const float4 f = is ? *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + 16 * i + 4 * t) : none;
                     top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
                     odd += (f.x + f.y) * 0.f + (f.z + f.w) * 0.f;  // (not a number, from one or an infinity)
                 }
@@ -473,7 +527,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
 #pragma unroll
                 for (int i = 0; i < 2 * NK; ++i) {
                     const int d = (i >> 2) * 64 + ((NK & 1) && i >= 2 * NK - 2 ? 8 * t + 4 * (i & 1) : 16 * t + 4 * (i & 3));
-                    const float4 f = *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + d);
+                    const float4 f = is ? *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + d) : none;
                     const float e4[4] = {f.x, f.y, f.z, f.w};
                     uint32_t digits[4], w[3];
 #pragma unroll
@@ -533,7 +587,8 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                     float sc[SETS][8][2];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        int d[3][4] = {};
+                        int d[3][4];
+                        sums_begin(d);
                         const uint8_t* kj = kb + j * (256 * NK);
 #pragma unroll
                         for (int ch = 0; ch < NK / 2; ++ch) {
@@ -624,7 +679,8 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                     for (int n = 0; n < NT; ++n) {
                         if (8 * n >= hd) break;
                         const uint4 f = *reinterpret_cast<const uint4*>(vb + n * 512 + lane * 16);
-                        int d[3][4] = {};
+                        int d[3][4];
+                        sums_begin(d);
 #pragma unroll
                         for (int k = 0; k < 3; ++k) {
                             mma_u8s8(d[k], pd[k][0][0], hi(pd[k][0], 2), pd[k][0][1], hi(pd[k][0], 3), f.x, f.y);
@@ -669,6 +725,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                     const int gn = min(kAtOpenRows, nr - g0);
                     __syncthreads();
                     stage_queries(open_q, LD, g0, gn, tid, kAtThreads);
+                    copies_wait<0>();
                     __syncthreads();
 #pragma unroll 1
                     for (int j0 = warp * 8; j0 < n_open; j0 += kAtWarps * 8) {  // a lane: a position (g) and every fourth four dimensions
@@ -752,110 +809,123 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 }
             };
             const auto factor = [](float one, float top) { return one == -CUDART_INF_F ? 0.f : exp2_of(one - top); };
-            const bool done = b0 == 0 && b1 == blocks;
+            const bool done = cuts == 1;
             const int d4s = (hd + 3) / 4, pieces_n = wide ? 1 : kAtWarps;
-            const auto slot = [&](int cta, int k) { return p.part + ((size_t)cta * 2 + k) * S::kTile * p.part_ld; };
-            float* part = slot(me, b0 == 0 ? 1 : 0);  // a stretch begins with a tile's end or middle, and ends with a beginning
+            const auto slot = [&](int k) { return p.part + (size_t)place_of(k) * S::kTile * p.part_ld; };
+            float* part = slot(cut);
+            if (tid < nr) {  // a row's largest score and sum, and factors in the place of the pieces' own
+                float top = open ? s_m[kAtWarps][tid] : -CUDART_INF_F, sum = 0.f;
 #pragma unroll 1
+                for (int w = 0; w < pieces_n; ++w) top = fmaxf(top, s_m[w][tid]);
+#pragma unroll 1
+                for (int w = 0; w <= kAtWarps; ++w) {
+                    const bool is = w < pieces_n || (w == kAtWarps && open);
+                    const float f = is ? factor(s_m[w][tid], top) : 0.f;
+                    if (is) sum = fmaf(s_l[w][tid], f, sum);
+                    s_m[w][tid] = f;
+                }
+                s_l[0][tid] = sum;
+                if (!done) __stcg(reinterpret_cast<float2*>(part + (size_t)tid * p.part_ld + 4 * d4s), make_float2(top, sum));
+            }
+            __syncthreads();
+#pragma unroll 2
             for (int i = tid; i < nr * d4s; i += kAtThreads) {
                 const int r = i / d4s, d = (i - r * d4s) * 4;
-                float top = open ? s_m[kAtWarps][r] : -CUDART_INF_F;
-#pragma unroll 1
-                for (int w = 0; w < pieces_n; ++w) top = fmaxf(top, s_m[w][r]);
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                float sum = 0.f;
+                const auto add = [&](const float* from, float f) {
+                    const float4 v = *reinterpret_cast<const float4*>(from + r * LD + d);
+                    // (f is 0 for a piece that has none of the row's positions: what stands there does not count)
+                    x.x = f != 0.f ? fmaf(v.x, f, x.x) : x.x;
+                    x.y = f != 0.f ? fmaf(v.y, f, x.y) : x.y;
+                    x.z = f != 0.f ? fmaf(v.z, f, x.z) : x.z;
+                    x.w = f != 0.f ? fmaf(v.w, f, x.w) : x.w;
+                };
 #pragma unroll 1
-                for (int w = 0; w < pieces_n + (open ? 1 : 0); ++w) {
-                    const int which = w < pieces_n ? w : kAtWarps;
-                    const float mm = s_m[which][r], f = factor(mm, top);
-                    sum = fmaf(s_l[which][r], f, sum);
-                    if (mm == -CUDART_INF_F) continue;
-                    const float4 v = *reinterpret_cast<const float4*>((w < pieces_n ? pieces + w * RW * LD : open_o) + r * LD + d);
-                    x.x = fmaf(v.x, f, x.x);
-                    x.y = fmaf(v.y, f, x.y);
-                    x.z = fmaf(v.z, f, x.z);
-                    x.w = fmaf(v.w, f, x.w);
-                }
-                if (done) {
-                    put(r, d, x, sum);
-                } else {
-                    __stcg(reinterpret_cast<float4*>(part + (size_t)r * p.part_ld + d), x);
-                    if (d == 0) __stcg(reinterpret_cast<float2*>(part + (size_t)r * p.part_ld + 4 * d4s), make_float2(top, sum));
-                }
+                for (int w = 0; w < pieces_n; ++w) add(pieces + w * RW * LD, s_m[w][r]);
+                if (open) add(open_o, s_m[kAtWarps][r]);
+                if (done) put(r, d, x, s_l[0][r]);
+                else __stcg(reinterpret_cast<float4*>(part + (size_t)r * p.part_ld + d), x);
             }
             if (!done) {
                 __threadfence();
                 __syncthreads();
-                // the CTAs whose stretches hold blocks of this tile: this one, and its neighbours as far as the tile goes
-                const auto takes = [&](int q) { return block_at(max(begin_of(q), unit0)) < min(blocks, block_at(min(begin_of(q + 1), unit0 + unit_work))); };
-                int lo = me, last = me;
-#pragma unroll 1
-                while (begin_of(lo) > unit0) --lo;
-#pragma unroll 1
-                while (begin_of(last + 1) < unit0 + unit_work) ++last;
-                if (warp == 0) {
-                    unsigned parts = 0;
-#pragma unroll 1
-                    for (int q = lo + lane; q <= last; q += 32) parts += takes(q);
-                    parts = __reduce_add_sync(0xffffffffu, parts);
-                    if (lane == 0) {
-                        s_last = atomicAdd(p.cnt + lo, 1u) + 1 == parts;
-                        if (s_last) p.cnt[lo] = 0;
-                    }
+                if (tid == 0) {
+                    unsigned* cnt = p.cnt + place_of(0);
+                    s_last = atomicAdd(cnt, 1u) + 1 == (unsigned)cuts;
+                    if (s_last) *cnt = 0;
                 }
                 __syncthreads();
                 if (s_last) {
                     __threadfence();
-                    float* fs = pieces;  // [lo .. last][nr] largest scores, then factors
-                    const auto stat = [&](int q, int r, int k) { return __ldcg(slot(q, q == lo ? 1 : 0) + (size_t)r * p.part_ld + 4 * d4s + k); };
+                    // rows of the parts, some at a time, through shared memory, every copy in flight at once
+                    const int ld = 4 * d4s + 4, room = (int)(S::kSmem / 4) - kAtWarps * 4;
+                    const int per = min(nr, max(1, room / (cuts * (ld + 1))));           // rows of a round
+                    const int fit = min(cuts, room / (per * (ld + 1)));                  // parts of a round: all of them, if one row's fit
+                    float* got = pieces;                  // [fit][per][ld]
+                    float* fs = got + fit * per * ld;     // [fit][per] factors
 #pragma unroll 1
-                    for (int i = tid; i < (last - lo + 1) * nr; i += kAtThreads) {
-                        const int q = lo + i / nr, r = i - (q - lo) * nr;
-                        fs[i] = takes(q) ? stat(q, r, 0) : -CUDART_INF_F;
-                    }
-                    __syncthreads();
-#pragma unroll 1
-                    for (int r = warp; r < nr; r += kAtWarps) {
+                    for (int g0 = 0; g0 < nr; g0 += per) {
+                        const int gn = min(per, nr - g0), row4 = gn * (ld / 4);
+                        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);  // (of the one row of a round, where the parts come in several)
                         float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll 1
-                        for (int q = lane; q <= last - lo; q += 32) top = fmaxf(top, fs[q * nr + r]);
-                        top = lb_warp_max(top);
+                        for (int q0 = 0; q0 < cuts; q0 += fit) {
+                            const int qn = min(fit, cuts - q0);
+                            __syncthreads();
 #pragma unroll 1
-                        for (int q = lane; q <= last - lo; q += 32) {
-                            const float f = factor(fs[q * nr + r], top);
-                            fs[q * nr + r] = f;
-                            if (takes(lo + q)) sum = fmaf(stat(lo + q, r, 1), f, sum);
-                        }
-#pragma unroll
-                        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                        if (lane == 0) s_l[0][r] = sum;
-                    }
-                    __syncthreads();
+                            for (int q = warp; q < qn; q += kAtWarps) {
+                                const float* from = slot(q0 + q) + (size_t)g0 * ld;
+#pragma unroll 4
+                                for (int j = lane; j < row4; j += 32) copy16(got + (q * row4 + j) * 4, from + j * 4);
+                            }
+                            copies_commit();
+                            copies_wait<0>();
+                            __syncthreads();
+                            const float was = top;
+                            if (fit < cuts || tid < gn) {  // a row to a thread; the one row of several rounds to every thread
+                                const int r = fit < cuts ? 0 : tid;
+#pragma unroll 4
+                                for (int q = 0; q < qn; ++q) top = fmaxf(top, got[(q * gn + r) * ld + 4 * d4s]);
+                                const float f0 = factor(was, top);
+                                sum *= f0;
+                                y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
+#pragma unroll 4
+                                for (int q = 0; q < qn; ++q) {
+                                    const float2 ml = *reinterpret_cast<const float2*>(got + (q * gn + r) * ld + 4 * d4s);
+                                    const float f = factor(ml.x, top);
+                                    sum = fmaf(ml.y, f, sum);
+                                    fs[q * gn + r] = f;
+                                }
+                                if (fit >= cuts) s_l[0][r] = sum;
+                            }
+                            __syncthreads();
 #pragma unroll 1
-                    for (int i = tid; i < nr * d4s; i += kAtThreads) {
-                        const int r = i / d4s, d = (i - r * d4s) * 4;
-                        const float* from = slot(lo, 0) + (size_t)r * p.part_ld + d;
-                        const size_t step = (size_t)2 * S::kTile * p.part_ld;
-                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                        for (int q = 0; q <= last - lo; ++q) {
-                            const float f = fs[q * nr + r];
-                            const float4 v = __ldcg(reinterpret_cast<const float4*>(q == 0 ? from + step / 2 : from + q * step));
-                            // (what a CTA without blocks of the tile, or a row that sees none of them, has left there does not count)
-                            x.x = f != 0.f ? fmaf(v.x, f, x.x) : x.x;
-                            x.y = f != 0.f ? fmaf(v.y, f, x.y) : x.y;
-                            x.z = f != 0.f ? fmaf(v.z, f, x.z) : x.z;
-                            x.w = f != 0.f ? fmaf(v.w, f, x.w) : x.w;
+                            for (int i = tid; i < gn * d4s; i += kAtThreads) {
+                                const int r = i / d4s, d = (i - r * d4s) * 4;
+#pragma unroll 4
+                                for (int q = 0; q < qn; ++q) {
+                                    const float f = fs[q * gn + r];
+                                    const float4 v4 = *reinterpret_cast<const float4*>(got + (q * gn + r) * ld + d);
+                                    y.x = f != 0.f ? fmaf(v4.x, f, y.x) : y.x;
+                                    y.y = f != 0.f ? fmaf(v4.y, f, y.y) : y.y;
+                                    y.z = f != 0.f ? fmaf(v4.z, f, y.z) : y.z;
+                                    y.w = f != 0.f ? fmaf(v4.w, f, y.w) : y.w;
+                                }
+                                if (fit < cuts) break;  // (one row has 64 groups of four dimensions at most: every thread has one of them, or none)
+                                put(g0 + r, d, y, s_l[0][r]);
+                                y = make_float4(0.f, 0.f, 0.f, 0.f);
+                            }
                         }
-                        put(r, d, x, s_l[0][r]);
+                        if (fit < cuts && tid < d4s) put(g0, tid * 4, y, sum);
                     }
                 }
                 __syncthreads();
             }
         }
-        if (at >= stop) break;
+        if (each) break;
     }
 }
+
 
 Kv8 view(const loom_b200_kv8* c) {
     return {c->seqs, c->max_len, c->heads, c->dim, c->blocks, c->dim_k, c->dim_v, c->dim_o, c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->ctx->status_dev};
@@ -884,8 +954,8 @@ template <int NK, int SETS>
 static int launch_attend(loom_b200_ctx* ctx, AttendParams p) {
     using S = AttendShape<NK, SETS>;
     p.ctas = ctx->sm_count * (S::kSmem <= 110 * 1024 ? kAtMostCtasPerSm : 1);
-    p.part = (float*)((uint8_t*)p.cnt + (size_t)ctx->sm_count * kAtMostCtasPerSm * 4 / 16 * 16 + 16);
-    const size_t factors = (size_t)p.ctas * S::kTile * 4, smem = factors > S::kSmem ? factors : S::kSmem;
+    p.part = (float*)((uint8_t*)p.cnt + (2 * (size_t)ctx->sm_count * kAtMostCtasPerSm + 1) * 4 / 16 * 16 + 16);
+    const size_t smem = S::kSmem;
     LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_attend_kernel<NK, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     LB_CUDA(ctx, launch_pdl(ctx, lb_kv8_attend_kernel<NK, SETS>, dim3(p.ctas), kAtThreads, smem, p));
     ctx->launches++;
@@ -917,7 +987,7 @@ int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_
     c->dim_o = (head_dim + 3) / 4 * 4;
     const size_t blocks = (size_t)sequences * kv_heads * c->blocks, open = (size_t)sequences * kv_heads * 2 * kKvBlock * c->dim_o * 4;
     const size_t ctas = (size_t)ctx->sm_count * kAtMostCtasPerSm;
-    c->work_bytes = ctas * 4 + 32 + ctas * 2 * AttendShape<4, 2>::kTile * ((head_dim + 3) / 4 * 4 + 4) * 4;
+    c->work_bytes = (2 * ctas + 1) * 4 + 32 + (2 * ctas + 1) * (head_dim > 128 ? AttendShape<8, 1>::kTile : AttendShape<4, 2>::kTile) * ((head_dim + 3) / 4 * 4 + 4) * 4;
     cudaError_t e = cudaSuccess;
     const auto get = [&](void** p, size_t bytes) {
         if (e == cudaSuccess) e = cudaMalloc(p, bytes);
@@ -996,6 +1066,8 @@ int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, int hea
     p.q_heads = heads;
     p.group = heads / c->heads;
     LB_REQUIRE(ctx, (long long)rows * p.group < (1 << 30), "kv8_attend: %d rows of %d heads", rows, heads);
+    if (p.group > 32768) return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_attend: %d query heads a KV head, 32768 at most", p.group);
+    p.group_inv = p.group > 1 ? (unsigned)((4294967296ull + p.group - 1) / p.group) : 0u;
     // the list of work is counted in 32 bits: blocks of tiles of eight rows, as if every sequence were full
     if ((double)c->heads * (c->blocks + 1) * ((double)rows * p.group / 8 + 8.0 * c->seqs) >= 4294967296.0)
         return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_attend: %d rows of %d heads over sequences of up to %d positions: fewer rows a call", rows, heads, c->max_len);
