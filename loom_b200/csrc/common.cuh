@@ -330,6 +330,8 @@ __device__ __forceinline__ bool lb_mbar_wait_bounded(uint64_t* bar, uint32_t par
 __device__ __forceinline__ void lb_fence_mbar_init() {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
+// Ordinary accesses in front of it against bulk copies behind it, to the same memory.
+__device__ __forceinline__ void lb_fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 // 1-D bulk copy global -> shared through the TMA engine; dst/src 16-byte aligned, bytes % 16 == 0.
 __device__ __forceinline__ void lb_bulk_g2s(void* dst_smem, const void* src_gmem, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(

@@ -192,9 +192,10 @@ __global__ void __launch_bounds__(kApThreads) lb_kv8_read_kernel(const ReadParam
 // for bit.
 constexpr int kAtThreads = 128;
 constexpr int kAtWarps = kAtThreads / 32;
-constexpr int kAtSlots = 12;      // of 64 keys or values each: three a warp, or six stages that all share
 constexpr int kAtWideRows = 48;   // rows of a sequence beyond which its tiles are wide
 constexpr int kAtSizes = 8;       // sizes of parts that are tried: 1, 1 + 1/8, 1 + 2/8 and so on of an equal share
+constexpr int kAtOpenFew = 6;     // what an open block costs, in blocks: beside one token's rows (5.8 us, four blocks 3.4 us)
+constexpr int kAtOpenWide = 3;    // and beside a wide tile's
 constexpr int kAtOpenRows = 16;   // rows that go through the open block together
 
 struct AttendParams {
@@ -255,6 +256,7 @@ __device__ __forceinline__ float digits_sum(int d0, int d1, int d2) {
     return fmaf(__int_as_float(d2) - kSumFrom, 256.f, low) - (kSumFrom + kSumFrom / 256.f);
 }
 
+__device__ __forceinline__ void add_scaled(float4& x, const float4& v, float f) { x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w)); }
 __device__ __forceinline__ void sums_begin(int (&d)[3][4]) {
 #pragma unroll
     for (int k = 0; k < 3; ++k)
@@ -267,25 +269,36 @@ template <int NK, int SETS>
 struct AttendShape {
     static constexpr int kRows = 8 * SETS;              // of a warp
     static constexpr int kTile = kAtWarps * kRows;      // of a wide tile
-    static constexpr int kSlot = kKvBlock * 32 * NK;    // bytes
+    static constexpr int kSlot = kKvBlock * 32 * NK;    // bytes of 64 keys or values
+    // CTAs of an SM, and slots of a warp.  Two CTAs with three slots stream the cache at 5.4 TB/s; three CTAs with two slots each at 4.1 (a
+    // warp then has one copy under way while it computes, and 168 registers).
+    static constexpr int kPerSm = NK > 4 ? 1 : 2;
+    static constexpr int kRing = 3;
+    static constexpr int kSlots = kAtWarps * kRing;             // or pairs of them that all share
     static constexpr int kLd = 32 * NK + 8;             // floats of a row of partial results (the eight spread rows over banks)
-    static constexpr size_t kMerge = ((size_t)2 * kTile * kLd + (size_t)kAtOpenRows * (kLd + 64)) * 4;
-    static constexpr size_t kSmem = kMerge > (size_t)kAtSlots * kSlot ? kMerge : (size_t)kAtSlots * kSlot;
+    static constexpr int kLdOpen = 32 * NK + 16;        // of a key of the open block (two rows of a quarter warp in different banks)
+    static constexpr size_t kMerge = ((size_t)(kTile + kAtOpenRows) * kLd + kKvBlock * kAtOpenRows + kKvBlock / 2 * (kLdOpen + 32 * NK)) * 4;
+    static constexpr size_t kSmem = kMerge > (size_t)kSlots * kSlot ? kMerge : (size_t)kSlots * kSlot;
 };
 
 template <int NK, int SETS>
-__global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_kv8_attend_kernel(const AttendParams p) {
     using S = AttendShape<NK, SETS>;
-    constexpr int RW = S::kRows, NT = 4 * NK, LD = S::kLd, D4 = 8 * NK, STAGES = kAtSlots / 2;
+    constexpr int RW = S::kRows, NT = 4 * NK, LD = S::kLd, D4 = 8 * NK, RING = S::kRing, STAGES = S::kSlots / 2;
     extern __shared__ __align__(16) uint8_t ring[];
     // over the ring, once a tile's blocks are through
     float* pieces = reinterpret_cast<float*>(ring);  // [4 warps][RW][LD], or [4 RW][LD] of a wide tile
-    float* open_o = pieces + S::kTile * LD;          // [RW or 4 RW][LD] the open block's part
-    float* open_q = open_o + S::kTile * LD;          // [16][LD]
+    float* open_q = pieces + S::kTile * LD;          // [16][LD]
     float* open_w = open_q + kAtOpenRows * LD;       // [64][16] scores, then weights
-    __shared__ float s_m[kAtWarps + 1][S::kTile], s_l[kAtWarps + 1][S::kTile];
+    float* open_k = open_w + kKvBlock * kAtOpenRows; // [32][kLdOpen] half of its keys, then of the values, [32][dim_o]
+    float* open_v = open_k + kKvBlock / 2 * S::kLdOpen;  // [32][dim_o] the other half of the values
+    __shared__ float s_m[kAtWarps][S::kTile], s_l[kAtWarps][S::kTile];
+    __shared__ float s_f[2][kAtOpenRows];            // factors of a row's piece and of its open block
+    __shared__ int s_span[kAtThreads][3];            // the first sequences' rows
     __shared__ unsigned s_scan[kAtWarps][kAtSizes], s_at;
     __shared__ int s_seq, s_last;
+    __shared__ __align__(8) uint64_t s_bar;  // copies of parts
+    uint32_t bar_phase = 0;
     const Kv8& c = p.c;
     const int hd = c.dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     lb_pdl_launch_dependents();
@@ -295,12 +308,25 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
     struct Seq {
         Span a;
         int blocks, tiles;  // blocks (the open one included) that its last row sees
+        int load;           // the same, with what the open one costs
         int cost;           // of a block of a tile: 2^cost
         unsigned work;
     };
+    if (tid == 0) {
+        lb_mbar_init(&s_bar, 1);
+        lb_fence_mbar_init();
+    }
+    for (int i = tid; i < min(c.seqs, kAtThreads); i += kAtThreads) {
+        const Span a = span_of(p.starts, p.lengths, p.rows, i);
+        s_span[i][0] = a.row;
+        s_span[i][1] = a.count;
+        s_span[i][2] = a.pos;
+    }
+    __syncthreads();
     const auto seq_of = [&](int s) {
         Seq q;
-        q.a = span_of(p.starts, p.lengths, p.rows, s);
+        if (s < kAtThreads) q.a = {s_span[s][0], s_span[s][1], s_span[s][2]};
+        else q.a = span_of(p.starts, p.lengths, p.rows, s);
         q.work = 0;
         if (q.a.count > 0 && fits(c, q.a)) {
             const int rows = q.a.count * p.group;
@@ -308,7 +334,8 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
             const int per = q.cost ? S::kTile : RW;
             q.blocks = (q.a.pos + q.a.count - 1) / kKvBlock + 1;
             q.tiles = (rows + per - 1) / per;
-            q.work = (unsigned)(c.heads * q.tiles * q.blocks) << q.cost;
+            q.load = q.blocks + ((q.a.pos + q.a.count) % kKvBlock ? (q.cost ? kAtOpenWide : kAtOpenFew) : 0);
+            q.work = (unsigned)(c.heads * q.tiles * q.load) << q.cost;
         }
         return q;
     };
@@ -324,7 +351,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
         for (int i = warp * (32 / kAtSizes) + lane / kAtSizes; i < c.seqs; i += kAtThreads / kAtSizes) {
             const Seq q = seq_of(i);
             if (pass == 1) {
-                if (q.work) v += c.heads * q.tiles * ((((unsigned)q.blocks << q.cost) + size - 1) / size);
+                if (q.work) v += c.heads * q.tiles * ((((unsigned)q.load << q.cost) + size - 1) / size);
                 continue;
             }
             v += q.work;
@@ -351,7 +378,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
             if (!each) size = (share + 7) / 8 * 8;  // (parts of a cut tile are half of it at least, which their places in p.part go by)
         }
     }
-    const auto parts_of = [&](const Seq& q) { return (int)((((unsigned)q.blocks << q.cost) + size - 1) / size); };  // of a tile
+    const auto parts_of = [&](const Seq& q) { return (int)((((unsigned)q.load << q.cost) + size - 1) / size); };  // of a tile
     // the sequence in which this CTA's first part lies, counted in parts (each) or in work
     const unsigned at = each ? me : (unsigned)((unsigned long long)total * me / p.ctas);
     const unsigned stop = each ? me + 1 : (unsigned)((unsigned long long)total * (me + 1) / p.ctas);
@@ -397,10 +424,11 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
     while (s < c.seqs) {
         const Seq sq = seq_of(s);
         const int blocks = sq.blocks, cuts = sq.work ? parts_of(sq) : 1;
-        const unsigned unit_work = (unsigned)blocks << sq.cost;
-        // a tile's blocks from which on a part is the part's
-        const auto block_at = [&](int cut) { return (int)((unsigned)blocks * cut / cuts); };
-        const auto work_at = [&](int part) { return (unsigned)(part / cuts) * unit_work + ((unsigned)block_at(part % cuts) << sq.cost); };
+        const unsigned unit_work = (unsigned)sq.load << sq.cost;
+        // the load from which on it is a part's, and its block: the last part has the open block, whatever its load
+        const auto load_at = [&](int cut) { return (int)((unsigned)sq.load * cut / cuts); };
+        const auto block_at = [&](int cut) { return cut == cuts ? blocks : min(load_at(cut), blocks - 1); };
+        const auto work_at = [&](int part) { return (unsigned)(part / cuts) * unit_work + ((unsigned)load_at(part % cuts) << sq.cost); };
         if (sq.work && part_at < 0) {
             part_at = each ? at - first : max(0, (int)((at - first) / unit_work) * cuts);
 #pragma unroll 1
@@ -463,9 +491,9 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
 #pragma unroll 4
                 for (int i = from * 16; i < bytes; i += step * 16) copy16(to + i, src + i);
             };
-            uint8_t* mine_ring = ring + warp * 3 * S::kSlot;
+            uint8_t* mine_ring = ring + warp * RING * S::kSlot;
             const int bstep = wide ? 1 : kAtWarps, bfirst = wide ? b0 : b0 + warp;
-            // split: keys, values, keys, ... of this warp's blocks into its three slots; wide: a block into the next two of twelve
+            // split: keys, values, keys, ... of this warp's blocks into its slots; wide: a block into the next two of all
             int ask_b = bfirst, ask_slot = 0;
             bool ask_v = false;
             const auto ask = [&]() {
@@ -477,15 +505,40 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 if (wide || ask_v) ask_b += bstep;
                 ask_v = !ask_v;
                 ask_slot += wide ? 2 : 1;
-                if (ask_slot == (wide ? kAtSlots : 3)) ask_slot = 0;
+                if (ask_slot == (wide ? S::kSlots : RING)) ask_slot = 0;
             };
             const int row0 = wide ? warp * RW : 0;  // this warp's rows in the tile
-            float* mine_q = reinterpret_cast<float*>(wide ? ring + (kAtSlots - 4 + warp) * S::kSlot : mine_ring + 2 * S::kSlot);
-            static_assert(RW * 32 * NK * 4 <= S::kSlot, "a warp's query rows in a slot");
-            __syncthreads();  // (the ring is free)
-            stage_queries(mine_q, 32 * NK, row0, min(RW, nr - row0), lane, 32);  // (none, if that is negative)
+            // ---- query rows as digits ----
+            uint32_t qd[3][NK][2 * SETS];
+            float cr[SETS];
+            int see[SETS];  // the row's last position, -1: no row
+            float o[SETS][NT][2], m[SETS], l[SETS];
+            float4 f[SETS][2 * NK];  // (asked for in front of the ring's copies, which keep the memory busy for microseconds)
+#pragma unroll
+            for (int z = 0; z < SETS; ++z) {
+                const int r = g + 8 * z;
+                const bool is = row0 + r < nr;
+                see[z] = is ? pos_of(row0 + r) : -1;
+                const float* src = p.q + row_at(is ? row0 + r : 0, p.ldq);
+#pragma unroll
+                for (int i = 0; i < 2 * NK; ++i) {
+                    const int d = (i >> 2) * 64 + ((NK & 1) && i >= 2 * NK - 2 ? 8 * t + 4 * (i & 1) : 16 * t + 4 * (i & 3));
+                    f[z][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (is && d < hd) {
+                        if (q_wide) {
+                            f[z][i] = __ldg(reinterpret_cast<const float4*>(src + d));
+                        } else {
+                            f[z][i].x = __ldg(src + d);
+                            if (d + 1 < hd) f[z][i].y = __ldg(src + d + 1);
+                            if (d + 2 < hd) f[z][i].z = __ldg(src + d + 2);
+                            if (d + 3 < hd) f[z][i].w = __ldg(src + d + 3);
+                        }
+                    }
+                }
+            }
+            __syncthreads();                        // (the ring is free)
 #pragma unroll 1
-            for (int i = 0; i < (wide ? STAGES - 2 : 2); ++i) ask();
+            for (int i = 0; i < (wide ? STAGES - 1 : RING); ++i) ask();
             if (open)
 #pragma unroll 1
                 for (int i = tid; i * 32 < n_open * c.dim_o; i += kAtThreads) {
@@ -493,26 +546,13 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                     asm volatile("prefetch.global.L2 [%0];" ::"l"(c.open_row(c.v_open, s, h, closed * kKvBlock) + i * 32));
                 }
 
-            // ---- query rows as digits, by way of the slots that are asked for last ----
-            if (wide) copies_wait<STAGES - 2>();
-            else copies_wait<2>();
-            __syncwarp();
-            uint32_t qd[3][NK][2 * SETS];
-            float cr[SETS];
-            int see[SETS];  // the row's last position, -1: no row
-            float o[SETS][NT][2], m[SETS], l[SETS];
 #pragma unroll
             for (int z = 0; z < SETS; ++z) {
-                const int r = g + 8 * z;
-                const bool is = row0 + r < nr;
-                see[z] = is ? pos_of(row0 + r) : -1;
-                const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
                 float top = 0.f, odd = 0.f;
 #pragma unroll
                 for (int i = 0; i < 2 * NK; ++i) {
-                    const float4 f = is ? *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + 16 * i + 4 * t) : none;
-                    top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))), fabsf(f.w));
-                    odd += (f.x + f.y) * 0.f + (f.z + f.w) * 0.f;  // (not a number, from one or an infinity)
+                    top = fmaxf(fmaxf(fmaxf(top, fabsf(f[z][i].x)), fmaxf(fabsf(f[z][i].y), fabsf(f[z][i].z))), fabsf(f[z][i].w));
+                    odd += (f[z][i].x + f[z][i].y) * 0.f + (f[z][i].z + f[z][i].w) * 0.f;  // (not a number, from one or an infinity)
                 }
 #pragma unroll
                 for (int x = 1; x < 4; x <<= 1) {
@@ -526,9 +566,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 l[z] = odd;  // 0, or not a number
 #pragma unroll
                 for (int i = 0; i < 2 * NK; ++i) {
-                    const int d = (i >> 2) * 64 + ((NK & 1) && i >= 2 * NK - 2 ? 8 * t + 4 * (i & 1) : 16 * t + 4 * (i & 3));
-                    const float4 f = is ? *reinterpret_cast<const float4*>(mine_q + r * 32 * NK + d) : none;
-                    const float e4[4] = {f.x, f.y, f.z, f.w};
+                    const float e4[4] = {f[z][i].x, f[z][i].y, f[z][i].z, f[z][i].w};
                     uint32_t digits[4], w[3];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -545,9 +583,6 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
             }
             const int first_seen = pos_of(min(row0, nr - 1));
             const int warp_last = row0 < nr ? pos_of(min(row0 + RW, nr) - 1) : -1;
-            if (wide) __syncthreads();  // (another warp's copies may go where this one's queries were)
-            __syncwarp();
-            ask();
 
             // ---- block by block: scores and their weights, then the weighted values ----
             const auto hi = [](const auto& x, int i) -> uint32_t { return SETS == 2 ? x[SETS == 2 ? i : 0] : 0u; };
@@ -571,14 +606,14 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                     ask();
                     kb = ring + slot_at * S::kSlot;
                     vb = kb + S::kSlot;
-                    slot_at = slot_at == kAtSlots - 2 ? 0 : slot_at + 2;
+                    slot_at = slot_at == S::kSlots - 2 ? 0 : slot_at + 2;
                 } else {
-                    copies_wait<2>();
+                    copies_wait<RING - 1>();
                     __syncwarp();
                     kb = mine_ring + slot_at * S::kSlot;
-                    slot_at = slot_at == 2 ? 0 : slot_at + 1;
+                    slot_at = slot_at == RING - 1 ? 0 : slot_at + 1;
                     vb = mine_ring + slot_at * S::kSlot;
-                    slot_at = slot_at == 2 ? 0 : slot_at + 1;
+                    slot_at = slot_at == RING - 1 ? 0 : slot_at + 1;
                 }
                 const bool works = warp_last >= b * kKvBlock;
                 uint32_t pd[3][2][2 * SETS];  // [digit][k step][a0, a2 of rows g, then of rows g + 8]
@@ -671,7 +706,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 if (!wide) {
                     __syncwarp();
                     ask();
-                    copies_wait<2>();
+                    copies_wait<RING - 1>();
                     __syncwarp();
                 }
                 if (works) {
@@ -716,38 +751,61 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 }
             }
 
-            // ---- the open block: float32 rows, plain multiply-adds, 16 rows at a time ----
+            // ---- the open block: float32 rows, plain multiply-adds, 16 rows at a time, into the first piece ----
             if (open) {
                 const float* ko = c.open_row(c.k_open, s, h, closed * kKvBlock);
                 const float* vo = c.open_row(c.v_open, s, h, closed * kKvBlock);
+                const int o4 = c.dim_o / 4, half = kKvBlock / 2;
+                const auto bring = [&](float* to, int ld, const float* from, int n) {  // rows, by warps
+#pragma unroll 1
+                    for (int j = warp; j < n; j += kAtWarps)
+#pragma unroll 1
+                        for (int d = lane; d < o4; d += 32) copy16(to + j * ld + d * 4, from + (size_t)j * c.dim_o + d * 4);
+                    copies_commit();
+                };
 #pragma unroll 1
                 for (int g0 = 0; g0 < nr; g0 += kAtOpenRows) {
                     const int gn = min(kAtOpenRows, nr - g0);
                     __syncthreads();
                     stage_queries(open_q, LD, g0, gn, tid, kAtThreads);
-                    copies_wait<0>();
-                    __syncthreads();
+                    bring(open_k, S::kLdOpen, ko, min(n_open, half));
+                    bring(open_v, c.dim_o, vo, min(n_open, half));
 #pragma unroll 1
-                    for (int j0 = warp * 8; j0 < n_open; j0 += kAtWarps * 8) {  // a lane: a position (g) and every fourth four dimensions
-                        const float* row = ko + (size_t)min(j0 + g, n_open - 1) * c.dim_o;
-                        float4 f[2 * NK];
-#pragma unroll
-                        for (int i = 0; i < 2 * NK; ++i)
-                            f[i] = 16 * i + 4 * t < c.dim_o ? __ldg(reinterpret_cast<const float4*>(row + 16 * i + 4 * t)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int j0 = warp * 8; j0 - warp * 8 < n_open; j0 += half) {  // a lane: a position (g) and every fourth four dimensions
+                        if (j0 >= half) {
+                            __syncthreads();
+                            bring(open_k, S::kLdOpen, ko + (size_t)half * c.dim_o, n_open - half);
+                            copies_wait<0>();
+                        } else {
+                            copies_wait<1>();
+                        }
+                        __syncthreads();
+                        const float* row = open_k + (j0 % half + g) * S::kLdOpen + 4 * t;  // (rows past the last: whatever is there)
 #pragma unroll 1
-                        for (int r = 0; r < gn; ++r) {
-                            float dot = 0.f;
+                        for (int r = 0; r < gn; r += 4) {
+                            float dot[4] = {};
 #pragma unroll
                             for (int i = 0; i < 2 * NK; ++i) {
-                                const float4 q = *reinterpret_cast<const float4*>(open_q + r * LD + 16 * i + 4 * t);
-                                dot = fmaf(q.x, f[i].x, fmaf(q.y, f[i].y, fmaf(q.z, f[i].z, fmaf(q.w, f[i].w, dot))));
+                                if (16 * i + 4 * t >= c.dim_o) break;
+                                const float4 f = *reinterpret_cast<const float4*>(row + 16 * i);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {  // (rows past gn: whatever is there)
+                                    const float4 q = *reinterpret_cast<const float4*>(open_q + (r + e) * LD + 16 * i + 4 * t);
+                                    dot[e] = fmaf(q.x, f.x, fmaf(q.y, f.y, fmaf(q.z, f.z, fmaf(q.w, f.w, dot[e]))));
+                                }
                             }
-                            dot += __shfl_xor_sync(0xffffffffu, dot, 1);
-                            dot += __shfl_xor_sync(0xffffffffu, dot, 2);
-                            if (t == 0 && j0 + g < n_open) open_w[(j0 + g) * kAtOpenRows + r] = dot * p.scale;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                dot[e] += __shfl_xor_sync(0xffffffffu, dot[e], 1);
+                                dot[e] += __shfl_xor_sync(0xffffffffu, dot[e], 2);
+                            }
+                            const float mine = t == 0 ? dot[0] : t == 1 ? dot[1] : t == 2 ? dot[2] : dot[3];
+                            if (j0 + g < n_open) open_w[(j0 + g) * kAtOpenRows + r + t] = mine * p.scale;
                         }
                     }
                     __syncthreads();
+                    if (n_open > half) bring(open_k, c.dim_o, vo + (size_t)half * c.dim_o, n_open - half);
+                    float* sm = s_m[0];
 #pragma unroll 1
                     for (int r = warp; r < gn; r += kAtWarps) {
                         const int vis = min(n_open, pos_of(g0 + r) - closed * kKvBlock + 1);  // (0 or less: none)
@@ -760,33 +818,56 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                         for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
                         open_w[lane * kAtOpenRows + r] = w0;
                         open_w[(lane + 32) * kAtOpenRows + r] = w1;
-                        if (lane == 0) {
-                            s_m[kAtWarps][g0 + r] = vis > 0 ? top : -CUDART_INF_F;
-                            s_l[kAtWarps][g0 + r] = sum;
+                        if (lane == 0) {  // the first piece's row and this one's on one scale
+                            const float was = sm[g0 + r], both = fmaxf(was, top);
+                            const float fp = was == -CUDART_INF_F ? 0.f : exp2_of(was - both), fo = vis > 0 ? exp2_of(top - both) : 0.f;
+                            s_f[0][r] = fp;
+                            s_f[1][r] = fo;
+                            sm[g0 + r] = both;
+                            s_l[0][g0 + r] = fmaf(s_l[0][g0 + r], fp, vis > 0 ? sum * fo : 0.f);
                         }
                     }
+                    copies_wait<0>();
                     __syncthreads();
                     const int seen = min(n_open, pos_of(g0 + gn - 1) - closed * kKvBlock + 1);
+                    const bool alike = pos_of(g0) == pos_of(g0 + gn - 1);
 #pragma unroll 1
                     for (int d = tid; d < hd; d += kAtThreads) {
 #pragma unroll 1
                         for (int r = 0; r < gn; r += 4) {
                             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                            for (int k = 0; k < 2; ++k) {
+                                const float* from = (k ? open_k : open_v) + d;
+                                const float* ws = open_w + k * half * kAtOpenRows + r;
+                                const int n = min(seen - k * half, half);
+                                if (alike) {
 #pragma unroll 8
-                            for (int j = 0; j < seen; ++j) {
-                                const float v = __ldg(vo + (size_t)j * c.dim_o + d);
-                                const float4 w = *reinterpret_cast<const float4*>(open_w + j * kAtOpenRows + r);
-                                // (a row that does not see position j must not meet what is there)
-                                sum.x = w.x != 0.f ? fmaf(w.x, v, sum.x) : sum.x;
-                                sum.y = w.y != 0.f ? fmaf(w.y, v, sum.y) : sum.y;
-                                sum.z = w.z != 0.f ? fmaf(w.z, v, sum.z) : sum.z;
-                                sum.w = w.w != 0.f ? fmaf(w.w, v, sum.w) : sum.w;
+                                    for (int j = 0; j < n; ++j) {
+                                        const float v = from[j * c.dim_o];
+                                        const float4 w = *reinterpret_cast<const float4*>(ws + j * kAtOpenRows);
+                                        sum = make_float4(fmaf(w.x, v, sum.x), fmaf(w.y, v, sum.y), fmaf(w.z, v, sum.z), fmaf(w.w, v, sum.w));
+                                    }
+                                } else {  // a row that does not see position j must not meet what is there
+#pragma unroll 2
+                                    for (int j = 0; j < n; ++j) {
+                                        const float v = from[j * c.dim_o];
+                                        const float4 w = *reinterpret_cast<const float4*>(ws + j * kAtOpenRows);
+                                        sum.x = w.x != 0.f ? fmaf(w.x, v, sum.x) : sum.x;
+                                        sum.y = w.y != 0.f ? fmaf(w.y, v, sum.y) : sum.y;
+                                        sum.z = w.z != 0.f ? fmaf(w.z, v, sum.z) : sum.z;
+                                        sum.w = w.w != 0.f ? fmaf(w.w, v, sum.w) : sum.w;
+                                    }
+                                }
                             }
-                            float* to = open_o + (g0 + r) * LD + d;
-                            to[0] = sum.x;
-                            if (r + 1 < gn) to[LD] = sum.y;
-                            if (r + 2 < gn) to[2 * LD] = sum.z;
-                            if (r + 3 < gn) to[3 * LD] = sum.w;
+                            const float e4[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (r + e < gn) {
+                                    float& x = pieces[(g0 + r + e) * LD + d];
+                                    const float fp = s_f[0][r + e], fo = s_f[1][r + e];
+                                    x = fmaf(fp, x, fo != 0.f ? fo * e4[e] : 0.f);
+                                }
                         }
                     }
                 }
@@ -814,38 +895,33 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
             const auto slot = [&](int k) { return p.part + (size_t)place_of(k) * S::kTile * p.part_ld; };
             float* part = slot(cut);
             if (tid < nr) {  // a row's largest score and sum, and factors in the place of the pieces' own
-                float top = open ? s_m[kAtWarps][tid] : -CUDART_INF_F, sum = 0.f;
+                float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll 1
                 for (int w = 0; w < pieces_n; ++w) top = fmaxf(top, s_m[w][tid]);
 #pragma unroll 1
-                for (int w = 0; w <= kAtWarps; ++w) {
-                    const bool is = w < pieces_n || (w == kAtWarps && open);
-                    const float f = is ? factor(s_m[w][tid], top) : 0.f;
-                    if (is) sum = fmaf(s_l[w][tid], f, sum);
+                for (int w = 0; w < pieces_n; ++w) {
+                    const float f = factor(s_m[w][tid], top);
+                    sum = fmaf(s_l[w][tid], f, sum);
                     s_m[w][tid] = f;
                 }
                 s_l[0][tid] = sum;
                 if (!done) __stcg(reinterpret_cast<float2*>(part + (size_t)tid * p.part_ld + 4 * d4s), make_float2(top, sum));
             }
             __syncthreads();
-#pragma unroll 2
-            for (int i = tid; i < nr * d4s; i += kAtThreads) {
-                const int r = i / d4s, d = (i - r * d4s) * 4;
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                const auto add = [&](const float* from, float f) {
-                    const float4 v = *reinterpret_cast<const float4*>(from + r * LD + d);
-                    // (f is 0 for a piece that has none of the row's positions: what stands there does not count)
-                    x.x = f != 0.f ? fmaf(v.x, f, x.x) : x.x;
-                    x.y = f != 0.f ? fmaf(v.y, f, x.y) : x.y;
-                    x.z = f != 0.f ? fmaf(v.z, f, x.z) : x.z;
-                    x.w = f != 0.f ? fmaf(v.w, f, x.w) : x.w;
-                };
 #pragma unroll 1
-                for (int w = 0; w < pieces_n; ++w) add(pieces + w * RW * LD, s_m[w][r]);
-                if (open) add(open_o, s_m[kAtWarps][r]);
-                if (done) put(r, d, x, s_l[0][r]);
-                else __stcg(reinterpret_cast<float4*>(part + (size_t)r * p.part_ld + d), x);
-            }
+            for (int r = warp; r < nr; r += kAtWarps)
+#pragma unroll 1
+                for (int d = lane * 4; d < hd; d += 128) {
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                    for (int w = 0; w < pieces_n; ++w) {
+                        const float f = s_m[w][r];
+                        // (0 for a piece that has none of the row's positions: what stands there does not count)
+                        if (f != 0.f) add_scaled(x, *reinterpret_cast<const float4*>(pieces + (w * RW + r) * LD + d), f);
+                    }
+                    if (done) put(r, d, x, s_l[0][r]);
+                    else __stcg(reinterpret_cast<float4*>(part + (size_t)r * p.part_ld + d), x);
+                }
             if (!done) {
                 __threadfence();
                 __syncthreads();
@@ -857,6 +933,7 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
                 __syncthreads();
                 if (s_last) {
                     __threadfence();
+                    lb_fence_proxy_async();  // (the other CTAs' ordinary stores, before copies that go another way)
                     // rows of the parts, some at a time, through shared memory, every copy in flight at once
                     const int ld = 4 * d4s + 4, room = (int)(S::kSmem / 4) - kAtWarps * 4;
                     const int per = min(nr, max(1, room / (cuts * (ld + 1))));           // rows of a round
@@ -871,49 +948,58 @@ __global__ void __launch_bounds__(kAtThreads) lb_kv8_attend_kernel(const AttendP
 #pragma unroll 1
                         for (int q0 = 0; q0 < cuts; q0 += fit) {
                             const int qn = min(fit, cuts - q0);
+                            lb_fence_proxy_async();  // (what stood there was read and written by ordinary accesses)
                             __syncthreads();
-#pragma unroll 1
-                            for (int q = warp; q < qn; q += kAtWarps) {
-                                const float* from = slot(q0 + q) + (size_t)g0 * ld;
-#pragma unroll 4
-                                for (int j = lane; j < row4; j += 32) copy16(got + (q * row4 + j) * 4, from + j * 4);
+                            if (warp == 0) {
+                                if (lane == 0) lb_mbar_expect_tx(&s_bar, (uint32_t)qn * row4 * 16);
+                                __syncwarp();
+                                for (int q = lane; q < qn; q += 32) lb_bulk_g2s(got + q * row4 * 4, slot(q0 + q) + (size_t)g0 * ld, row4 * 16, &s_bar);
                             }
-                            copies_commit();
-                            copies_wait<0>();
+                            if (!lb_mbar_wait_bounded(&s_bar, bar_phase)) atomicExch(c.status, 1);
+                            bar_phase ^= 1;
                             __syncthreads();
                             const float was = top;
-                            if (fit < cuts || tid < gn) {  // a row to a thread; the one row of several rounds to every thread
-                                const int r = fit < cuts ? 0 : tid;
-#pragma unroll 4
-                                for (int q = 0; q < qn; ++q) top = fmaxf(top, got[(q * gn + r) * ld + 4 * d4s]);
-                                const float f0 = factor(was, top);
-                                sum *= f0;
-                                y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
-#pragma unroll 4
-                                for (int q = 0; q < qn; ++q) {
-                                    const float2 ml = *reinterpret_cast<const float2*>(got + (q * gn + r) * ld + 4 * d4s);
-                                    const float f = factor(ml.x, top);
-                                    sum = fmaf(ml.y, f, sum);
+#pragma unroll 1
+                            for (int r = fit < cuts ? 0 : warp; r < gn; r += kAtWarps) {  // (the one row of several rounds: every warp)
+                                const auto stat = [&](int q, int k) { return got[(q * gn + r) * ld + 4 * d4s + k]; };
+                                float now = was, more = 0.f;
+#pragma unroll 1
+                                for (int q = lane; q < qn; q += 32) now = fmaxf(now, stat(q, 0));
+                                now = lb_warp_max(now);
+#pragma unroll 1
+                                for (int q = lane; q < qn; q += 32) {
+                                    const float f = factor(stat(q, 0), now);
+                                    more = fmaf(stat(q, 1), f, more);
                                     fs[q * gn + r] = f;
                                 }
-                                if (fit >= cuts) s_l[0][r] = sum;
+#pragma unroll
+                                for (int x = 16; x > 0; x >>= 1) more += __shfl_xor_sync(0xffffffffu, more, x);
+                                if (fit < cuts) {
+                                    const float f0 = factor(was, now);
+                                    sum = fmaf(sum, f0, more);
+                                    y = make_float4(y.x * f0, y.y * f0, y.z * f0, y.w * f0);
+                                    top = now;
+                                } else if (lane == 0) {
+                                    s_l[0][r] = more;
+                                }
                             }
                             __syncthreads();
-#pragma unroll 1
-                            for (int i = tid; i < gn * d4s; i += kAtThreads) {
-                                const int r = i / d4s, d = (i - r * d4s) * 4;
+                            if (fit < cuts) {  // (a row has 64 groups of four dimensions at most: every thread has one, or none)
+                                if (tid < d4s)
 #pragma unroll 4
-                                for (int q = 0; q < qn; ++q) {
-                                    const float f = fs[q * gn + r];
-                                    const float4 v4 = *reinterpret_cast<const float4*>(got + (q * gn + r) * ld + d);
-                                    y.x = f != 0.f ? fmaf(v4.x, f, y.x) : y.x;
-                                    y.y = f != 0.f ? fmaf(v4.y, f, y.y) : y.y;
-                                    y.z = f != 0.f ? fmaf(v4.z, f, y.z) : y.z;
-                                    y.w = f != 0.f ? fmaf(v4.w, f, y.w) : y.w;
-                                }
-                                if (fit < cuts) break;  // (one row has 64 groups of four dimensions at most: every thread has one of them, or none)
-                                put(g0 + r, d, y, s_l[0][r]);
-                                y = make_float4(0.f, 0.f, 0.f, 0.f);
+                                    for (int q = 0; q < qn; ++q)
+                                        if (const float f = fs[q]) add_scaled(y, *reinterpret_cast<const float4*>(got + q * ld + tid * 4), f);
+                            } else {
+#pragma unroll 1
+                                for (int r = warp; r < gn; r += kAtWarps)
+#pragma unroll 1
+                                    for (int d = lane * 4; d < hd; d += 128) {
+                                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                                        for (int q = 0; q < qn; ++q)
+                                            if (const float f = fs[q * gn + r]) add_scaled(x, *reinterpret_cast<const float4*>(got + (q * gn + r) * ld + d), f);
+                                        put(g0 + r, d, x, s_l[0][r]);
+                                    }
                             }
                         }
                         if (fit < cuts && tid < d4s) put(g0, tid * 4, y, sum);
@@ -953,7 +1039,8 @@ constexpr int kAtMostCtasPerSm = 2;
 template <int NK, int SETS>
 static int launch_attend(loom_b200_ctx* ctx, AttendParams p) {
     using S = AttendShape<NK, SETS>;
-    p.ctas = ctx->sm_count * (S::kSmem <= 110 * 1024 ? kAtMostCtasPerSm : 1);
+    p.ctas = ctx->sm_count * S::kPerSm;
+    static_assert(S::kPerSm * (S::kSmem + 6 * 1024) <= 228 * 1024, "shared memory of an SM");
     p.part = (float*)((uint8_t*)p.cnt + (2 * (size_t)ctx->sm_count * kAtMostCtasPerSm + 1) * 4 / 16 * 16 + 16);
     const size_t smem = S::kSmem;
     LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_attend_kernel<NK, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
