@@ -494,7 +494,7 @@ int loom_b200_decoder_extend(loom_b200_decoder* dec, const int32_t* tokens, int 
  *          first) times all of it
  * temperature 0 or less: the first largest logit.  Not-a-numbers and minus infinity are never chosen; plus infinities share alike; a row
  * with nothing to choose gives -1.  logprob [rows] or NULL: logarithm of the chosen token's share of the kept weight (not a number for -1).
- * Sums are integers and repeat bit for bit.  vocab <= 737,280. */
+ * Sums are integers and repeat bit for bit.  vocab <= 655,360. */
 int loom_b200_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logits, long long stride, const float* temperature,
                      const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* tokens, float* logprob);
 

@@ -298,6 +298,9 @@ __device__ __forceinline__ uint32_t lb_cluster_addr(uint32_t smem_addr, uint32_t
 __device__ __forceinline__ void lb_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// its two halves
+__device__ __forceinline__ void lb_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void lb_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // float64 matrix instruction: eight rows x four columns times four columns x eight columns
 __device__ __forceinline__ void lb_dmma_884(double (&c)[2], double a, double b) {
     asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};" : "+d"(c[0]), "+d"(c[1]) : "d"(a), "d"(b));

@@ -11,11 +11,21 @@
 // T <= 0 is the first largest logit.  Weights are integers, round(w 2^S) with S such that a whole row's sum stays below 2^62: sums do not
 // depend on their order then, and are within vocab * 2^-S of the real ones (S = 44 for 128,256 tokens: 7e-9 of the largest weight).
 //
-// One cluster of CTAs per row, each with a slice of the row in shared memory, so the row is read once and by one launch.  What the kept
-// set ends with is one place in the order -- a (logit, index) pair: top-k finds it from a histogram of counts over 1024 linear bins of
-// m - l, top-p from one of weights; the bins are added up across the cluster through distributed shared memory, the few values of
-// the bin that the limit falls into are gathered in one CTA and ranked there among each other.  A bin with more than 1024 values (long
-// stretches of equal or nearly equal logits) is divided further by the bits of the values, down to a single value, whose ties go by index.
+// One cluster of CTAs per row, each with a slice of the row in shared memory, so the row is read once and by one launch.  What is kept
+// ends at a place in the order, a (logit, index) pair.  A place is found from a histogram -- of counts for top-k, of weights for
+// top-p -- over linear bins of m - l: the values of the bin that the limit falls into are few, and are put in order by another one, down to
+// what a handful of comparisons settles.  Three ways there, the cheapest that holds:
+//   few     values that no kept one is below are gathered in the first CTA, which does the rest by itself while the others' places are
+//           free for the next rows.  top-k: with G >= k groups of tokens, at least k values reach the smallest of the groups' largest
+//           ones, of values in random order about G ln G do (270 for k up to 64); min-p: the values not below it; small vocabularies: all.  2048
+//           values at most
+//   cluster the CTAs' histograms are added up through distributed shared memory.  Weights enter them in units of 2^-17 of the largest, by
+//           32-bit atomics: they say which bins to look at, and what lies in front of those is then added up exactly
+//   whole   the same with exact weights, bins divided further by the bits of the values down to a single value, whose ties go by index: long
+//           stretches of equal or nearly equal logits, top-p next to 1
+//
+// Weights are exp2 of a double by a table of 32 entries and a polynomial (P. T. P. Tang, Table-driven implementation of the exponential
+// function, ACM TOMS 15, 1989): eleven float64 operations at 64 lanes a clock and one conversion; error 2^-48 of the value.
 #include "common.cuh"
 
 #include <math_constants.h>
@@ -25,8 +35,11 @@ namespace {
 constexpr int kSpThreads = 512;
 constexpr int kSpWarps = kSpThreads / 32;
 constexpr int kSpBins = 1024;
-constexpr int kSpCap = 1024;        // values that are ranked among each other
-constexpr int kSpMaxSlice = 46080;  // logits of a CTA: 180 KB
+constexpr int kSpFine = 4096;       // bins of a cluster of four CTAs and more
+constexpr int kSpCap = 1024;        // values of one bin that are ranked among each other
+constexpr int kSpFew = 2048;        // values that the first CTA sorts
+constexpr float kSpReach = 12.5f;   // distances that histograms of weights take, in temperatures: beyond them a weight is less than half a unit
+constexpr int kSpMaxSlice = 40960;  // logits of a CTA: 160 KB
 constexpr int kSpMaxCluster = 16;
 
 
@@ -44,20 +57,38 @@ struct SampleParams {
 
 using u64 = unsigned long long;
 
-struct SampleShared {
-    u64 mass[kSpBins];
-    u64 cand[kSpCap], cand_w[kSpCap];
-    u64 share_mass[kSpBins];  // running sums over this CTA's share of the bins
+struct __align__(16) SampleShared {  // (the slice behind it is written sixteen bytes at a time)
+    double exp2_32[32];      // 2^(j/32)
+    u64 mass[kSpBins];       // bins of weights; running sums over this CTA's share of finer ones; with cand, values on their way to the first CTA
+    u64 cand[kSpCap];        // values on their way, their weights
+    union {
+        u64 few[kSpFew];         // in the first CTA: all CTAs' values that are left, as places
+        unsigned fine[kSpFine];  // finer bins
+        struct {
+            u64 share_mass[kSpBins];  // running sums over this CTA's share of the bins
+            unsigned share_count[kSpBins];
+            unsigned count[kSpBins];
+        };
+    };
+    union {
+        unsigned wlist[kSpFew];  // a bin's values
+        u64 cand_w[kSpCap];
+    };
     u64 xa[2][kSpMaxCluster], xb[2][kSpMaxCluster];  // a pair of words from every CTA, two exchanges alternating
     u64 ra[2], rb[2], rc[2];                          // an answer from one CTA
     u64 wsum[kSpWarps];
-    unsigned count[kSpBins];
-    unsigned share_count[kSpBins];
+    float wf[kSpWarps];
     unsigned wcount[kSpWarps];
     unsigned n_cand;
     int flag;
 };
-
+// (declared again wherever it is used, so that the compiler knows the accesses for shared ones)
+#define LB_SAMPLE_SHARED                                       \
+    extern __shared__ __align__(16) uint8_t lb_sample_smem[]; \
+    SampleShared& s = *reinterpret_cast<SampleShared*>(lb_sample_smem)
+static_assert(sizeof(SampleShared) % 16 == 0, "alignment of the slice");
+static_assert(kSpBins + kSpCap >= kSpFew, "the values that are left, in the place of the bins");
+constexpr size_t kSpLeast = (size_t)kSpFew * 8;  // bytes of the slice's place, where the first CTA keeps weights later
 static_assert(sizeof(SampleShared) + (size_t)kSpMaxSlice * 4 <= 227 * 1024, "shared memory of a CTA");
 
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, u64 v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory"); }
@@ -68,7 +99,7 @@ __device__ __forceinline__ u64 ld_cluster_u64(uint32_t addr) {
 }
 __device__ __forceinline__ unsigned ld_cluster_u32(uint32_t addr) {
     unsigned v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
 __device__ __forceinline__ unsigned add_cluster_u32(uint32_t addr, unsigned v) {
@@ -123,17 +154,34 @@ struct Row {
     float top;     // the largest logit
     double inv_t;
     float bin_scale;
+    float far;     // no weight beyond it: 48 temperatures
     int bits;
 
     __device__ __forceinline__ double distance(float l) const { return ((double)l - (double)top) * inv_t; }
-    // round(exp(d) 2^S).  Below exp(-15) = 2^-21.6 the float exponential's error, 2^-22 of the value, is 2^-43 of the largest weight.
+    // round(2^S exp(d)), d <= 0
+    __device__ __forceinline__ u64 weight_at(double d) const {
+        const double y = d * 1.4426950408889634;                      // log2(e)
+        if (!(y > -62.0)) return 0;                                   // (not a number: too)
+        const double big = 6755399441055744.0 / 32;                   // 1.5 2^52 / 32: the sum's low word is y rounded to 32nds
+        const double k = y + big;
+        const int n = __double2loint(k);                              // 32 y
+        // the rest in natural units, from d itself: 32nds of ln 2 in two parts, the first with 32 bits
+        const double j = k - big;
+        const double x = fma(j, -1.9082149292705877e-10, fma(j, -0.6931471803691238, d));
+        double e = fma(x, 1.0 / 120, 1.0 / 24);
+        e = fma(e, x, 1.0 / 6);
+        e = fma(e, x, 0.5);
+        e = fma(e, x, 1.0);
+        LB_SAMPLE_SHARED;
+        const double t = s.exp2_32[n & 31];
+        e = fma(t * x, e, t);                                         // 2^(n % 32 / 32) exp(x)
+        e = __hiloint2double(__double2hiint(e) + ((n >> 5) + bits) * (1 << 20), __double2loint(e));
+        return __double2ull_rn(e);
+    }
     __device__ __forceinline__ u64 weight(float l) const {
         if (l == top) return 1ull << bits;
         if (top == CUDART_INF_F || l == -CUDART_INF_F) return 0;
-        const double d = distance(l);
-        if (d < -44.0) return 0;  // exp(-44) < 2^-63
-        if (d < -15.0) return __float2ull_rn(ldexpf(expf((float)d), bits));
-        return __double2ull_rn(ldexp(exp(d), bits));
+        return weight_at(distance(l));
     }
     __device__ __forceinline__ int bin(float l) const {
         const int b = (int)((top - l) * bin_scale);  // (not a number, from equal infinities: 0)
@@ -141,17 +189,16 @@ struct Row {
     }
 };
 
-struct Cluster {
-    SampleShared& s;
-    const float* x;  // this CTA's slice
-    int n, first;    // its logits, and the first one's index in the row
-    unsigned rank, size;
-    int turn;
+__device__ __forceinline__ uint32_t remote(const void* p, unsigned r) { return lb_cluster_addr(lb_smem_u32(p), r); }
 
-    __device__ __forceinline__ uint32_t remote(const void* p, unsigned r) const { return lb_cluster_addr(lb_smem_u32(p), r); }
+struct Cluster {
+    int n, first;    // this CTA's logits, and the first one's index in the row
+    int n_most;      // logits of a CTA, at most
+    unsigned rank, size;
 
     // a pair of words from every CTA to every CTA: s.xa[turn], s.xb[turn] by rank; all threads call
-    __device__ __forceinline__ int exchange(u64 a, u64 b) {
+    __device__ __forceinline__ int exchange(int& turn, u64 a, u64 b) const {
+        LB_SAMPLE_SHARED;
         turn ^= 1;
         if (threadIdx.x < size) {
             st_cluster_u64(remote(&s.xa[turn][rank], threadIdx.x), a);
@@ -161,7 +208,8 @@ struct Cluster {
         return turn;
     }
     // one CTA's answer to every CTA (`mine`: whether this is the one; a, b, c are read from thread 0 .. size-1 of it)
-    __device__ __forceinline__ int answer(bool mine, u64 a, u64 b, u64 c) {
+    __device__ __forceinline__ int answer(int& turn, bool mine, u64 a, u64 b, u64 c) const {
+        LB_SAMPLE_SHARED;
         turn ^= 1;
         if (mine && threadIdx.x < size) {
             st_cluster_u64(remote(&s.ra[turn], threadIdx.x), a);
@@ -180,8 +228,8 @@ struct Found {
 };
 
 // The histogram of every CTA is complete: adds it up over the cluster, every CTA a share of the bins.  Returns the weight of all bins.
-__device__ u64 add_bins(Cluster& c, bool mass, int& turn) {
-    SampleShared& s = c.s;
+__device__ __noinline__ u64 add_bins(const Cluster c, bool mass, int& turn) {
+    LB_SAMPLE_SHARED;
     const int share = kSpBins / c.size, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     lb_cluster_sync();
     u64 run_m = 0;
@@ -193,8 +241,8 @@ __device__ u64 add_bins(Cluster& c, bool mass, int& turn) {
         if (b < share) {
             const int at = c.rank * share + b;
             for (unsigned r = 0; r < c.size; ++r) {
-                n += ld_cluster_u32(c.remote(&s.count[at], r));
-                if (mass) m += ld_cluster_u64(c.remote(&s.mass[at], r));
+                n += ld_cluster_u32(remote(&s.count[at], r));
+                if (mass) m += ld_cluster_u64(remote(&s.mass[at], r));
             }
         }
         u64 sm = warp_scan_u64(m, lane);
@@ -220,15 +268,15 @@ __device__ u64 add_bins(Cluster& c, bool mass, int& turn) {
         }
         __syncthreads();
     }
-    turn = c.exchange(run_c, run_m);
+    c.exchange(turn, run_c, run_m);
     u64 total = 0;
     for (unsigned r = 0; r < c.size; ++r) total += s.xb[turn][r];
     return total;
 }
 
 // The first bin at which the count (mass: the weight) reaches `limit`; `turn` as add_bins left it.
-__device__ Found find_bin(Cluster& c, bool mass, u64 limit, int turn) {
-    SampleShared& s = c.s;
+__device__ __noinline__ Found find_bin(const Cluster c, bool mass, u64 limit, int& turn) {
+    LB_SAMPLE_SHARED;
     const int share = kSpBins / c.size;
     u64 before = 0;
     unsigned owner = c.size - 1;
@@ -260,15 +308,16 @@ __device__ Found find_bin(Cluster& c, bool mass, u64 limit, int turn) {
         b = at ? before + (mass ? s.share_mass[at - 1] : (u64)s.share_count[at - 1]) : before;
         n = s.share_count[at] - (at ? s.share_count[at - 1] : 0u);
     }
-    const int t = c.answer(c.rank == owner, a, b, n);
+    const int t = c.answer(turn, c.rank == owner, a, b, n);
     return {(int)s.ra[t], s.rb[t], (unsigned)s.rc[t]};
 }
 
 // The place of the last value, among those at or in front of `cut` in the order, that the limit lets through: the limit-th one, or with
 // `mass` the first one with which the weight reaches the limit.  limit >= 1 and at most what there is.  With mass and share > 0 the limit
 // is that share of the weight.
-__device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limit, float share) {
-    SampleShared& s = c.s;
+__device__ __noinline__ u64 find_cut(const Cluster c, const Row row, int& turn, u64 cut, bool mass, u64 limit, float share) {
+    LB_SAMPLE_SHARED;
+    const float* const x = reinterpret_cast<const float*>(lb_sample_smem + sizeof(SampleShared));
     const unsigned top_key = key_of(row.top);
     int lin = -1;                              // the linear bin that the search has come to, then
     unsigned lo = 0, hi = 0xffffffffu;         // the stretch of top_key - key inside it
@@ -282,7 +331,7 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
         }
         __syncthreads();
         for (int i = threadIdx.x; i < c.n; i += kSpThreads) {
-            const float l = c.x[i];
+            const float l = x[i];
             if (place_of(l, c.first + i) < cut) continue;
             int b = row.bin(l);
             if (level > 0) {
@@ -296,7 +345,6 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
                 if (w) atomicAdd(&s.mass[b], w);
             }
         }
-        int turn;
         const u64 total = add_bins(c, mass, turn);
         if (level == 0 && mass && share >= 0.f) {
             limit = part_of(share, total, true);
@@ -318,14 +366,14 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
         if (threadIdx.x == 0) s.n_cand = 0;
         lb_cluster_sync();
         for (int i = threadIdx.x; i < c.n; i += kSpThreads) {
-            const float l = c.x[i];
+            const float l = x[i];
             const u64 p = place_of(l, c.first + i);
             const unsigned d = top_key - key_of(l);
             if (p < cut || row.bin(l) != lin || d < lo || d > hi) continue;
-            const unsigned at = add_cluster_u32(c.remote(&s.n_cand, 0), 1u);
+            const unsigned at = add_cluster_u32(remote(&s.n_cand, 0), 1u);
             if (at < kSpCap) {
-                st_cluster_u64(c.remote(&s.cand[at], 0), p);
-                st_cluster_u64(c.remote(&s.cand_w[at], 0), mass ? row.weight(l) : 1ull);
+                st_cluster_u64(remote(&s.cand[at], 0), p);
+                st_cluster_u64(remote(&s.cand_w[at], 0), mass ? row.weight(l) : 1ull);
             }
         }
         lb_cluster_sync();
@@ -344,7 +392,7 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
             __syncthreads();
             for (int w = 0; w < kSpWarps; ++w) last = s.wsum[w] < last ? s.wsum[w] : last;
         }
-        const int t = c.answer(c.rank == 0, last, 0, 0);
+        const int t = c.answer(turn, c.rank == 0, last, 0, 0);
         return s.ra[t];
     }
     // one value that more than kSpCap tokens share: the tie-th of them by index
@@ -358,7 +406,7 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
     const int per = ((c.n + kSpThreads - 1) / kSpThreads + 31) / 32 * 32 * 32;  // a warp's stretch of the slice
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int from = min(c.n, warp * per), to = min(c.n, from + per);
-    const auto is_tie = [&](int i) { return key_of(c.x[i]) == key && place_of(c.x[i], c.first + i) >= cut; };
+    const auto is_tie = [&](int i) { return key_of(x[i]) == key && place_of(x[i], c.first + i) >= cut; };
     unsigned mine = 0;
     for (int i = from + lane; i < to; i += 32) mine += is_tie(i);
     mine = __reduce_add_sync(0xffffffffu, mine);
@@ -366,7 +414,7 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
     __syncthreads();
     u64 all = 0;
     for (int w = 0; w < kSpWarps; ++w) all += s.wcount[w];
-    const int t0 = c.exchange(all, 0);
+    const int t0 = c.exchange(turn, all, 0);
     u64 before = 0;
     unsigned owner = 0;
     for (unsigned r = 0; r < c.size; ++r) {
@@ -385,7 +433,7 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
                 const unsigned hit = __ballot_sync(0xffffffffu, i < to && is_tie(i));
                 const unsigned need = (unsigned)(tie - ahead);
                 if (__popc(hit) >= (int)need) {
-                    if ((hit >> lane & 1u) && __popc(hit & ((2u << lane) - 1u)) == (int)need) s.cand[0] = place_of(c.x[i], c.first + i);
+                    if ((hit >> lane & 1u) && __popc(hit & ((2u << lane) - 1u)) == (int)need) s.cand[0] = place_of(x[i], c.first + i);
                     break;
                 }
                 ahead += __popc(hit);
@@ -393,96 +441,516 @@ __device__ u64 find_cut(Cluster& c, const Row& row, u64 cut, bool mass, u64 limi
         __syncthreads();
     }
     const u64 at = c.rank == owner ? s.cand[0] : 0;
-    const int t = c.answer(c.rank == owner, at, 0, 0);
+    const int t = c.answer(turn, c.rank == owner, at, 0, 0);
+    return s.ra[t];
+}
+
+__device__ __forceinline__ float value_of_key(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ float value_of_place(u64 place) { return value_of_key((unsigned)(place >> 32)); }
+
+// Among the n <= kSpFew places in s.few that are at or in front of `cut`, with weights `w` (in shared memory; null: 1 each): the place of the last one that the limit
+// lets through, the first one with which they reach it.  limit >= 1 and at most what there is.  Values further
+// than `far` below the largest one have no weight: where the limit falls among them the place is 0, that is, all.  All of one CTA's threads.
+__device__ __noinline__ u64 local_cut(const u64* w, int n, u64 cut, u64 limit, float top, float far) {
+    LB_SAMPLE_SHARED;
+    const u64* v = s.few;
+    __builtin_assume(__isShared(w));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    float least = CUDART_INF_F;
+    for (int i = tid; i < n; i += kSpThreads)
+        if (v[i] >= cut && (!w || w[i])) least = fminf(least, value_of_place(v[i]));
+    least = -lb_warp_max(-least);
+    __syncthreads();
+    if (lane == 0) s.wf[warp] = least;
+    for (int b = tid; b < kSpBins; b += kSpThreads) s.mass[b] = 0;
+    __syncthreads();
+    for (int i = 0; i < kSpWarps; ++i) least = fminf(least, s.wf[i]);
+    const float scale = (float)kSpBins / fminf(top - least, far);
+    const auto bin_of = [&](u64 place) {
+        const int b = (int)((top - value_of_place(place)) * scale);  // (not a number, from equal ones: 0)
+        return b < kSpBins - 1 ? b : kSpBins - 1;
+    };
+    for (int i = tid; i < n; i += kSpThreads)
+        if (v[i] >= cut) {
+            const u64 x = w ? w[i] : 1;
+            if (x) atomicAdd(&s.mass[bin_of(v[i])], x);
+        }
+    if (tid == 0) {
+        s.n_cand = 0;
+        s.rc[0] = 0;
+    }
+    __syncthreads();
+    constexpr int B = kSpBins / kSpThreads;
+    u64 m[B], sum = 0;
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+        m[e] = s.mass[tid * B + e];
+        sum += m[e];
+    }
+    const u64 upto = warp_scan_u64(sum, lane);
+    if (lane == 31) s.wsum[warp] = upto;
+    __syncthreads();
+    u64 ahead = upto - sum;
+    for (int i = 0; i < warp; ++i) ahead += s.wsum[i];
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+        if (ahead < limit && ahead + m[e] >= limit) {
+            s.ra[0] = tid * B + e;
+            s.rb[0] = ahead;
+        }
+        ahead += m[e];
+    }
+    __syncthreads();
+    const int bin = (int)s.ra[0];
+    const u64 base = s.rb[0];
+    if (!w && bin == kSpBins - 1 && !(top - least <= far)) return 0;
+    unsigned* list = s.wlist;
+    for (int i = tid; i < n; i += kSpThreads)
+        if (v[i] >= cut && bin_of(v[i]) == bin) list[atomicAdd(&s.n_cand, 1u)] = (unsigned)i;
+    __syncthreads();
+    const int members = (int)s.n_cand;
+    for (int a = tid; a < members; a += kSpThreads) {
+        const unsigned i = list[a];
+        const u64 mine = v[i], x = w ? w[i] : 1;
+        u64 before = base;
+        for (int b = 0; b < members; ++b) {
+            const unsigned j = list[b];
+            if (v[j] > mine) before += w ? w[j] : 1;
+        }
+        if (before < limit && before + x >= limit) s.rc[0] = mine;
+    }
+    __syncthreads();
+    return s.rc[0];
+}
+
+// What the first CTA does with the n values that are left (in s.few): cuts, kept weight, token.
+__device__ __noinline__ void choose(const Row row, const SampleParams p, int r, int n, int k, float top_p, float min_p) {
+    LB_SAMPLE_SHARED;
+    u64* weights = reinterpret_cast<u64*>(lb_sample_smem + sizeof(SampleShared));  // (the slice has been read)
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 cut = 0;
+    if (k > 0 && k < n) cut = local_cut(nullptr, n, 0, (u64)k, row.top, row.far);
+    u64 mass = 0;
+    const double log_min = min_p > 0.f ? log((double)min_p) : -CUDART_INF;
+    for (int i = tid; i < n; i += kSpThreads) {
+        const u64 place = s.few[i], w = place >= cut ? row.weight(value_of_place(place)) : 0;
+        weights[i] = w;
+        mass += w;
+    }
+    if (top_p < 1.f) {
+        mass = warp_sum_u64(mass);
+        __syncthreads();
+        if (lane == 0) s.wsum[warp] = mass;
+        __syncthreads();
+        mass = 0;
+        for (int i = 0; i < kSpWarps; ++i) mass += s.wsum[i];
+        u64 need = part_of(fmaxf(top_p, 0.f), mass, true);
+        if (need == 0) need = 1;
+        __syncthreads();
+        const u64 at = local_cut(weights, n, cut, need, row.top, row.far);
+        cut = at > cut ? at : cut;
+    }
+    __syncthreads();
+    for (int b = tid; b < kSpBins; b += kSpThreads) s.mass[b] = 0;
+    if (tid == 0) s.n_cand = 0;
+    __syncthreads();
+    // by index: weights over stretches of indices, the stretch that the random number falls into, the place in it
+    int shift = 0;
+    while ((p.vocab - 1) >> shift >= kSpBins) ++shift;
+    for (int i = tid; i < n; i += kSpThreads) {
+        const u64 place = s.few[i];
+        u64 w = place >= cut ? weights[i] : 0;
+        if (w && min_p > 0.f) {
+            const float l = value_of_place(place);
+            if (l != row.top) {
+                const double d = row.distance(l);
+                if (!(d > log_min + 1e-6 || (d > log_min - 1e-6 && exp(d) >= (double)min_p))) w = 0;
+            }
+        }
+        weights[i] = w;
+        if (w) atomicAdd(&s.mass[~(unsigned)place >> shift], w);
+    }
+    __syncthreads();
+    constexpr int B = kSpBins / kSpThreads;
+    u64 m[B], msum = 0;
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+        m[e] = s.mass[tid * B + e];
+        msum += m[e];
+    }
+    const u64 mupto = warp_scan_u64(msum, lane);
+    if (lane == 31) s.wsum[warp] = mupto;
+    __syncthreads();
+    u64 ahead = mupto - msum, total = 0;
+    for (int i = 0; i < kSpWarps; ++i) {
+        if (i < warp) ahead += s.wsum[i];
+        total += s.wsum[i];
+    }
+    const float u = __ldg(p.uniform + r);
+    const u64 target = u >= 1.f ? total - 1 : u > 0.f ? part_of(u, total, false) : 0;
+#pragma unroll
+    for (int e = 0; e < B; ++e) {
+        if (target >= ahead && target < ahead + m[e]) {
+            s.ra[1] = tid * B + e;
+            s.rb[1] = ahead;
+        }
+        ahead += m[e];
+    }
+    __syncthreads();
+    const unsigned bin = (unsigned)s.ra[1];
+    const u64 base = s.rb[1];
+    for (int i = tid; i < n; i += kSpThreads)
+        if (weights[i] && ~(unsigned)s.few[i] >> shift == bin) s.wlist[atomicAdd(&s.n_cand, 1u)] = (unsigned)i;
+    __syncthreads();
+    const int members = (int)s.n_cand;
+    for (int a = tid; a < members; a += kSpThreads) {
+        const unsigned i = s.wlist[a];
+        const u64 place = s.few[i];
+        u64 from = base;
+        for (int b = 0; b < members; ++b) {
+            const unsigned j = s.wlist[b];
+            if ((unsigned)s.few[j] > (unsigned)place) from += weights[j];  // (the index' complement)
+        }
+        if (target >= from && target < from + weights[i]) {
+            p.tokens[r] = (int)~(unsigned)place;
+            if (p.logprob) {
+                const float l = value_of_place(place);
+                const double d = l == row.top ? 0.0 : row.distance(l);
+                p.logprob[r] = (float)(d - log(ldexp((double)total, -p.bits)));
+            }
+        }
+    }
+}
+
+// The place at which the limit (count, or with MASS a share of the weight) ends, among the row's values at or in front of `cut` that are
+// not below `floor_l`; 0 where the search has to take the whole row.
+template <bool MASS>
+__device__ __noinline__ u64 cluster_cut(const Cluster c, const Row row, int& turn, u64 cut, float floor_l, u64 limit, float share, float reach) {
+    LB_SAMPLE_SHARED;
+    const float* const x = reinterpret_cast<const float*>(lb_sample_smem + sizeof(SampleShared));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float cut_l = fmaxf(floor_l, cut ? value_of_place(cut) : -CUDART_INF_F);
+    const auto is_in = [&](float l, int i) { return l > cut_l || (l == cut_l && l > -CUDART_INF_F && place_of(l, c.first + i) >= cut); };
+    const int bins = c.size >= 4 ? kSpFine : kSpBins, share_bins = bins / c.size;
+    const float scale = (float)bins / reach;
+    const auto bin_of = [&](float l) {
+        const int b = (int)((row.top - l) * scale);
+        return b < bins - 1 ? b : bins - 1;
+    };
+    int log2 = 14;  // (a CTA's sum in units stays below 2^32)
+    while ((1 << log2) < c.n_most) ++log2;
+    const int unit = row.bits - (31 - log2);
+    for (int b = tid; b < bins; b += kSpThreads) s.fine[b] = 0;
+    __syncthreads();
+    u64 sum = 0;
+#pragma unroll 2
+    for (int i = tid; i < c.n; i += kSpThreads) {
+        const float l = x[i];
+        if (!is_in(l, i)) continue;
+        unsigned q = 1;
+        if (MASS) {
+            const u64 w = row.weight(l);
+            sum += w;
+            q = (unsigned)((w + (1ull << (unit - 1))) >> unit);
+        }
+        if (q) atomicAdd(&s.fine[bin_of(l)], q);
+    }
+    if (MASS) {
+        sum = warp_sum_u64(sum);
+        if (lane == 0) s.wsum[warp] = sum;
+        __syncthreads();
+        sum = 0;
+        for (int w = 0; w < kSpWarps; ++w) sum += s.wsum[w];
+    }
+    lb_cluster_sync();
+    u64 run = 0;
+    for (int b0 = 0; b0 < share_bins; b0 += kSpThreads) {  // this CTA's share of the bins, over the cluster
+        const int b = b0 + tid;
+        u64 n = 0;
+        if (b < share_bins)
+#pragma unroll
+            for (unsigned r = 0; r < kSpMaxCluster; ++r)  // (all under way at once)
+                if (r < c.size) n += ld_cluster_u32(remote(&s.fine[c.rank * share_bins + b], r));
+        u64 upto = warp_scan_u64(n, lane);
+        __syncthreads();
+        if (lane == 31) s.wsum[warp] = upto;
+        __syncthreads();
+        upto += run;
+        for (int w = 0; w < kSpWarps; ++w) {
+            if (w < warp) upto += s.wsum[w];
+            run += s.wsum[w];
+        }
+        if (b < share_bins) s.mass[b] = upto;
+    }
+    int t = c.exchange(turn, run, sum);
+    u64 all = 0, counted = 0;
+    for (unsigned r = 0; r < c.size; ++r) {
+        counted += s.xa[t][r];
+        all += s.xb[t][r];
+    }
+    u64 need = limit;
+    if (MASS) {
+        limit = part_of(share, all, true);
+        if (limit == 0) limit = 1;
+        need = (limit >> unit) + 1;
+    }
+    if (counted < need) return 0;
+    u64 before = 0;
+    unsigned owner = 0;
+    for (; owner + 1 < c.size && before + s.xa[t][owner] < need; ++owner) before += s.xa[t][owner];
+    u64 found = 0, base = 0;
+    if (c.rank == owner) {
+        for (int b = tid; b < share_bins; b += kSpThreads) {
+            const u64 to = before + s.mass[b], from = b ? before + s.mass[b - 1] : before;
+            if (to >= need && from < need) {
+                s.ra[t] = owner * share_bins + b;  // (this exchange's own words are free)
+                s.rb[t] = from;
+            }
+        }
+        __syncthreads();
+        found = s.ra[t];
+        base = s.rb[t];
+    }
+    t = c.answer(turn, c.rank == owner, found, base, 0);
+    // weights: units may point a bin or two aside
+    const int lo = (int)s.ra[t] - (MASS ? 2 : 0), hi = (int)s.ra[t] + (MASS ? 2 : 0);
+    base = s.rb[t];
+    if (tid == 0) s.n_cand = 0;
+    __syncthreads();
+    u64* list = s.cand;
+    sum = 0;
+#pragma unroll 2
+    for (int i = tid; i < c.n; i += kSpThreads) {
+        const float l = x[i];
+        if (!is_in(l, i)) continue;
+        const int b = bin_of(l);
+        if (MASS && b < lo) sum += row.weight(l);
+        if (b < lo || b > hi) continue;
+        const unsigned at = atomicAdd(&s.n_cand, 1u);
+        if (at < kSpCap) list[at] = place_of(l, c.first + i);
+    }
+    if (MASS) {
+        sum = warp_sum_u64(sum);
+        if (lane == 0) s.wsum[warp] = sum;
+    }
+    __syncthreads();
+    const unsigned mine = s.n_cand;
+    sum = 0;
+    if (MASS)
+        for (int w = 0; w < kSpWarps; ++w) sum += s.wsum[w];
+    t = c.exchange(turn, mine, sum);
+    unsigned from = 0, members = 0;
+    if (MASS) base = 0;
+    for (unsigned r = 0; r < c.size; ++r) {
+        if (r < c.rank) from += (unsigned)s.xa[t][r];
+        members += (unsigned)s.xa[t][r];
+        if (MASS) base += s.xb[t][r];
+    }
+    if (members > kSpCap || (MASS && base >= limit)) return 0;
+    for (unsigned i = tid; i < mine; i += kSpThreads) st_cluster_u64(remote(&s.few[from + i], 0), list[i]);
+    lb_cluster_sync();
+    u64 at = 0;
+    if (c.rank == 0) {
+        u64* w = nullptr;
+        bool reached = true;
+        if (MASS) {
+            w = s.cand;
+            u64 mass = 0;
+            for (unsigned i = tid; i < members; i += kSpThreads) {
+                w[i] = row.weight(value_of_place(s.few[i]));
+                mass += w[i];
+            }
+            mass = warp_sum_u64(mass);
+            __syncthreads();
+            if (lane == 0) s.wsum[warp] = mass;
+            __syncthreads();
+            mass = 0;
+            for (int i = 0; i < kSpWarps; ++i) mass += s.wsum[i];
+            reached = base + mass >= limit;
+            __syncthreads();
+        }
+        if (reached) at = local_cut(w, (int)members, 0, limit - base, row.top, row.far);
+    }
+    t = c.answer(turn, c.rank == 0, at, 0, 0);
     return s.ra[t];
 }
 
 __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParams p) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    SampleShared& s = *reinterpret_cast<SampleShared*>(smem_raw);
-    float* x = reinterpret_cast<float*>(smem_raw + sizeof(SampleShared));
+    LB_SAMPLE_SHARED;
+    float* x = reinterpret_cast<float*>(lb_sample_smem + sizeof(SampleShared));
     unsigned size;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-    const int r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const unsigned rank = lb_cluster_rank();
     const int first = (int)rank * p.slice, n = max(0, min(p.slice, p.vocab - first));
+    lb_cluster_arrive();  // (waited for in front of the first access to another CTA's memory)
+    if (tid < 32) s.exp2_32[tid] = exp2((double)tid / 32);
+    lb_pdl_launch_dependents();
+    lb_pdl_wait();
     const float* __restrict__ src = p.logits + (size_t)r * p.stride + first;
-    Cluster c{s, x, n, first, rank, size, 0};
+    const float temp = p.temperature ? __ldg(p.temperature + r) : 1.f;
+    const int k_asked = p.top_k ? __ldg(p.top_k + r) : 0, k = k_asked > 0 && k_asked < p.vocab ? k_asked : 0;
+    const float top_p = p.top_p ? __ldg(p.top_p + r) : 1.f;
+    const float asked = p.min_p ? __ldg(p.min_p + r) : 0.f;
+    const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;
+    const Cluster c{n, first, p.slice, rank, size};
+    int turn = 0;
 
-    // the slice, its first largest value and its smallest finite one
-    u64 best = 0;
-    float least = CUDART_INF_F;
-    const auto take = [&](int i, float l) {
-        l = l != l ? -CUDART_INF_F : l + 0.0f;  // (one zero)
-        x[i] = l;
-        const u64 at = place_of(l, first + i);
-        best = at > best ? at : best;
-        if (l > -CUDART_INF_F) least = fminf(least, l);
-    };
-    if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        for (int i = threadIdx.x; i < n / 4; i += kSpThreads) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(src) + i);
-            take(4 * i, v.x);
-            take(4 * i + 1, v.y);
-            take(4 * i + 2, v.z);
-            take(4 * i + 3, v.w);
-        }
-        for (int i = n / 4 * 4 + threadIdx.x; i < n; i += kSpThreads) take(i, __ldg(src + i));
-    } else {
-        for (int i = threadIdx.x; i < n; i += kSpThreads) take(i, __ldg(src + i));
+    // the slice and its largest value
+    float best = -CUDART_INF_F;
+    const auto clean = [](float l) { return l != l ? -CUDART_INF_F : l + 0.0f; };  // (one zero)
+    const int n4 = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? n / 4 : 0;
+#pragma unroll 4
+    for (int i = tid; i < n4; i += kSpThreads) {
+        float4 v = __ldg(reinterpret_cast<const float4*>(src) + i);
+        v = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+        *reinterpret_cast<float4*>(x + 4 * i) = v;
+        best = fmaxf(best, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     }
-    best = warp_max_u64(best);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+#pragma unroll 4
+    for (int i = n4 * 4 + tid; i < n; i += kSpThreads) {
+        const float l = clean(__ldg(src + i));
+        x[i] = l;
+        best = fmaxf(best, l);
+    }
+    // what some lanes, a warp or some warps together have read is a group: the smallest of the groups' largest values
+    int lanes = 32;  // lanes a group, then warps a group: as many as leave k groups
+    while (lanes > 1 && (int)size * (kSpThreads / lanes) < k) lanes /= 2;
+    float bound = best;
+    for (int o = 1; o < lanes; o *= 2) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+    bound = -lb_warp_max(-bound);
+    best = lb_warp_max(best);
     if (lane == 0) {
-        s.wsum[warp] = best;
-        s.wcount[warp] = __float_as_uint(least);
+        s.wf[warp] = best;
+        s.wcount[warp] = __float_as_uint(bound);
     }
     __syncthreads();
-    for (int w = 0; w < kSpWarps; ++w) {
-        best = s.wsum[w] > best ? s.wsum[w] : best;
-        least = fminf(least, __uint_as_float(s.wcount[w]));
+    int per = 1;
+    while (lanes == 32 && per < kSpWarps && (int)size * (kSpWarps / (per * 2)) >= k) per *= 2;
+    bound = CUDART_INF_F;
+    for (int w = 0; w < kSpWarps; w += per) {
+        float group = __uint_as_float(s.wcount[w]);
+        for (int v = 1; v < per; ++v) group = fmaxf(group, __uint_as_float(s.wcount[w + v]));
+        bound = fminf(bound, group);
     }
-    lb_cluster_sync();  // every CTA of the cluster runs: its shared memory may be written
-    const int t0 = c.exchange(best, __float_as_uint(least));
+    for (int w = 0; w < kSpWarps; ++w) best = fmaxf(best, s.wf[w]);
+    lb_cluster_wait();
+    const int t0 = c.exchange(turn, (u64)key_of(best), (u64)key_of(bound));
+    unsigned best_key = key_of(best), bound_key = key_of(bound);
     for (unsigned q = 0; q < size; ++q) {
-        best = s.xa[t0][q] > best ? s.xa[t0][q] : best;
-        least = fminf(least, __uint_as_float((unsigned)s.xb[t0][q]));
+        best_key = max(best_key, (unsigned)s.xa[t0][q]);
+        bound_key = min(bound_key, (unsigned)s.xb[t0][q]);
     }
-    const unsigned best_key = (unsigned)(best >> 32);
     Row row;
-    row.top = __uint_as_float(best_key & 0x80000000u ? best_key & 0x7fffffffu : ~best_key);
+    row.top = value_of_key(best_key);
     row.bits = p.bits;
-    const float temp = p.temperature ? __ldg(p.temperature + r) : 1.f;
-    const bool writes = rank == 0 && threadIdx.x == 0;
     if (row.top == -CUDART_INF_F) {  // nothing to choose
-        if (writes) {
+        if (rank == 0 && tid == 0) {
             p.tokens[r] = -1;
             if (p.logprob) p.logprob[r] = CUDART_NAN_F;
         }
         return;
     }
-    if (!(temp > 0.f)) {  // (not a number: too)
-        if (writes) {
-            p.tokens[r] = (int)~(unsigned)best;
+    if (!(temp > 0.f)) {  // (not a number: too) the first largest value
+        unsigned at = 0xffffffffu;
+        for (int i = tid; i < n; i += kSpThreads)
+            if (x[i] == row.top) at = min(at, (unsigned)(first + i));
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) s.wcount[warp] = at;
+        __syncthreads();
+        for (int w = 0; w < kSpWarps; ++w) at = min(at, s.wcount[w]);
+        const int t = c.exchange(turn, at, 0);
+        for (unsigned q = 0; q < size; ++q) at = min(at, (unsigned)s.xa[t][q]);
+        if (rank == 0 && tid == 0) {
+            p.tokens[r] = (int)at;
             if (p.logprob) p.logprob[r] = 0.f;
         }
         return;
     }
     row.inv_t = 1.0 / (double)temp;
-    row.bin_scale = (float)kSpBins / fminf(32.f * temp, row.top - least);
+    row.far = 48.f * temp;
+
+    // a value that no kept one is below, where one is known
+    float floor_l = -CUDART_INF_F;
+    const bool groups = k && (int)size * kSpThreads >= k;
+    bool few = false;  // whether not many values can be left
+    if (p.vocab <= kSpFew && (k || top_p < 1.f || min_p > 0.f)) {
+        few = true;
+    } else if (k) {
+        if (groups) floor_l = value_of_key(bound_key);
+        few = k <= kSpFew / 8;
+    } else if (min_p > 0.f && top_p >= 1.f && row.top < CUDART_INF_F) {
+        few = true;
+        floor_l = row.top + logf(min_p) * temp * 1.0001f - fabsf(row.top) * 1e-6f;
+    }
+    if (floor_l != floor_l) floor_l = -CUDART_INF_F;  // (no distance at an infinite temperature)
+    if (few) {
+        u64* list = s.mass;  // and s.cand behind it
+        if (tid == 0) s.n_cand = 0;
+        __syncthreads();
+        for (int i0 = 0; i0 < n; i0 += kSpThreads) {
+            const int i = i0 + tid;
+            const bool is = i < n && x[i] >= floor_l;
+            const unsigned hit = __ballot_sync(0xffffffffu, is);
+            unsigned at = 0;
+            if (lane == 0 && hit) at = atomicAdd(&s.n_cand, (unsigned)__popc(hit));
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(hit & ((1u << lane) - 1u));
+            if (is && at < kSpFew) list[at] = place_of(x[i], first + i);
+        }
+        __syncthreads();
+        const unsigned mine = s.n_cand;
+        const int t = c.exchange(turn, mine, 0);
+        unsigned from = 0, left = 0;
+        for (unsigned q = 0; q < size; ++q) {
+            if (q < rank) from += (unsigned)s.xa[t][q];
+            left += (unsigned)s.xa[t][q];
+        }
+        if (left <= kSpFew) {
+            for (unsigned i = tid; i < mine; i += kSpThreads) st_cluster_u64(remote(&s.few[from + i], 0), list[i]);
+            lb_cluster_sync();
+            if (rank == 0) choose(row, p, r, (int)left, k, top_p, min_p);
+            return;
+        }
+    }
 
     u64 cut = 0;
-    const int k = p.top_k ? __ldg(p.top_k + r) : 0;
-    if (k > 0 && k < p.vocab) cut = find_cut(c, row, cut, false, (u64)k, -1.f);
-    const float top_p = p.top_p ? __ldg(p.top_p + r) : 1.f;
-    if (top_p < 1.f) cut = find_cut(c, row, cut, true, 1, fmaxf(top_p, 0.f));
-    const float asked = p.min_p ? __ldg(p.min_p + r) : 0.f;
-    const float min_p = asked > 0.f ? fminf(asked, 1.f) : 0.f;
+    float scale = 0.f;
+    const auto whole_scale = [&]() {  // of the whole row's bins
+        if (scale != 0.f) return;
+        float least = CUDART_INF_F;
+        for (int i = tid; i < n; i += kSpThreads)
+            if (x[i] > -CUDART_INF_F) least = fminf(least, x[i]);
+        least = -lb_warp_max(-least);
+        __syncthreads();
+        if (lane == 0) s.wf[warp] = least;
+        __syncthreads();
+        for (int w = 0; w < kSpWarps; ++w) least = fminf(least, s.wf[w]);
+        const int t = c.exchange(turn, __float_as_uint(least), 0);
+        for (unsigned q = 0; q < size; ++q) least = fminf(least, __uint_as_float((unsigned)s.xa[t][q]));
+        row.bin_scale = scale = (float)kSpBins / fminf(32.f * temp, row.top - least);
+    };
+    const bool plain = row.top < CUDART_INF_F;
+    if (k) {
+        if (plain && groups && floor_l > -CUDART_INF_F) cut = cluster_cut<false>(c, row, turn, 0, floor_l, (u64)k, 0.f, row.top - floor_l);
+        if (cut == 0) {
+            whole_scale();
+            cut = find_cut(c, row, turn, 0, false, (u64)k, -1.f);
+        }
+    }
+    if (top_p < 1.f) {
+        u64 at = 0;
+        if (plain) at = cluster_cut<true>(c, row, turn, cut, -CUDART_INF_F, 0, fmaxf(top_p, 0.f), kSpReach * temp);
+        if (at == 0) {
+            whole_scale();
+            at = find_cut(c, row, turn, cut, true, 1, fmaxf(top_p, 0.f));
+        }
+        cut = at;
+    }
+    const float cut_l = cut ? value_of_place(cut) : -CUDART_INF_F;
     const double log_min = min_p > 0.f ? log((double)min_p) : -CUDART_INF;
     const auto kept = [&](int i) -> u64 {
         const float l = x[i];
-        if (place_of(l, first + i) < cut) return 0;
+        if (l < cut_l || (l == cut_l && place_of(l, first + i) < cut)) return 0;
         if (min_p > 0.f) {
             if (row.top == CUDART_INF_F ? l != row.top : l == -CUDART_INF_F) return 0;
             const double d = l == row.top ? 0.0 : row.distance(l);
@@ -492,17 +960,17 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
         return row.weight(l);
     };
     // kept weight by warp, whose stretches follow one another
-    const int per = (n + kSpWarps * 32 - 1) / (kSpWarps * 32) * 32;
-    const int from = min(n, warp * per), to = min(n, from + per);
+    const int stretch = (n + kSpWarps * 32 - 1) / (kSpWarps * 32) * 32;
+    const int from = min(n, warp * stretch), to = min(n, from + stretch);
     u64 mine = 0;
     for (int i = from + lane; i < to; i += 32) mine += kept(i);
     mine = warp_sum_u64(mine);
     __syncthreads();
     if (lane == 0) s.wsum[warp] = mine;
     __syncthreads();
-    u64 all = 0;
-    for (int w = 0; w < kSpWarps; ++w) all += s.wsum[w];
-    const int t = c.exchange(all, 0);
+    u64 here = 0;
+    for (int w = 0; w < kSpWarps; ++w) here += s.wsum[w];
+    const int t = c.exchange(turn, here, 0);
     u64 total = 0, ahead = 0;
     for (unsigned q = 0; q < size; ++q) {
         if (q < rank) ahead += s.xa[t][q];
@@ -510,7 +978,7 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
     }
     const float u = __ldg(p.uniform + r);
     const u64 target = u >= 1.f ? total - 1 : u > 0.f ? part_of(u, total, false) : 0;
-    if (target < ahead || target >= ahead + all) return;
+    if (target < ahead || target >= ahead + here) return;
     for (int w = 0; w < warp; ++w) ahead += s.wsum[w];
     if (target < ahead || target >= ahead + s.wsum[warp]) return;
     for (int i0 = from; i0 < to; i0 += 32) {
@@ -531,10 +999,10 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
 
 }  // namespace
 
-// bytes of shared memory and CTAs of a row's cluster
-static int sample_cluster(int vocab) {
+// CTAs of a row's cluster: 2048 logits each for few rows, up to 16,384 where the rows fill the device
+static int sample_cluster(const loom_b200_ctx* ctx, int rows, int vocab) {
     int size = 1;
-    while (size < kSpMaxCluster && (vocab + size - 1) / size > 8192) size *= 2;
+    while (size < kSpMaxCluster && (vocab + size - 1) / size > (rows * size * 2 <= ctx->sm_count * 2 ? 2048 : 16384)) size *= 2;
     return size;
 }
 
@@ -544,7 +1012,7 @@ int lb_launch_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logit
     p.logits = logits;
     p.stride = stride;
     p.vocab = vocab;
-    const int size = sample_cluster(vocab);
+    const int size = sample_cluster(ctx, rows, vocab);
     p.slice = ((vocab + size - 1) / size + 3) / 4 * 4;
     int log2 = 0;
     while (((long long)1 << log2) < (long long)vocab + 1) ++log2;
@@ -554,7 +1022,7 @@ int lb_launch_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logit
     p.top_p = top_p;
     p.min_p = min_p;
     p.uniform = uniform;
-    const size_t smem = sizeof(SampleShared) + (size_t)p.slice * 4;
+    const size_t slice = (size_t)p.slice * 4, smem = sizeof(SampleShared) + (slice > kSpLeast ? slice : kSpLeast);
     if (!(ctx->func_attr_mask2 & (1u << 28))) {
         LB_CUDA(ctx, cudaFuncSetAttribute(lb_sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(SampleShared) + (size_t)kSpMaxSlice * 4)));
         LB_CUDA(ctx, cudaFuncSetAttribute(lb_sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -575,13 +1043,15 @@ int lb_launch_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logit
         cfg.blockDim = dim3(kSpThreads);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = ctx->stream;
-        cudaLaunchAttribute attr[1];
+        cudaLaunchAttribute attr[2];
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = size;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
+        cfg.numAttrs = ctx->opt_pdl ? 2 : 1;
         LB_CUDA(ctx, cudaLaunchKernelEx(&cfg, lb_sample_kernel, p));
         ctx->launches++;
     }

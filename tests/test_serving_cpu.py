@@ -45,7 +45,7 @@ def test_sample_refusals(fakes):
     refused(f, call(u=None), INVALID, "NULL")
     refused(f, call(out=None), INVALID, "NULL")
     refused(f, call(stride=9), INVALID, "stride 9")
-    refused(f, call(vocab=737281, stride=737281), UNSUPPORTED, "737280")
+    refused(f, call(vocab=655361, stride=655361), UNSUPPORTED, "655360")
 
 
 def test_adapter_refusals(fakes):
