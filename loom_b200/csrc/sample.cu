@@ -19,16 +19,18 @@
 //           free for the next rows.  top-k: with G >= k groups of tokens, at least k values reach the smallest of the groups' largest
 //           ones, of values in random order about G ln G do (270 for k up to 64); min-p: the values not below it; small vocabularies: all.  2048
 //           values at most
-//   cluster the CTAs' histograms are added up through distributed shared memory.  Weights enter them in units of 2^-17 of the largest, by
+//   cluster the CTAs' histograms are added up through distributed shared memory.  Weights enter them in units of 2^-22 of the largest, by
 //           32-bit atomics: they say which bins to look at, and what lies in front of those is then added up exactly
 //   whole   the same with exact weights, bins divided further by the bits of the values down to a single value, whose ties go by index: long
 //           stretches of equal or nearly equal logits, top-p next to 1
 //
-// Weights are exp2 of a double by a table of 32 entries and a polynomial (P. T. P. Tang, Table-driven implementation of the exponential
-// function, ACM TOMS 15, 1989): eleven float64 operations at 64 lanes a clock and one conversion; error 2^-48 of the value.
+// Weights near the largest are exp2 of a double by a table of 32 entries and a polynomial (P. T. P. Tang, Table-driven implementation of the
+// exponential function, ACM TOMS 15, 1989), error 2^-48; the many others take a float32 exponential of a distance that is exact.
 #include "common.cuh"
 
 #include <math_constants.h>
+
+#include <cstddef>
 
 namespace {
 
@@ -38,7 +40,9 @@ constexpr int kSpBins = 1024;
 constexpr int kSpFine = 4096;       // bins of a cluster of four CTAs and more
 constexpr int kSpCap = 1024;        // values of one bin that are ranked among each other
 constexpr int kSpFew = 2048;        // values that the first CTA sorts
-constexpr float kSpReach = 12.5f;   // distances that histograms of weights take, in temperatures: beyond them a weight is less than half a unit
+constexpr int kSpList = kSpFew / kSpWarps;  // values of a warp's list
+constexpr int kSpStretch = 1024;   // places of a warp's list: its share of the bins' room
+constexpr float kSpReach = 16.f;   // distances that histograms of weights take, in temperatures: beyond them a weight is less than half a unit
 constexpr int kSpMaxSlice = 40960;  // logits of a CTA: 160 KB
 constexpr int kSpMaxCluster = 16;
 
@@ -87,6 +91,7 @@ struct __align__(16) SampleShared {  // (the slice behind it is written sixteen 
     extern __shared__ __align__(16) uint8_t lb_sample_smem[]; \
     SampleShared& s = *reinterpret_cast<SampleShared*>(lb_sample_smem)
 static_assert(sizeof(SampleShared) % 16 == 0, "alignment of the slice");
+static_assert((kSpBins + kSpCap + kSpFew) * 8 >= kSpWarps * kSpStretch * 2 && offsetof(SampleShared, few) == offsetof(SampleShared, mass) + (kSpBins + kSpCap) * 8, "lists over the bins");
 static_assert(kSpBins + kSpCap >= kSpFew, "the values that are left, in the place of the bins");
 constexpr size_t kSpLeast = (size_t)kSpFew * 8;  // bytes of the slice's place, where the first CTA keeps weights later
 static_assert(sizeof(SampleShared) + (size_t)kSpMaxSlice * 4 <= 227 * 1024, "shared memory of a CTA");
@@ -153,6 +158,7 @@ __device__ __forceinline__ u64 part_of(float f, u64 total, bool up) {
 struct Row {
     float top;     // the largest logit
     double inv_t;
+    float inv_hi, inv_lo;  // log2(e) / temperature as two floats
     float bin_scale;
     float far;     // no weight beyond it: 48 temperatures
     int bits;
@@ -178,10 +184,23 @@ struct Row {
         e = __hiloint2double(__double2hiint(e) + ((n >> 5) + bits) * (1 << 20), __double2loint(e));
         return __double2ull_rn(e);
     }
+    // Beyond four temperatures a float32 exponential will do: its error, 2^-21 of the value, is 2^-27 of the largest weight, and the sums
+    // that a choice hangs on are off by a few 10^-9 of it.  The distance itself is the exact difference, as two floats.
     __device__ __forceinline__ u64 weight(float l) const {
-        if (l == top) return 1ull << bits;
-        if (top == CUDART_INF_F || l == -CUDART_INF_F) return 0;
-        return weight_at(distance(l));
+        const float far_l = l - top;
+        const float y = far_l * inv_hi;
+        if (!(y <= -4.f * 1.442695f)) {  // near, equal or not a number
+            if (l == top) return 1ull << bits;
+            if (top == CUDART_INF_F || l == -CUDART_INF_F) return 0;
+            return weight_at(distance(l));
+        }
+        if (!(y > -62.f)) return 0;
+        const float back = far_l - l, rest = (l - (far_l - back)) - (top + back);
+        const float z = fmaf(rest, inv_hi, fmaf(far_l, inv_lo, fmaf(far_l, inv_hi, -y)));
+        const float k = y + 12582912.f;  // 1.5 2^23: its low bits are y rounded
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((y - (k - 12582912.f)) + z));
+        return __float2ull_rn(__int_as_float(__float_as_int(e) + (__float_as_int(k) - 0x4b400000 + bits) * (1 << 23)));
     }
     __device__ __forceinline__ int bin(float l) const {
         const int b = (int)((top - l) * bin_scale);  // (not a number, from equal infinities: 0)
@@ -448,170 +467,186 @@ __device__ __noinline__ u64 find_cut(const Cluster c, const Row row, int& turn, 
 __device__ __forceinline__ float value_of_key(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ float value_of_place(u64 place) { return value_of_key((unsigned)(place >> 32)); }
 
-// Among the n <= kSpFew places in s.few that are at or in front of `cut`, with weights `w` (in shared memory; null: 1 each): the place of the last one that the limit
-// lets through, the first one with which they reach it.  limit >= 1 and at most what there is.  Values further
-// than `far` below the largest one have no weight: where the limit falls among them the place is 0, that is, all.  All of one CTA's threads.
-__device__ __noinline__ u64 local_cut(const u64* w, int n, u64 cut, u64 limit, float top, float far) {
+// Sorts the n <= kSpFew places in s.few, into bins and then within them: by value, largest first, or by index.  By value, those further than `far`
+// below the largest have no weight and are left out: how many there are then.  All of one CTA's threads.
+template <bool INDEX>
+__device__ __noinline__ int sort_few(int n, float far, int shift) {
     LB_SAMPLE_SHARED;
-    const u64* v = s.few;
-    __builtin_assume(__isShared(w));
+    u64* sorted = s.mass;  // and s.cand behind it
+    unsigned *count = s.wlist, *start = s.wlist + kSpBins;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    float least = CUDART_INF_F;
-    for (int i = tid; i < n; i += kSpThreads)
-        if (v[i] >= cut && (!w || w[i])) least = fminf(least, value_of_place(v[i]));
-    least = -lb_warp_max(-least);
-    __syncthreads();
-    if (lane == 0) s.wf[warp] = least;
-    for (int b = tid; b < kSpBins; b += kSpThreads) s.mass[b] = 0;
-    __syncthreads();
-    for (int i = 0; i < kSpWarps; ++i) least = fminf(least, s.wf[i]);
-    const float scale = (float)kSpBins / fminf(top - least, far);
-    const auto bin_of = [&](u64 place) {
-        const int b = (int)((top - value_of_place(place)) * scale);  // (not a number, from equal ones: 0)
-        return b < kSpBins - 1 ? b : kSpBins - 1;
-    };
-    for (int i = tid; i < n; i += kSpThreads)
-        if (v[i] >= cut) {
-            const u64 x = w ? w[i] : 1;
-            if (x) atomicAdd(&s.mass[bin_of(v[i])], x);
+    constexpr int E = kSpFew / kSpThreads, B = kSpBins / kSpThreads;
+    u64 v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = tid + e * kSpThreads < n ? s.few[tid + e * kSpThreads] : 0;
+    float top = -CUDART_INF_F, scale = 0.f;
+    if (!INDEX) {
+        float least = CUDART_INF_F;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (v[e]) {
+                const float l = value_of_place(v[e]);
+                top = fmaxf(top, l);
+                least = fminf(least, l);
+            }
+        least = -lb_warp_max(-least);
+        top = lb_warp_max(top);
+        if (lane == 0) {
+            s.wf[warp] = least;
+            s.wcount[warp] = __float_as_uint(top);
         }
-    if (tid == 0) {
-        s.n_cand = 0;
-        s.rc[0] = 0;
+    }
+    for (int b = tid; b < kSpBins; b += kSpThreads) count[b] = 0;
+    __syncthreads();
+    if (!INDEX) {
+        float least = CUDART_INF_F;
+        for (int w = 0; w < kSpWarps; ++w) {
+            least = fminf(least, s.wf[w]);
+            top = fmaxf(top, __uint_as_float(s.wcount[w]));
+        }
+        scale = 1.f / fminf(top - least, far);
+    }
+    int bin[E];
+    unsigned slot[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        bin[e] = -1;
+        if (v[e]) {
+            if (INDEX) {
+                bin[e] = (int)(~(unsigned)v[e] >> shift);
+            } else {
+                const float d = top - value_of_place(v[e]);
+                // finer towards the far end, where most values are (not a number, from equal ones: 0)
+                if (!(d > far)) bin[e] = kSpBins - 1 - min((int)(sqrtf(fmaxf(1.f - d * scale, 0.f)) * kSpBins), kSpBins - 1);
+            }
+            if (bin[e] >= 0) slot[e] = atomicAdd(&count[bin[e]], 1u);
+        }
     }
     __syncthreads();
-    constexpr int B = kSpBins / kSpThreads;
-    u64 m[B], sum = 0;
+    unsigned m[B], sum = 0;
 #pragma unroll
     for (int e = 0; e < B; ++e) {
-        m[e] = s.mass[tid * B + e];
+        m[e] = count[tid * B + e];
         sum += m[e];
     }
-    const u64 upto = warp_scan_u64(sum, lane);
+    unsigned upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned u = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += u;
+    }
     if (lane == 31) s.wsum[warp] = upto;
     __syncthreads();
-    u64 ahead = upto - sum;
-    for (int i = 0; i < warp; ++i) ahead += s.wsum[i];
+    unsigned all = 0, ahead = upto - sum;
+    for (int w = 0; w < kSpWarps; ++w) {
+        if (w < warp) ahead += (unsigned)s.wsum[w];
+        all += (unsigned)s.wsum[w];
+    }
 #pragma unroll
     for (int e = 0; e < B; ++e) {
-        if (ahead < limit && ahead + m[e] >= limit) {
-            s.ra[0] = tid * B + e;
-            s.rb[0] = ahead;
-        }
+        start[tid * B + e] = ahead;
         ahead += m[e];
     }
     __syncthreads();
-    const int bin = (int)s.ra[0];
-    const u64 base = s.rb[0];
-    if (!w && bin == kSpBins - 1 && !(top - least <= far)) return 0;
-    unsigned* list = s.wlist;
-    for (int i = tid; i < n; i += kSpThreads)
-        if (v[i] >= cut && bin_of(v[i]) == bin) list[atomicAdd(&s.n_cand, 1u)] = (unsigned)i;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (bin[e] >= 0) sorted[start[bin[e]] + slot[e]] = v[e];
     __syncthreads();
-    const int members = (int)s.n_cand;
-    for (int a = tid; a < members; a += kSpThreads) {
-        const unsigned i = list[a];
-        const u64 mine = v[i], x = w ? w[i] : 1;
-        u64 before = base;
-        for (int b = 0; b < members; ++b) {
-            const unsigned j = list[b];
-            if (v[j] > mine) before += w ? w[j] : 1;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (bin[e] >= 0) {
+            const unsigned from = start[bin[e]], to = from + count[bin[e]];
+            unsigned at = from;
+            for (unsigned j = from; j < to; ++j) at += INDEX ? (unsigned)sorted[j] > (unsigned)v[e] : sorted[j] > v[e];  // (the index' complement)
+            s.few[at] = v[e];
         }
-        if (before < limit && before + x >= limit) s.rc[0] = mine;
-    }
     __syncthreads();
-    return s.rc[0];
+    return (int)all;
 }
 
-// What the first CTA does with the n values that are left (in s.few): cuts, kept weight, token.
-__device__ __noinline__ void choose(const Row row, const SampleParams p, int r, int n, int k, float top_p, float min_p) {
+// Weights of the first n of s.few, four neighbours a thread, and the sum in front of the thread's; the sum of all.
+constexpr int kSpEach = kSpFew / kSpThreads;
+__device__ __forceinline__ u64 weights_of_few(const Row& row, int n, u64 (&w)[kSpEach], u64& before) {
     LB_SAMPLE_SHARED;
-    u64* weights = reinterpret_cast<u64*>(lb_sample_smem + sizeof(SampleShared));  // (the slice has been read)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    u64 cut = 0;
-    if (k > 0 && k < n) cut = local_cut(nullptr, n, 0, (u64)k, row.top, row.far);
-    u64 mass = 0;
-    const double log_min = min_p > 0.f ? log((double)min_p) : -CUDART_INF;
-    for (int i = tid; i < n; i += kSpThreads) {
-        const u64 place = s.few[i], w = place >= cut ? row.weight(value_of_place(place)) : 0;
-        weights[i] = w;
-        mass += w;
+    u64 sum = 0;
+#pragma unroll
+    for (int e = 0; e < kSpEach; ++e) {
+        const int i = tid * kSpEach + e;
+        w[e] = i < n ? row.weight(value_of_place(s.few[i])) : 0;
+        sum += w[e];
     }
+    const u64 upto = warp_scan_u64(sum, lane);
+    __syncthreads();
+    if (lane == 31) s.wsum[warp] = upto;
+    __syncthreads();
+    u64 all = 0;
+    before = upto - sum;
+    for (int i = 0; i < kSpWarps; ++i) {
+        if (i < warp) before += s.wsum[i];
+        all += s.wsum[i];
+    }
+    return all;
+}
+
+// What the first CTA does with the n values that are left (in s.few): cuts, kept weight, token.  `given`: the weight that top-p wants, where that
+// is a share of the whole row's; else 0.
+__device__ __noinline__ void choose(const Row row, const SampleParams p, int r, int n, int k, float top_p, float min_p, u64 given) {
+    LB_SAMPLE_SHARED;
+    const int tid = threadIdx.x, lane = tid & 31;
+    n = sort_few<false>(n, row.far, 0);
+    u64 w[kSpEach], before;
+    u64 mass = weights_of_few(row, n, w, before);
+    const int first = k > 0 && k < n ? k : n;  // top-k
+    if (first < n) {
+        u64 upto = before;
+#pragma unroll
+        for (int e = 0; e < kSpEach; ++e) {
+            upto += w[e];
+            if (tid * kSpEach + e == first - 1) s.ra[0] = upto;
+        }
+        __syncthreads();
+        mass = s.ra[0];
+    }
+    u64 need = ~0ull;
     if (top_p < 1.f) {
-        mass = warp_sum_u64(mass);
-        __syncthreads();
-        if (lane == 0) s.wsum[warp] = mass;
-        __syncthreads();
-        mass = 0;
-        for (int i = 0; i < kSpWarps; ++i) mass += s.wsum[i];
-        u64 need = part_of(fmaxf(top_p, 0.f), mass, true);
+        need = given ? given : part_of(fmaxf(top_p, 0.f), mass, true);
         if (need == 0) need = 1;
-        __syncthreads();
-        const u64 at = local_cut(weights, n, cut, need, row.top, row.far);
-        cut = at > cut ? at : cut;
     }
-    __syncthreads();
-    for (int b = tid; b < kSpBins; b += kSpThreads) s.mass[b] = 0;
     if (tid == 0) s.n_cand = 0;
-    __syncthreads();
-    // by index: weights over stretches of indices, the stretch that the random number falls into, the place in it
-    int shift = 0;
-    while ((p.vocab - 1) >> shift >= kSpBins) ++shift;
-    for (int i = tid; i < n; i += kSpThreads) {
-        const u64 place = s.few[i];
-        u64 w = place >= cut ? weights[i] : 0;
-        if (w && min_p > 0.f) {
-            const float l = value_of_place(place);
+    const double log_min = min_p > 0.f ? log((double)min_p) : -CUDART_INF;
+    // kept: a run from the front
+    unsigned kept = 0;
+#pragma unroll
+    for (int e = 0; e < kSpEach; ++e) {
+        const int i = tid * kSpEach + e;
+        bool is = i < first && before < need && w[e] > 0;
+        if (is && min_p > 0.f) {
+            const float l = value_of_place(s.few[i]);
             if (l != row.top) {
                 const double d = row.distance(l);
-                if (!(d > log_min + 1e-6 || (d > log_min - 1e-6 && exp(d) >= (double)min_p))) w = 0;
+                is = d > log_min + 1e-6 || (d > log_min - 1e-6 && exp(d) >= (double)min_p);
             }
         }
-        weights[i] = w;
-        if (w) atomicAdd(&s.mass[~(unsigned)place >> shift], w);
+        kept += is;
+        before += w[e];
     }
+    kept = __reduce_add_sync(0xffffffffu, kept);
     __syncthreads();
-    constexpr int B = kSpBins / kSpThreads;
-    u64 m[B], msum = 0;
-#pragma unroll
-    for (int e = 0; e < B; ++e) {
-        m[e] = s.mass[tid * B + e];
-        msum += m[e];
-    }
-    const u64 mupto = warp_scan_u64(msum, lane);
-    if (lane == 31) s.wsum[warp] = mupto;
+    if (lane == 0 && kept) atomicAdd(&s.n_cand, kept);
     __syncthreads();
-    u64 ahead = mupto - msum, total = 0;
-    for (int i = 0; i < kSpWarps; ++i) {
-        if (i < warp) ahead += s.wsum[i];
-        total += s.wsum[i];
-    }
+    kept = s.n_cand;
+    // by index
+    int shift = 0;
+    while ((p.vocab - 1) >> shift >= kSpBins) ++shift;
+    sort_few<true>((int)kept, 0.f, shift);
+    const u64 total = weights_of_few(row, (int)kept, w, before);
     const float u = __ldg(p.uniform + r);
     const u64 target = u >= 1.f ? total - 1 : u > 0.f ? part_of(u, total, false) : 0;
 #pragma unroll
-    for (int e = 0; e < B; ++e) {
-        if (target >= ahead && target < ahead + m[e]) {
-            s.ra[1] = tid * B + e;
-            s.rb[1] = ahead;
-        }
-        ahead += m[e];
-    }
-    __syncthreads();
-    const unsigned bin = (unsigned)s.ra[1];
-    const u64 base = s.rb[1];
-    for (int i = tid; i < n; i += kSpThreads)
-        if (weights[i] && ~(unsigned)s.few[i] >> shift == bin) s.wlist[atomicAdd(&s.n_cand, 1u)] = (unsigned)i;
-    __syncthreads();
-    const int members = (int)s.n_cand;
-    for (int a = tid; a < members; a += kSpThreads) {
-        const unsigned i = s.wlist[a];
-        const u64 place = s.few[i];
-        u64 from = base;
-        for (int b = 0; b < members; ++b) {
-            const unsigned j = s.wlist[b];
-            if ((unsigned)s.few[j] > (unsigned)place) from += weights[j];  // (the index' complement)
-        }
-        if (target >= from && target < from + weights[i]) {
+    for (int e = 0; e < kSpEach; ++e) {
+        if (target >= before && target < before + w[e]) {
+            const u64 place = s.few[tid * kSpEach + e];
             p.tokens[r] = (int)~(unsigned)place;
             if (p.logprob) {
                 const float l = value_of_place(place);
@@ -619,13 +654,15 @@ __device__ __noinline__ void choose(const Row row, const SampleParams p, int r, 
                 p.logprob[r] = (float)(d - log(ldexp((double)total, -p.bits)));
             }
         }
+        before += w[e];
     }
 }
 
 // The place at which the limit (count, or with MASS a share of the weight) ends, among the row's values at or in front of `cut` that are
-// not below `floor_l`; 0 where the search has to take the whole row.
+// not below `floor_l`; 0 where the search has to take the whole row; kSpDone where few values were left and the first CTA has seen to them.
+constexpr u64 kSpDone = ~0ull;
 template <bool MASS>
-__device__ __noinline__ u64 cluster_cut(const Cluster c, const Row row, int& turn, u64 cut, float floor_l, u64 limit, float share, float reach) {
+__device__ __noinline__ u64 cluster_cut(const Cluster c, const Row row, int& turn, u64 cut, float floor_l, u64 limit, float share, float reach, const SampleParams p, int r, int k, float top_p, float min_p) {
     LB_SAMPLE_SHARED;
     const float* const x = reinterpret_cast<const float*>(lb_sample_smem + sizeof(SampleShared));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -637,9 +674,8 @@ __device__ __noinline__ u64 cluster_cut(const Cluster c, const Row row, int& tur
         const int b = (int)((row.top - l) * scale);
         return b < bins - 1 ? b : bins - 1;
     };
-    int log2 = 14;  // (a CTA's sum in units stays below 2^32)
-    while ((1 << log2) < c.n_most) ++log2;
-    const int unit = row.bits - (31 - log2);
+    int unit = row.bits - 22;
+again:
     for (int b = tid; b < bins; b += kSpThreads) s.fine[b] = 0;
     __syncthreads();
     u64 sum = 0;
@@ -683,10 +719,17 @@ __device__ __noinline__ u64 cluster_cut(const Cluster c, const Row row, int& tur
         if (b < share_bins) s.mass[b] = upto;
     }
     int t = c.exchange(turn, run, sum);
-    u64 all = 0, counted = 0;
+    u64 all = 0, counted = 0, most = 0;
     for (unsigned r = 0; r < c.size; ++r) {
         counted += s.xa[t][r];
         all += s.xb[t][r];
+        most = s.xb[t][r] > most ? s.xb[t][r] : most;
+    }
+    if (MASS && (most >> unit) >= 0xf0000000ull) {  // (a bin may have passed 2^32: larger units, in which no CTA's sum does)
+        int log2 = 14;
+        while ((1 << log2) < c.n_most) ++log2;
+        unit = row.bits - (31 - log2);
+        goto again;
     }
     u64 need = limit;
     if (MASS) {
@@ -713,69 +756,136 @@ __device__ __noinline__ u64 cluster_cut(const Cluster c, const Row row, int& tur
     }
     t = c.answer(turn, c.rank == owner, found, base, 0);
     // weights: units may point a bin or two aside
-    const int lo = (int)s.ra[t] - (MASS ? 2 : 0), hi = (int)s.ra[t] + (MASS ? 2 : 0);
+    const int lo = (int)s.ra[t] - (MASS ? 3 : 0), hi = (int)s.ra[t] + (MASS ? 3 : 0);
     base = s.rb[t];
     if (tid == 0) s.n_cand = 0;
     __syncthreads();
-    u64* list = s.cand;
-    sum = 0;
+    // the values down to that bin (the lowest value that can be in one saves the others' bins)
+    const float low_l = hi >= bins - 1 ? -CUDART_INF_F : row.top - (float)(hi + 2) / scale;
+    unsigned window = 0, mine = 0;
+    unsigned* list = s.wlist + warp * kSpList;
 #pragma unroll 2
-    for (int i = tid; i < c.n; i += kSpThreads) {
+    for (int i0 = 0; i0 < c.n; i0 += kSpThreads) {
+        const int i = i0 + tid;
+        const float l = i < c.n ? x[i] : -CUDART_INF_F;
+        bool is = l >= low_l && is_in(l, i);
+        if (is) {
+            const int b = bin_of(l);
+            is = b <= hi;
+            window += is && b >= lo;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, is), at = mine + __popc(hit & ((1u << lane) - 1u));
+        if (is && at < kSpList) list[at] = (unsigned)i;
+        mine += __popc(hit);
+    }
+    const bool listed = mine <= kSpList;  // (this warp's)
+    window = __reduce_add_sync(0xffffffffu, window);
+    if (lane == 0) {
+        s.wcount[warp] = window;
+        s.wsum[warp] = mine;
+    }
+    const int all_listed = __syncthreads_and(listed);
+    unsigned near = 0, ahead = 0;
+    window = 0;
+    for (int w = 0; w < kSpWarps; ++w) {
+        window += s.wcount[w];
+        if (w < warp) ahead += (unsigned)s.wsum[w];
+        near += (unsigned)s.wsum[w];
+    }
+    if (!all_listed) near += kSpFew;  // (then there is no list to give away)
+    t = c.exchange(turn, near, window);
+    unsigned from = 0, wfrom = 0, members = 0, left = 0;
+    for (unsigned q = 0; q < c.size; ++q) {
+        if (q < c.rank) {
+            from += (unsigned)s.xa[t][q];
+            wfrom += (unsigned)s.xb[t][q];
+        }
+        left += (unsigned)s.xa[t][q];
+        members += (unsigned)s.xb[t][q];
+    }
+    if (left <= kSpFew) {
+        for (unsigned a = lane; a < mine; a += 32) st_cluster_u64(remote(&s.few[from + ahead + a], 0), place_of(x[list[a]], c.first + list[a]));
+        lb_cluster_sync();
+        bool ok = true;
+        if (MASS) {
+            if (c.rank == 0) {
+                u64 mass = 0;
+                for (unsigned i = tid; i < left; i += kSpThreads) mass += row.weight(value_of_place(s.few[i]));
+                mass = warp_sum_u64(mass);
+                __syncthreads();
+                if (lane == 0) s.wsum[warp] = mass;
+                __syncthreads();
+                mass = 0;
+                for (int i = 0; i < kSpWarps; ++i) mass += s.wsum[i];
+                ok = mass >= limit;
+            }
+            t = c.answer(turn, c.rank == 0, ok, 0, 0);
+            ok = s.ra[t] != 0;
+        }
+        if (ok) {
+            if (c.rank == 0) choose(row, p, r, (int)left, k, top_p, min_p, MASS ? limit : 0);
+            return kSpDone;
+        }
+        return 0;
+    }
+    if (members > kSpCap) return 0;
+    // the weight in front of the bins exactly, and their values to the first CTA
+    if (tid == 0) s.n_cand = 0;
+    __syncthreads();
+    sum = 0;
+    for (int a = listed ? lane : tid; a < (listed ? (int)mine : c.n); a += listed ? 32 : kSpThreads) {
+        const int i = listed ? (int)list[a] : a;
         const float l = x[i];
-        if (!is_in(l, i)) continue;
+        if (!listed && !(l >= low_l && is_in(l, i))) continue;
         const int b = bin_of(l);
-        if (MASS && b < lo) sum += row.weight(l);
-        if (b < lo || b > hi) continue;
-        const unsigned at = atomicAdd(&s.n_cand, 1u);
-        if (at < kSpCap) list[at] = place_of(l, c.first + i);
+        if (b > hi) continue;
+        if (b < lo) {
+            if (MASS) sum += row.weight(l);
+        } else {
+            const unsigned at = atomicAdd(&s.n_cand, 1u);
+            st_cluster_u64(remote(&s.few[wfrom + at], 0), place_of(l, c.first + i));
+        }
     }
     if (MASS) {
         sum = warp_sum_u64(sum);
         if (lane == 0) s.wsum[warp] = sum;
-    }
-    __syncthreads();
-    const unsigned mine = s.n_cand;
-    sum = 0;
-    if (MASS)
+        __syncthreads();
+        sum = 0;
         for (int w = 0; w < kSpWarps; ++w) sum += s.wsum[w];
-    t = c.exchange(turn, mine, sum);
-    unsigned from = 0, members = 0;
-    if (MASS) base = 0;
-    for (unsigned r = 0; r < c.size; ++r) {
-        if (r < c.rank) from += (unsigned)s.xa[t][r];
-        members += (unsigned)s.xa[t][r];
-        if (MASS) base += s.xb[t][r];
+        t = c.exchange(turn, 0, sum);
+        base = 0;
+        for (unsigned q = 0; q < c.size; ++q) base += s.xb[t][q];
+        if (base >= limit) return 0;
+    } else {
+        lb_cluster_sync();
     }
-    if (members > kSpCap || (MASS && base >= limit)) return 0;
-    for (unsigned i = tid; i < mine; i += kSpThreads) st_cluster_u64(remote(&s.few[from + i], 0), list[i]);
-    lb_cluster_sync();
     u64 at = 0;
     if (c.rank == 0) {
-        u64* w = nullptr;
-        bool reached = true;
+        const int n = sort_few<false>((int)members, CUDART_INF_F, 0);
+        u64 w[kSpEach], before;
+        if (tid == 0) s.rc[0] = 0;
         if (MASS) {
-            w = s.cand;
-            u64 mass = 0;
-            for (unsigned i = tid; i < members; i += kSpThreads) {
-                w[i] = row.weight(value_of_place(s.few[i]));
-                mass += w[i];
-            }
-            mass = warp_sum_u64(mass);
-            __syncthreads();
-            if (lane == 0) s.wsum[warp] = mass;
-            __syncthreads();
-            mass = 0;
-            for (int i = 0; i < kSpWarps; ++i) mass += s.wsum[i];
-            reached = base + mass >= limit;
+            weights_of_few(row, n, w, before);
+        } else {
+            before = (u64)tid * kSpEach;
             __syncthreads();
         }
-        if (reached) at = local_cut(w, (int)members, 0, limit - base, row.top, row.far);
+        before += base;
+#pragma unroll
+        for (int e = 0; e < kSpEach; ++e) {
+            const int i = tid * kSpEach + e;
+            const u64 x = MASS ? w[e] : 1;
+            if (i < n && before < limit && before + x >= limit) s.rc[0] = s.few[i];
+            before += x;
+        }
+        __syncthreads();
+        at = s.rc[0];
     }
     t = c.answer(turn, c.rank == 0, at, 0, 0);
     return s.ra[t];
 }
 
-__global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSpThreads, 2) lb_sample_kernel(const SampleParams p) {
     LB_SAMPLE_SHARED;
     float* x = reinterpret_cast<float*>(lb_sample_smem + sizeof(SampleShared));
     unsigned size;
@@ -868,6 +978,8 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
         return;
     }
     row.inv_t = 1.0 / (double)temp;
+    row.inv_hi = (float)(1.4426950408889634 * row.inv_t);
+    row.inv_lo = (float)(1.4426950408889634 * row.inv_t - (double)row.inv_hi);
     row.far = 48.f * temp;
 
     // a value that no kept one is below, where one is known
@@ -885,34 +997,40 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
     }
     if (floor_l != floor_l) floor_l = -CUDART_INF_F;  // (no distance at an infinite temperature)
     if (few) {
-        u64* list = s.mass;  // and s.cand behind it
-        if (tid == 0) s.n_cand = 0;
-        __syncthreads();
+        unsigned* list = s.wlist + warp * kSpList;
+        unsigned mine = 0;
+#pragma unroll 2
         for (int i0 = 0; i0 < n; i0 += kSpThreads) {
             const int i = i0 + tid;
             const bool is = i < n && x[i] >= floor_l;
-            const unsigned hit = __ballot_sync(0xffffffffu, is);
-            unsigned at = 0;
-            if (lane == 0 && hit) at = atomicAdd(&s.n_cand, (unsigned)__popc(hit));
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(hit & ((1u << lane) - 1u));
-            if (is && at < kSpFew) list[at] = place_of(x[i], first + i);
+            const unsigned hit = __ballot_sync(0xffffffffu, is), at = mine + __popc(hit & ((1u << lane) - 1u));
+            if (is && at < kSpList) list[at] = (unsigned)i;
+            mine += __popc(hit);
         }
         __syncthreads();
-        const unsigned mine = s.n_cand;
-        const int t = c.exchange(turn, mine, 0);
+        if (lane == 0) s.wcount[warp] = mine;
+        const int all_listed = __syncthreads_and(mine <= kSpList);
+        unsigned ahead = 0, here = 0;
+        for (int w = 0; w < kSpWarps; ++w) {
+            if (w < warp) ahead += s.wcount[w];
+            here += s.wcount[w];
+        }
+        if (!all_listed) here += kSpFew;  // (then there is no list to give away)
+        const int t = c.exchange(turn, here, 0);
         unsigned from = 0, left = 0;
         for (unsigned q = 0; q < size; ++q) {
             if (q < rank) from += (unsigned)s.xa[t][q];
             left += (unsigned)s.xa[t][q];
         }
         if (left <= kSpFew) {
-            for (unsigned i = tid; i < mine; i += kSpThreads) st_cluster_u64(remote(&s.few[from + i], 0), list[i]);
+            for (unsigned a = lane; a < mine; a += 32) st_cluster_u64(remote(&s.few[from + ahead + a], 0), place_of(x[list[a]], first + list[a]));
             lb_cluster_sync();
-            if (rank == 0) choose(row, p, r, (int)left, k, top_p, min_p);
+            if (rank == 0) choose(row, p, r, (int)left, k, top_p, min_p, 0);
             return;
         }
     }
 
+    // the whole row
     u64 cut = 0;
     float scale = 0.f;
     const auto whole_scale = [&]() {  // of the whole row's bins
@@ -931,7 +1049,8 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
     };
     const bool plain = row.top < CUDART_INF_F;
     if (k) {
-        if (plain && groups && floor_l > -CUDART_INF_F) cut = cluster_cut<false>(c, row, turn, 0, floor_l, (u64)k, 0.f, row.top - floor_l);
+        if (plain && groups && floor_l > -CUDART_INF_F) cut = cluster_cut<false>(c, row, turn, 0, floor_l, (u64)k, 0.f, row.top - floor_l, p, r, k, top_p, min_p);
+        if (cut == kSpDone) return;
         if (cut == 0) {
             whole_scale();
             cut = find_cut(c, row, turn, 0, false, (u64)k, -1.f);
@@ -939,7 +1058,8 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
     }
     if (top_p < 1.f) {
         u64 at = 0;
-        if (plain) at = cluster_cut<true>(c, row, turn, cut, -CUDART_INF_F, 0, fmaxf(top_p, 0.f), kSpReach * temp);
+        if (plain) at = cluster_cut<true>(c, row, turn, cut, -CUDART_INF_F, 0, fmaxf(top_p, 0.f), kSpReach * temp, p, r, 0, top_p, min_p);
+        if (at == kSpDone) return;
         if (at == 0) {
             whole_scale();
             at = find_cut(c, row, turn, cut, true, 1, fmaxf(top_p, 0.f));
@@ -962,8 +1082,25 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
     // kept weight by warp, whose stretches follow one another
     const int stretch = (n + kSpWarps * 32 - 1) / (kSpWarps * 32) * 32;
     const int from = min(n, warp * stretch), to = min(n, from + stretch);
+    // (few of a row's values are kept once it has been cut: their places first, so that weights are computed for full warps)
+    unsigned short* list = reinterpret_cast<unsigned short*>(s.mass) + warp * kSpStretch;
+    const bool listed = cut != 0 && stretch <= kSpStretch;
+    int kept_n = 0;
+    __syncthreads();
+    if (listed)
+        for (int i0 = from; i0 < to; i0 += 32) {
+            const int i = i0 + lane;
+            const float l = i < to ? x[i] : -CUDART_INF_F;
+            const bool is = i < to && (l > cut_l || (l == cut_l && place_of(l, first + i) >= cut));
+            const unsigned hit = __ballot_sync(0xffffffffu, is);
+            if (is) list[kept_n + __popc(hit & ((1u << lane) - 1u))] = (unsigned short)(i - from);
+            kept_n += __popc(hit);
+        }
+    __syncwarp();
+    const int begin = listed ? 0 : from, end = listed ? kept_n : to;
+    const auto at_of = [&](int j) { return listed ? from + list[j] : j; };
     u64 mine = 0;
-    for (int i = from + lane; i < to; i += 32) mine += kept(i);
+    for (int j = begin + lane; j < end; j += 32) mine += kept(at_of(j));
     mine = warp_sum_u64(mine);
     __syncthreads();
     if (lane == 0) s.wsum[warp] = mine;
@@ -981,9 +1118,9 @@ __global__ void __launch_bounds__(kSpThreads) lb_sample_kernel(const SampleParam
     if (target < ahead || target >= ahead + here) return;
     for (int w = 0; w < warp; ++w) ahead += s.wsum[w];
     if (target < ahead || target >= ahead + s.wsum[warp]) return;
-    for (int i0 = from; i0 < to; i0 += 32) {
-        const int i = i0 + lane;
-        const u64 w = i < to ? kept(i) : 0;
+    for (int j0 = begin; j0 < end; j0 += 32) {
+        const int i = j0 + lane < end ? at_of(j0 + lane) : 0;
+        const u64 w = j0 + lane < end ? kept(i) : 0;
         const u64 upto = ahead + warp_scan_u64(w, lane);
         if (upto > target && upto - w <= target) {
             p.tokens[r] = first + i;
