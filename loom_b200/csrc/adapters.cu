@@ -2,13 +2,20 @@
 // with down [rank, cols], up [rows, rank] and the factor c of the adapter that token t's slot names.
 //
 // One launch.  A cluster of CTAs takes a tile of tokens that share an adapter; which tokens, every CTA works out from the slots (a histogram,
-// then the tile's stretch of the adapter's tokens in their order).  The CTAs split the columns of down x, add up their parts through
-// distributed shared memory -- always in the order of their ranks -- and then split the rows of up h.
+// then the tile's stretch of the adapter's tokens in their order; up to 16 tokens are a tile each, no histogram).  The CTAs split the
+// columns of down x, add up their parts through distributed shared memory -- always in the order of their ranks -- and then split
+// the rows of up h.
 //
 // Both products run on bf16 matrix instructions with float32 sums.  A float32 operand is the sum of three bf16 numbers, cut off it from the
 // top eight bits at a time, exactly; a product with a bf16 matrix is then three instructions, with a float32 one six (what is left out
 // is 2^-24 of the product).  So x, h and float32 adapters enter with all their bits, whatever the matrices' type.  A row of x that
 // is not finite makes its output not-a-numbers.
+//
+// Bound: the rows of x, base and out; for few tokens the latencies of slot, row, sum and rows one behind the other.  2999 tokens, 2560 columns
+// to 6912 rows of rank 16, five adapters: 62.8 us, 0.49 of what 197 MB take at the copy's rate -- 8 us to find the tiles, 10 for down x,
+// 3 for its sums, 35 for up h and the rows of base and out at 5 TB/s.  (Asking L2 for rows of x and base some steps ahead: 64 to 69 us; tiles
+// of 64 tokens, which read the adapter less often: 60.7 us, but 28 us instead of 20 for 512 tokens.)  One token 5.0 us, sixteen tokens of as
+// many adapters, 4096 to 14336: 20.9 us.
 #include "serving.cuh"
 
 #include <cuda_bf16.h>
@@ -19,7 +26,10 @@ constexpr int kAdThreads = 256;
 constexpr int kAdWarps = kAdThreads / 32;
 constexpr int kAdMaxRank = 256;
 constexpr int kAdMaxSlots = 4096;
-constexpr int kAdPass = 64;  // ranks of one pass over x
+constexpr int kAdMostCtas = 16;
+constexpr int kAdGroups = 24 * 1024;  // where the tokens' groups stand while a tile is being found, behind histogram and flags
+constexpr int kAdKept = 4096;         // tokens whose group is kept there
+constexpr int kAdTile = 16;  // tokens
 
 struct AdapterParams {
     const void *down, *up;
@@ -30,7 +40,8 @@ struct AdapterParams {
     float* out;
     long long ldx;
     int slots, rows, cols, rank_pad, cols_pad, rows_pad, tokens;
-    int copy;  // tokens without an adapter have something to be written
+    int copy;    // tokens without an adapter have something to be written
+    int single;  // a tile is one token
 };
 
 // a float32 value's top sixteen bits, and what is left
@@ -59,6 +70,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 // a[part][register] . b: the parts of both that reach 2^-24
 template <bool F32>
 __device__ __forceinline__ void products(float (&d)[4], const uint32_t (&a)[3][4], const uint32_t (&b0)[3], const uint32_t (&b1)[3]) {
@@ -72,26 +85,51 @@ __device__ __forceinline__ void products(float (&d)[4], const uint32_t (&a)[3][4
     mma_bf16(d, a[0][0], a[0][1], a[0][2], a[0][3], b0[0], b1[0]);
 }
 
-// four consecutive values of a row of an adapter's matrix as B registers of both pairs
-template <bool F32>
-__device__ __forceinline__ void load4(const void* base, size_t at, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
-    if (F32) {
-        const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at));
-        split2(f.x, f.y, b0);
-        split2(f.z, f.w, b1);
+// consecutive values of a row of an adapter's matrix, four or eight, as they come
+template <bool F32, int N>
+struct Raw {
+    uint32_t w[F32 ? N : N / 2];
+};
+template <bool F32, int N>
+__device__ __forceinline__ void load_raw(const void* base, size_t at, Raw<F32, N>& r) {
+    constexpr int W = F32 ? N : N / 2;
+    const uint8_t* p = static_cast<const uint8_t*>(base) + at * (F32 ? 4 : 2);
+    if (W == 2) {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        r.w[0] = v.x;
+        r.w[1] = v.y;
     } else {
-        const uint2 f = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(base) + at));
-        b0[0] = f.x;
-        b1[0] = f.y;
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+            r.w[i] = v.x;
+            r.w[i + 1] = v.y;
+            r.w[i + 2] = v.z;
+            r.w[i + 3] = v.w;
+        }
+    }
+}
+// the four values from 4 i on as B registers of both pairs
+template <bool F32, int N>
+__device__ __forceinline__ void parts_of(const Raw<F32, N>& r, int i, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
+    if (F32) {
+        split2(__uint_as_float(r.w[F32 ? 4 * i : 0]), __uint_as_float(r.w[F32 ? 4 * i + 1 : 0]), b0);
+        split2(__uint_as_float(r.w[F32 ? 4 * i + 2 : 0]), __uint_as_float(r.w[F32 ? 4 * i + 3 : 0]), b1);
+    } else {
+        b0[0] = r.w[F32 ? 0 : 2 * i];
+        b1[0] = r.w[F32 ? 0 : 2 * i + 1];
     }
 }
 
-// MT: tiles of 16 tokens in a cluster's tile
-template <int MT, bool F32>
-__global__ void __launch_bounds__(kAdThreads) lb_adapters_kernel(const AdapterParams p) {
-    constexpr int M = 16 * MT, KS = kAdWarps / MT;
+// CTAs of an SM (three or four with fewer registers: 62 and 107 us for 2999 tokens, 62.8 with two, and more for all other sizes)
+constexpr int ad_per_sm(int tiles, bool f32) { return tiles > 4 && f32 ? 1 : 2; }
+
+// TILES: ranks of one pass over x / 8
+template <int TILES, bool F32>
+__global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters_kernel(const AdapterParams p) {
+    constexpr int M = kAdTile, KS = kAdWarps, kAdPass = 8 * TILES;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    float* part = reinterpret_cast<float*>(smem_raw);  // [KS][M][kAdPass] down x of this CTA's columns; the groups' histogram before that
+    float* part = reinterpret_cast<float*>(smem_raw);  // [KS][M][kAdPass] down x of this CTA's columns
     const int hs_ld = p.rank_pad + 4;
     __nv_bfloat16* hs = reinterpret_cast<__nv_bfloat16*>(part + KS * M * kAdPass);  // [3][M][hs_ld] h in three parts
     __shared__ int s_tok[M];
@@ -101,19 +139,43 @@ __global__ void __launch_bounds__(kAdThreads) lb_adapters_kernel(const AdapterPa
     unsigned size;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
     const unsigned crank = lb_cluster_rank();
-    int tile = blockIdx.x / size;
+    const int tile = blockIdx.x / size;
+    lb_pdl_launch_dependents();
+    lb_pdl_wait();
 
-    // the tile's adapter and tokens
-    const auto group_of = [&](int token) {
-        const int s = __ldg(p.slot + token);
-        return s >= 0 && s < p.slots && __ldg(p.rank + s) > 0 ? s : p.slots;
-    };
-    {
-        int* count = reinterpret_cast<int*>(part);  // [slots + 1]
-        for (int i = tid; i <= p.slots; i += kAdThreads) count[i] = 0;
+    // ---- the tile's adapter and tokens ----
+    int group;
+    if (p.single) {
+        // (its x and base, which no slot has to be known for)
+        for (int k = ((int)crank * KS + warp) * 32; k < p.cols; k += (int)size * KS * 32)
+            if (lane == 0) prefetch_l2(p.x + (size_t)tile * p.ldx + k);
+        const int c = ((int)crank * KS + warp) * 64 + lane * 32;
+        if (p.base && lane < 2 && c < p.rows) prefetch_l2(p.base + (size_t)tile * p.rows + c);
+        group = __ldg(p.slot + tile);
+        if (group < 0 || group >= p.slots || __ldg(p.rank + group) <= 0) group = p.slots;
+        if (group == p.slots && !p.copy) return;
+        if (tid < M) s_tok[tid] = tid == 0 ? tile : -1;
+        __syncthreads();
+    } else {
+        int* count = reinterpret_cast<int*>(smem_raw);                                          // [slots + 1]
+        unsigned short* groups = reinterpret_cast<unsigned short*>(smem_raw + kAdGroups);       // [tokens] the first of them, at least
+        uint8_t* valid = smem_raw + kAdGroups - kAdMaxSlots;                                     // [slots]
+        for (int i = tid; i <= p.slots; i += kAdThreads) {
+            count[i] = 0;
+            if (i < p.slots) valid[i] = __ldg(p.rank + i) > 0;
+        }
         if (tid == 0) s_group = -1;
         __syncthreads();
-        for (int i = tid; i < p.tokens; i += kAdThreads) atomicAdd(&count[group_of(i)], 1);
+        const auto group_at = [&](int token) {
+            const int s = __ldg(p.slot + token);
+            return s >= 0 && s < p.slots && valid[s] ? s : p.slots;
+        };
+#pragma unroll 8
+        for (int i = tid; i < p.tokens; i += kAdThreads) {
+            const int s = group_at(i);
+            atomicAdd(&count[s], 1);
+            if (i < kAdKept) groups[i] = (unsigned short)s;
+        }
         __syncthreads();
         int before = 0;
         for (int g0 = 0; g0 <= p.slots; g0 += kAdThreads) {
@@ -128,6 +190,7 @@ __global__ void __launch_bounds__(kAdThreads) lb_adapters_kernel(const AdapterPa
             if (lane == 31) s_warp[warp] = sum;
             __syncthreads();
             int all = 0;
+#pragma unroll
             for (int w = 0; w < kAdWarps; ++w) {
                 if (w < warp) sum += s_warp[w];
                 all += s_warp[w];
@@ -139,41 +202,50 @@ __global__ void __launch_bounds__(kAdThreads) lb_adapters_kernel(const AdapterPa
             before += all;
             __syncthreads();
         }
-    }
-    const int group = s_group;
-    if (group < 0) return;  // (the whole cluster: fewer tiles than the grid has room for)
-    tile = s_tile;
-    if (tid < M) s_tok[tid] = -1;
-    int seen = 0;
-    for (int i0 = 0; i0 < p.tokens && seen < (tile + 1) * M; i0 += kAdThreads) {
-        const int i = i0 + tid;
-        const bool mine = i < p.tokens && group_of(i) == group;
-        const unsigned hit = __ballot_sync(0xffffffffu, mine);
+        group = s_group;
+        if (group < 0) return;  // (the whole cluster: fewer tiles than the grid has room for)
+        const int first = s_tile * M;
+        if (tid < M) s_tok[tid] = -1;
+        // the tokens in their order: a stretch of them to every warp, how many of each are the group's, then the tile's
+        const int per = ((p.tokens + kAdWarps - 1) / kAdWarps + 31) / 32 * 32, from = warp * per, to = min(p.tokens, from + per);
+        const auto is_mine = [&](int i) { return i < to && (i < kAdKept ? groups[i] : group_at(i)) == group; };
+        int here = 0;
+        for (int i0 = from; i0 < to; i0 += 32) here += __popc(__ballot_sync(0xffffffffu, is_mine(i0 + lane)));
+        if (lane == 0) s_warp[warp] = here;
         __syncthreads();
-        if (lane == 0) s_warp[warp] = __popc(hit);
+        int at = 0;
+        for (int w = 0; w < warp; ++w) at += s_warp[w];
+        if (at < first + M && at + here > first)
+            for (int i0 = from; i0 < to && at < first + M; i0 += 32) {
+                const bool mine = is_mine(i0 + lane);
+                const unsigned hit = __ballot_sync(0xffffffffu, mine);
+                const int k = at + __popc(hit & ((1u << lane) - 1u));
+                if (mine && k >= first && k < first + M) s_tok[k - first] = i0 + lane;
+                at += __popc(hit);
+            }
         __syncthreads();
-        int at = seen + __popc(hit & ((1u << lane) - 1u));
-        for (int w = 0; w < kAdWarps; ++w) {
-            if (w < warp) at += s_warp[w];
-            seen += s_warp[w];
-        }
-        if (mine && at >= tile * M && at < (tile + 1) * M) s_tok[at - tile * M] = i;
     }
-    __syncthreads();
     if (group == p.slots) {  // no adapter: the base as it is
         for (int r = 0; r < M && s_tok[r] >= 0; ++r) {
             const size_t at = (size_t)s_tok[r] * p.rows;
+#pragma unroll 4
             for (int i = crank * kAdThreads + tid; i < p.rows; i += size * kAdThreads) p.out[at + i] = p.base ? p.base[at + i] : 0.f;
         }
         return;
     }
     const int rank = __ldg(p.rank + group);
     const float scale = __ldg(p.scale + group);
-    const int mt = warp % MT, ks = warp / MT;
-    const int tok0 = s_tok[16 * mt + g], tok1 = s_tok[16 * mt + g + 8];
+    const int tok0 = s_tok[g], tok1 = s_tok[g + 8];
     const size_t wsize = F32 ? 4 : 2;
+    constexpr int CH = TILES == 8 || !F32 ? 4 : 2;  // columns of out that a warp takes at a time, in sixteens
+    const uint8_t* up = static_cast<const uint8_t*>(p.up) + (size_t)group * p.rows_pad * p.rank_pad * wsize;
+    {  // the first of them: the rows of up that they take
+        const int c = ((int)crank * KS + warp) * 16 * CH, n = min(16 * CH, p.rows_pad - c);
+        const int bytes = n * p.rank_pad * (int)wsize;
+        for (int i = lane * 128; i < bytes; i += 32 * 128) prefetch_l2(up + (size_t)c * p.rank_pad * wsize + i);
+    }
 
-    // h = c down x
+    // ---- h = c down x: 32 columns at a time, eight of them a lane ----
     {
         const float* x0 = p.x + (size_t)(tok0 < 0 ? 0 : tok0) * p.ldx;
         const float* x1 = p.x + (size_t)(tok1 < 0 ? 0 : tok1) * p.ldx;
@@ -190,53 +262,68 @@ __global__ void __launch_bounds__(kAdThreads) lb_adapters_kernel(const AdapterPa
         };
         const uint8_t* down = static_cast<const uint8_t*>(p.down) + (size_t)group * p.rank_pad * p.cols_pad * wsize;
         for (int n0 = 0; n0 < rank; n0 += kAdPass) {
-            const int tiles = (min(rank - n0, kAdPass) + 7) / 8;
-            float acc[kAdPass / 8][4] = {};
-            for (int k0 = ((int)crank * KS + ks) * 16; k0 < p.cols_pad; k0 += (int)size * KS * 16) {
-                const int k = k0 + 4 * t;
-                const float4 f0 = load_x(x0, tok0 >= 0, k), f1 = load_x(x1, tok1 >= 0, k);
-                uint32_t a[3][4], w[3];
-                split2(f0.x, f0.y, w);
+            const int tiles = (min(rank - n0, kAdPass) + 7) / 8, width = 8 * tiles;
+            float acc[TILES][4] = {};
+#pragma unroll 1
+            for (int k0 = ((int)crank * KS + warp) * 32; k0 < p.cols_pad; k0 += (int)size * KS * 32) {
+                const int k = k0 + 8 * t;
+                float4 f[2][2];
 #pragma unroll
-                for (int i = 0; i < 3; ++i) a[i][0] = w[i];
-                split2(f1.x, f1.y, w);
+                for (int i = 0; i < 2; ++i) {
+                    f[0][i] = load_x(x0, tok0 >= 0, k + 4 * i);
+                    f[1][i] = load_x(x1, tok1 >= 0, k + 4 * i);
+                }
+                Raw<F32, 8> w[TILES];
 #pragma unroll
-                for (int i = 0; i < 3; ++i) a[i][1] = w[i];
-                split2(f0.z, f0.w, w);
+                for (int n = 0; n < TILES; ++n)
+                    if (n < tiles) load_raw<F32, 8>(down, (size_t)(n0 + 8 * n + g) * p.cols_pad + k, w[n]);
 #pragma unroll
-                for (int i = 0; i < 3; ++i) a[i][2] = w[i];
-                split2(f1.z, f1.w, w);
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t a[3][4], v[3];
 #pragma unroll
-                for (int i = 0; i < 3; ++i) a[i][3] = w[i];
+                    for (int z = 0; z < 2; ++z) {
+                        split2(f[z][i].x, f[z][i].y, v);
 #pragma unroll
-                for (int n = 0; n < kAdPass / 8; ++n) {
-                    if (n >= tiles) break;
-                    uint32_t b0[3], b1[3];
-                    load4<F32>(down, (size_t)(n0 + 8 * n + g) * p.cols_pad + k, b0, b1);
-                    products<F32>(acc[n], a, b0, b1);
+                        for (int j = 0; j < 3; ++j) a[j][z] = v[j];
+                        split2(f[z][i].z, f[z][i].w, v);
+#pragma unroll
+                        for (int j = 0; j < 3; ++j) a[j][2 + z] = v[j];
+                    }
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n)
+                        if (n < tiles) {
+                            uint32_t b0[3], b1[3];
+                            parts_of<F32, 8>(w[n], i, b0, b1);
+                            products<F32>(acc[n], a, b0, b1);
+                        }
                 }
             }
-            __syncthreads();  // (the histogram, or the pass before, has been read)
+            __syncthreads();  // (what stood there has been read)
 #pragma unroll
-            for (int n = 0; n < kAdPass / 8; ++n) {
+            for (int n = 0; n < TILES; ++n) {
                 if (n >= tiles) break;
-                float* to = part + ((size_t)ks * M + 16 * mt + g) * kAdPass + 8 * n + 2 * t;
+                float* to = part + ((size_t)warp * M + g) * kAdPass + 8 * n + 2 * t;
                 *reinterpret_cast<float2*>(to) = make_float2(acc[n][0], acc[n][1]);
                 *reinterpret_cast<float2*>(to + 8 * kAdPass) = make_float2(acc[n][2], acc[n][3]);
             }
             __syncthreads();
-            for (int i = tid; i < M * kAdPass; i += kAdThreads) {
-                float sum = part[i];
-                for (int j = 1; j < KS; ++j) sum += part[(size_t)j * M * kAdPass + i];
-                part[i] = sum;
+            for (int i = tid; i < M * width; i += kAdThreads) {
+                float* at = part + i / width * kAdPass + i % width;
+                float sum = *at;
+#pragma unroll
+                for (int j = 1; j < KS; ++j) sum += at[(size_t)j * M * kAdPass];
+                *at = sum;
             }
             lb_cluster_sync();
             for (int i = tid; i < M * kAdPass; i += kAdThreads) {
                 const int r = i / kAdPass, n = i % kAdPass;
-                if (n0 + n >= p.rank_pad) continue;
+                if (n0 + n >= p.rank_pad || s_tok[r] < 0) continue;  // (rows that are not there: whatever stands in hs)
                 float sum = 0.f;
-                if (n < 8 * tiles)
-                    for (unsigned q = 0; q < size; ++q) sum += ld_cluster_f32(lb_cluster_addr(lb_smem_u32(part + i), q));
+                if (n < width) {
+#pragma unroll
+                    for (unsigned q = 0; q < kAdMostCtas; ++q)
+                        if (q < size) sum += ld_cluster_f32(lb_cluster_addr(lb_smem_u32(part + i), q));
+                }
                 sum *= scale;
 #pragma unroll
                 for (int k = 0; k < 3; ++k) hs[((size_t)k * M + r) * hs_ld + n0 + n] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(cut(sum)) >> 16));
@@ -245,52 +332,64 @@ __global__ void __launch_bounds__(kAdThreads) lb_adapters_kernel(const AdapterPa
         }
     }
 
-    // out = base + up h
-    const uint8_t* up = static_cast<const uint8_t*>(p.up) + (size_t)group * p.rows_pad * p.rank_pad * wsize;
+    // ---- out = base + up h: 64 columns at a time ----
     const bool wide = (p.rows & 3) == 0 && ((reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.base)) & 15) == 0;
     const int col_a = 4 * (g >> 1) + (g & 1);  // the rows of up whose sums lane t gets as four neighbours
-    for (int c0 = ((int)crank * KS + ks) * 16; c0 < p.rows_pad; c0 += (int)size * KS * 16) {
-        float acc[2][4] = {};
+    for (int c0 = ((int)crank * KS + warp) * 16 * CH; c0 < p.rows_pad; c0 += (int)size * KS * 16 * CH) {
+        float4 base[CH][2];
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int tok = z ? tok1 : tok0, c = c0 + 16 * j + 4 * t;
+                base[j][z] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (wide && p.base && tok >= 0 && c < p.rows) base[j][z] = __ldcs(reinterpret_cast<const float4*>(p.base + (size_t)tok * p.rows + c));
+            }
+        float acc[CH][2][4] = {};
         for (int k0 = 0; k0 < rank; k0 += 16) {
+            Raw<F32, 4> w[CH][2];
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    if (c0 + 16 * j < p.rows_pad) load_raw<F32, 4>(up, (size_t)(c0 + 16 * j + col_a + 2 * n) * p.rank_pad + k0 + 4 * t, w[j][n]);
             uint32_t a[3][4];
 #pragma unroll
             for (int i = 0; i < 3; ++i) {
-                const __nv_bfloat16* from = hs + ((size_t)i * M + 16 * mt + g) * hs_ld + k0 + 4 * t;
-                const uint2 r0 = *reinterpret_cast<const uint2*>(from), r1 = *reinterpret_cast<const uint2*>(from + 8 * hs_ld);
+                const __nv_bfloat16* from = hs + ((size_t)i * M + g) * hs_ld + k0 + 4 * t;
+                uint2 r0 = *reinterpret_cast<const uint2*>(from), r1 = *reinterpret_cast<const uint2*>(from + 8 * hs_ld);
                 a[i][0] = r0.x;
                 a[i][1] = r1.x;
                 a[i][2] = r0.y;
                 a[i][3] = r1.y;
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                uint32_t b0[3], b1[3];
-                load4<F32>(up, (size_t)(c0 + col_a + 2 * n) * p.rank_pad + k0 + 4 * t, b0, b1);
-                products<F32>(acc[n], a, b0, b1);
-            }
-        }
-        const int c = c0 + 4 * t;
+            for (int j = 0; j < CH; ++j)
+                if (c0 + 16 * j < p.rows_pad)
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            const int tok = z ? tok1 : tok0;
-            if (tok < 0) continue;
-            const size_t at = (size_t)tok * p.rows + c;
-            float f[4] = {acc[0][2 * z], acc[0][2 * z + 1], acc[1][2 * z], acc[1][2 * z + 1]};
-            if (wide && c < p.rows) {
-                if (p.base) {
-                    const float4 b = *reinterpret_cast<const float4*>(p.base + at);
-                    f[0] += b.x;
-                    f[1] += b.y;
-                    f[2] += b.z;
-                    f[3] += b.w;
+                    for (int n = 0; n < 2; ++n) {
+                        uint32_t b0[3], b1[3];
+                        parts_of<F32, 4>(w[j][n], 0, b0, b1);
+                        products<F32>(acc[j][n], a, b0, b1);
+                    }
+        }
+#pragma unroll
+        for (int j = 0; j < CH; ++j)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const int tok = z ? tok1 : tok0, c = c0 + 16 * j + 4 * t;
+                if (tok < 0 || c >= p.rows) continue;
+                const size_t at = (size_t)tok * p.rows + c;
+                float f[4] = {acc[j][0][2 * z], acc[j][0][2 * z + 1], acc[j][1][2 * z], acc[j][1][2 * z + 1]};
+                if (wide) {
+                    const float4 b = base[j][z];
+                    __stcs(reinterpret_cast<float4*>(p.out + at), make_float4(f[0] + b.x, f[1] + b.y, f[2] + b.z, f[3] + b.w));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + e < p.rows) p.out[at + e] = f[e] + (p.base ? p.base[at + e] : 0.f);
                 }
-                *reinterpret_cast<float4*>(p.out + at) = make_float4(f[0], f[1], f[2], f[3]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < p.rows) p.out[at + e] = f[e] + (p.base ? p.base[at + e] : 0.f);
             }
-        }
     }
 }
 
@@ -310,28 +409,37 @@ __global__ void lb_adapters_meta_kernel(int* rank, float* scale, int r, float s)
     *scale = s;
 }
 
-template <int MT, bool F32>
+template <int TILES, bool F32>
 int launch_adapters(loom_b200_ctx* ctx, const AdapterParams& p, int tiles) {
-    constexpr int M = 16 * MT, KS = kAdWarps / MT;
-    const size_t front = (size_t)KS * M * kAdPass * 4;
-    static_assert((size_t)KS * M * kAdPass >= kAdMaxSlots + 1, "room for the histogram");
+    constexpr int M = kAdTile;
+    constexpr size_t find = (size_t)kAdGroups + kAdKept * 2, parts = (size_t)kAdWarps * M * 8 * TILES * 4, front = find > parts ? find : parts;
+    static_assert((size_t)kAdGroups >= (kAdMaxSlots + 1) * 4 + kAdMaxSlots, "room for what finds a tile");
     const size_t smem = front + (size_t)3 * M * (p.rank_pad + 4) * 2;
-    LB_CUDA(ctx, cudaFuncSetAttribute(lb_adapters_kernel<MT, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(front + (size_t)3 * M * (kAdMaxRank + 4) * 2)));
-    int size = 8;
-    while (size > 1 && tiles * size > 4 * ctx->sm_count) size /= 2;
+    const auto kern = lb_adapters_kernel<TILES, F32>;
+    LB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(front + (size_t)3 * M * (kAdMaxRank + 4) * 2)));
+    LB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    // As many CTAs a tile as are there at once.  Clusters of more than eight find their places in a GPC less and less well (256 tokens of
+    // two adapters: 12 CTAs a tile 13.9 us, 14 18.6 us), so those leave a quarter free; 16 of 16 fit (16 tokens: 20.9 us, with 13 26.2 us).
+    const int most = ad_per_sm(TILES, F32) * ctx->sm_count;
+    int size = most * 7 / 8 / tiles;
+    if (size >= kAdMostCtas) size = kAdMostCtas;
+    else if (size > 8) size = most * 3 / 4 / tiles > 8 ? most * 3 / 4 / tiles : 8;
+    else if (size < 4) size = most / tiles > 4 ? 4 : most / tiles > 0 ? most / tiles : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(tiles * size);
     cfg.blockDim = dim3(kAdThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = size;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    LB_CUDA(ctx, cudaLaunchKernelEx(&cfg, lb_adapters_kernel<MT, F32>, p));
+    cfg.numAttrs = ctx->opt_pdl ? 2 : 1;
+    LB_CUDA(ctx, cudaLaunchKernelEx(&cfg, kern, p));
     ctx->launches++;
     return 0;
 }
@@ -456,11 +564,12 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
     p.rows_pad = a->rows_pad;
     p.tokens = tokens;
     p.copy = base != out;
-    const int groups = a->slots + 1, m = tokens >= 256 ? 64 : 16;
-    const int tiles = tokens <= groups ? tokens : groups + (tokens - groups) / m;  // at most
-    const bool f32 = a->dtype == LOOM_B200_DTYPE_F32;
-    if (m == 64) return f32 ? launch_adapters<4, true>(ctx, p, tiles) : launch_adapters<4, false>(ctx, p, tiles);
-    return f32 ? launch_adapters<1, true>(ctx, p, tiles) : launch_adapters<1, false>(ctx, p, tiles);
+    p.single = tokens <= 16;
+    const int groups = a->slots + 1;
+    const int tiles = p.single || tokens <= groups ? tokens : groups + (tokens - groups) / kAdTile;  // at most
+    const auto launch = a->dtype == LOOM_B200_DTYPE_F32 ? a->max_rank <= 16 ? launch_adapters<2, true> : a->max_rank <= 32 ? launch_adapters<4, true> : launch_adapters<8, true>
+                                                        : a->max_rank <= 16 ? launch_adapters<2, false> : a->max_rank <= 32 ? launch_adapters<4, false> : launch_adapters<8, false>;
+    return launch(ctx, p, tiles);
 }
 
 }  // extern "C"
