@@ -60,114 +60,341 @@ __device__ __forceinline__ int key_byte(int p, int d, int dim_k) {
 }
 __device__ __forceinline__ int value_byte(int p, int d) { return (d >> 3) * 512 + (d & 7) * 64 + (p >> 1 & 3) * 16 + (p >> 3) * 2 + (p & 1); }
 
-// ---- rows in ---------------------------------------------------------------------------------------------------------------------
+// ---- rows in, and rows out as the cache holds them ---------------------------------------------------------------------------------
 //
-// A CTA takes one block of one sequence and head that the call's rows touch.  It writes them to the open rows where the block is one of the
-// last two, and where they complete it (the first of its rows may be there already) makes the codes.  Open rows go by the block's parity:
-// the rows that the first block still reads there may be what a block two further on replaces, so the CTA of the first block
-// writes for that one too, after its own reads.
-constexpr int kApThreads = 256;
+// An item is a block that the call's rows touch, of one KV head, keys or values; a CTA finds its block in the list of them by itself.  A
+// thread has eight positions of four dimensions at a time, so that its codes are words of what the cache holds and every access
+// fills whole sectors: keys, positions j, 8 + j, 16 + j and so on; values, the pairs 2 t, 2 t + 1 of four groups of eight.
+//
+// Append writes the rows to the open rows where the block is one of the last two, and where they complete it (the first of its rows may
+// be there already) makes the codes.  Open rows go by the block's parity: the rows that the first block still reads there may be what
+// a block two further on replaces, so the CTA of the first block writes for that one too, after its own reads.
+//
+// A code is the float32 product where that is further than 2^-10 from a half (its error is below 2^-16) and the float64 arithmetic
+// elsewhere, one value in five hundred: conversions and float64 take sixteen values a clock of an SM.
+//
+// Bound: memory; for few rows, latencies.  About 8000 rows of eight heads of 128 in 8 sequences: append 20.0 us, read 14.1 us (81 MB
+// each way, 4 and 5.8 TB/s); one row of each of 64 sequences: 7.7 and 6.0 us.  A CTA for each head: with two, four and all eight heads
+// a CTA the append takes 28, 38 and 66 us.
+constexpr int kRowThreads = 256;
 
-struct AppendParams {
+struct RowParams {
     Kv8 c;
     int rows;
     const int32_t *starts, *lengths;
-    const float *k, *v;
-    long long ld;  // floats from one row of k (and of v) to the next
+    const float *k, *v;  // append's
+    long long ld;        // floats from one row of k (and of v) to the next
+    float *k_out, *v_out;  // read's: [rows][heads][dim]
+    int wide;            // rows begin on 16 bytes
 };
 
-__global__ void __launch_bounds__(kApThreads) lb_kv8_append_kernel(const AppendParams p) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
-    float* x = reinterpret_cast<float*>(smem_raw);  // [64][dim]
-    __shared__ float s_top[kApThreads / 32];
-    const Kv8& c = p.c;
-    const int s = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-    const Span a = span_of(p.starts, p.lengths, p.rows, s);
-    if (a.count == 0) return;
-    if (!fits(c, a)) {
-        if (blockIdx.x == 0 && h == 0 && tid == 0) atomicExch(c.status, 7);
-        return;
-    }
-    const int end = a.pos + a.count;
-    const int first = a.pos / kKvBlock, last = (end - 1) / kKvBlock;  // blocks
-    for (int b = first + (int)blockIdx.x; b <= last; b += gridDim.x) {
-        const int from = max(a.pos, b * kKvBlock), to = min(end, (b + 1) * kKvBlock);
-        const bool whole = to == (b + 1) * kKvBlock;
-        for (int kv = 0; kv < 2; ++kv) {
-            const float* src = (kv ? p.v : p.k) + (size_t)h * c.dim;
-            float* open = kv ? c.v_open : c.k_open;
-            const auto row_of = [&](int pos) { return src + (size_t)(a.row + pos - a.pos) * p.ld; };
-            if (whole) {
-                float top = 0.f;
-                bool odd = false;
-                for (int i = tid; i < kKvBlock * c.dim; i += kApThreads) {
-                    const int pos = b * kKvBlock + i / c.dim, d = i % c.dim;
-                    const float f = pos >= from ? row_of(pos)[d] : c.open_row(open, s, h, pos)[d];
-                    x[i] = f;
-                    top = fmaxf(top, fabsf(f));
-                    odd |= !(fabsf(f) <= CUDART_MAX_NORMAL_F);
-                }
-                top = lb_warp_max(odd ? CUDART_INF_F : top);
-                if ((tid & 31) == 0) s_top[tid >> 5] = top;
-                __syncthreads();
-                for (int w = 0; w < kApThreads / 32; ++w) top = fmaxf(top, s_top[w]);
-                const bool fine = top <= CUDART_MAX_NORMAL_F && top > 0.f;
-                const double mul = fine ? __ddiv_rn(127.0, (double)top) : 0.0;
-                const size_t at = c.head_of(s, h) * c.blocks + b;
-                const int dims = kv ? c.dim_v : c.dim_k;
-                uint8_t* codes = (kv ? c.v : c.k) + at * kKvBlock * dims;
-                if (tid == 0) (kv ? c.v_top : c.k_top)[at] = fine || top == 0.f ? top : CUDART_NAN_F;
-                for (int i = tid; i < kKvBlock * dims; i += kApThreads) {
-                    const int pos = i / dims, d = i % dims;
-                    const int code = fine && d < c.dim ? lb_quant_i8((double)x[pos * c.dim + d], mul) : 0;
-                    codes[kv ? value_byte(pos, d) : key_byte(pos, d, c.dim_k)] = (uint8_t)code;
-                }
-                __syncthreads();
+struct Unit {
+    int col, oct;  // dimensions 4 col .. 4 col + 3; which positions
+};
+// unit u of a block: warps take 32 bytes of four key positions, or the values of four columns whole
+template <bool V>
+__device__ __forceinline__ Unit unit_of(int u) {
+    const int l = u & 31, w = u >> 5;
+    if (V) return {4 * w + (l & 3), l >> 2};
+    return {8 * (w >> 1) + (l & 7), 4 * (w & 1) + (l >> 3)};
+}
+template <bool V>
+__device__ __forceinline__ int place_of(int oct, int i) {
+    return V ? 8 * (4 * (oct & 1) + (i >> 1)) + 2 * (oct >> 1) + (i & 1) : 8 * i + oct;
+}
+
+__device__ __forceinline__ int blocks_of(const Kv8& c, const Span& a) {
+    if (a.count == 0) return 0;
+    return fits(c, a) ? (a.pos + a.count - 1) / kKvBlock - a.pos / kKvBlock + 1 : 1;
+}
+
+// Block n of the list, in the sequences' order: its sequence, or -1, and which of the sequence's it is.  For the whole CTA.
+struct Item {
+    Span a;
+    int seq, block;
+    bool more;  // the list goes on behind this round of the grid
+};
+__device__ __forceinline__ Item item_of(const RowParams& p, int n) {
+    __shared__ int s_sum[kRowThreads / 32], s_seq, s_block, s_span[3];
+    Item r;
+    if (!p.starts) {
+        r.seq = n < min(p.rows, p.c.seqs) ? n : -1;
+        r.block = 0;
+        r.more = false;
+        if (r.seq >= 0) r.a = span_of(p.starts, p.lengths, p.rows, r.seq);
+    } else {
+        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+        __syncthreads();  // (the item before has been read)
+        if (tid == 0) s_seq = -1;
+        for (int s0 = 0; s0 < p.c.seqs; s0 += kRowThreads) {
+            const int s = s0 + tid;
+            Span a = {0, 0, 0};
+            if (s < p.c.seqs) a = span_of(p.starts, p.lengths, p.rows, s);
+            const int mine = blocks_of(p.c, a);
+            int sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
             }
-            const auto keep = [&](int blk) {
-                const int f0 = max(a.pos, blk * kKvBlock), f1 = min(end, (blk + 1) * kKvBlock);
-                for (int i = tid; i < (f1 - f0) * c.dim; i += kApThreads) {
-                    const int pos = f0 + i / c.dim, d = i % c.dim;
-                    c.open_row(open, s, h, pos)[d] = row_of(pos)[d];
-                }
-            };
-            if (b >= last - 1 && (b == first || ((b - first) & 1))) keep(b);
-            if (b == first)
-                for (int blk = max(first + 2, last - 1); blk <= last; ++blk)
-                    if (!((blk - first) & 1)) keep(blk);
+            if (lane == 31) s_sum[warp] = sum;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < kRowThreads / 32; ++w) {
+                const int u = s_sum[w];
+                sum += w < warp ? u : 0;
+                all += u;
+            }
+            if (n < sum && n >= sum - mine) {
+                s_seq = s;
+                s_block = n - (sum - mine);
+                s_span[0] = a.row;
+                s_span[1] = a.count;
+                s_span[2] = a.pos;
+            }
+            n -= all;
+            __syncthreads();
+        }
+        r.more = n + (int)gridDim.y >= 0;
+        r.seq = s_seq;
+        r.block = s_block;
+        r.a = {s_span[0], s_span[1], s_span[2]};
+    }
+    return r;
+}
+
+__device__ __forceinline__ float4 load_four(const float* row, int d, int dim, bool wide) {
+    if (wide) return __ldcs(reinterpret_cast<const float4*>(row + d));
+    return make_float4(__ldcs(row + d), d + 1 < dim ? __ldcs(row + d + 1) : 0.f, d + 2 < dim ? __ldcs(row + d + 2) : 0.f, d + 3 < dim ? __ldcs(row + d + 3) : 0.f);
+}
+
+__device__ __forceinline__ void store_four(float* row, int d, int dim, bool wide, const float4& f) {
+    if (wide) {
+        __stcs(reinterpret_cast<float4*>(row + d), f);
+    } else {
+        row[d] = f.x;
+        if (d + 1 < dim) row[d + 1] = f.y;
+        if (d + 2 < dim) row[d + 2] = f.z;
+        if (d + 3 < dim) row[d + 3] = f.w;
+    }
+}
+
+// codes of four values, a byte each
+__device__ __noinline__ uint32_t codes_exactly(float4 x, double mul) {
+    const uint32_t n0 = lb_quant_i8((double)x.x, mul), n1 = lb_quant_i8((double)x.y, mul), n2 = lb_quant_i8((double)x.z, mul), n3 = lb_quant_i8((double)x.w, mul);
+    return __byte_perm(__byte_perm(n0, n1, 0x0040), __byte_perm(n2, n3, 0x0040), 0x5410);
+}
+__device__ __forceinline__ uint32_t codes_of(const float4& x, float mulf, double mul) {
+    constexpr float kRound = 12582912.f;  // 1.5 2^23: a sum's low bits are the nearest integer
+    const float f[4] = {x.x, x.y, x.z, x.w};
+    uint32_t n[4];
+    float off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float r = fmaf(f[e], mulf, kRound);
+        n[e] = __float_as_uint(r);
+        off = fmaxf(off, fabsf(fmaf(f[e], mulf, kRound - r)));
+    }
+    if (off > 0.5f - 1.f / 1024.f) return codes_exactly(x, mul);
+    return __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+}
+
+template <int NU, bool V>
+__device__ __forceinline__ void append_block(const RowParams& p, const Item& it, int b, int h, bool keep, uint32_t* s_top) {
+    const Kv8& c = p.c;
+    const Span a = it.a;
+    const int tid = threadIdx.x, s = it.seq;
+    const int dims = V ? c.dim_v : c.dim_k;
+    const int units = V ? (dims + 15) / 16 * 32 : dims * 2;
+    const float* src = (V ? p.v : p.k) + (size_t)h * c.dim;
+    float* open = V ? c.v_open : c.k_open;
+    const auto row_of = [&](int pos) { return src + (size_t)(a.row + pos - a.pos) * p.ld; };
+    const auto open_of = [&](int pos) { return c.open_row(open, s, h, pos); };
+    float4 x[NU][8];
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+        const Unit w = unit_of<V>(tid + j * kRowThreads);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int pos = b * kKvBlock + place_of<V>(w.oct, i);
+            x[j][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (4 * w.col >= c.dim) continue;
+            if (pos >= a.pos) x[j][i] = load_four(row_of(pos), 4 * w.col, c.dim, p.wide);
+            else x[j][i] = *reinterpret_cast<const float4*>(open_of(pos) + 4 * w.col);
+        }
+    }
+    uint32_t bits = 0;  // the largest magnitude's, or those of what is no finite value, which are above all
+#pragma unroll
+    for (int j = 0; j < NU; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 f = x[j][i];
+            bits = max(max(bits, __float_as_uint(f.x) & 0x7fffffffu), __float_as_uint(f.y) & 0x7fffffffu);
+            bits = max(max(bits, __float_as_uint(f.z) & 0x7fffffffu), __float_as_uint(f.w) & 0x7fffffffu);
+        }
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    if ((tid & 31) == 0) s_top[tid >> 5] = bits;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowThreads / 32; ++w) bits = max(bits, s_top[w]);
+    const float top = __uint_as_float(bits);
+    const bool fine = top <= CUDART_MAX_NORMAL_F && top > 0.f;
+    const double mul = fine ? __ddiv_rn(127.0, (double)top) : 0.0;
+    const bool fast = top > 1e-30f && top < 1e30f;  // (the float32 factor is a normal number)
+    const float mulf = (float)mul;
+    const size_t at = c.head_of(s, h) * c.blocks + b;
+    uint8_t* codes = (V ? c.v : c.k) + at * kKvBlock * dims;
+    if (tid == 0) (V ? c.v_top : c.k_top)[at] = fine || top == 0.f ? top : CUDART_NAN_F;
+#pragma unroll
+    for (int j = 0; j < NU; ++j) {
+        const int u = tid + j * kRowThreads;
+        const Unit w = unit_of<V>(u);
+        if (u >= units || 4 * w.col >= dims) continue;
+        uint32_t n[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n[i] = fast ? codes_of(x[j][i], mulf, mul) : fine ? codes_exactly(x[j][i], mul) : 0u;
+        if (V) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t sel = e | (e + 4) << 4;
+                const uint32_t lo = __byte_perm(__byte_perm(n[0], n[1], sel), __byte_perm(n[2], n[3], sel), 0x5410);
+                const uint32_t hi = __byte_perm(__byte_perm(n[4], n[5], sel), __byte_perm(n[6], n[7], sel), 0x5410);
+                *reinterpret_cast<uint2*>(codes + value_byte(place_of<V>(w.oct, 0), 4 * w.col + e)) = make_uint2(lo, hi);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *reinterpret_cast<uint32_t*>(codes + key_byte(place_of<V>(w.oct, i), 4 * w.col, dims)) = n[i];
+        }
+    }
+    if (keep)
+#pragma unroll
+        for (int j = 0; j < NU; ++j) {
+            const Unit w = unit_of<V>(tid + j * kRowThreads);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int pos = b * kKvBlock + place_of<V>(w.oct, i);
+                if (4 * w.col < c.dim && pos >= a.pos) *reinterpret_cast<float4*>(open_of(pos) + 4 * w.col) = x[j][i];
+            }
+        }
+    __syncthreads();  // (s_top)
+}
+
+// rows of block b into the open rows, or out of them
+template <bool IN>
+__device__ __forceinline__ void copy_rows(const RowParams& p, const Item& it, int b, int kv, int h) {
+    const Kv8& c = p.c;
+    const Span a = it.a;
+    const int from = max(a.pos, b * kKvBlock), n = min(a.pos + a.count, (b + 1) * kKvBlock) - from;
+    const int d4 = c.dim_o / 4;
+    float* open = kv ? c.v_open : c.k_open;
+    const float* src = kv ? p.v : p.k;
+    float* out = kv ? p.v_out : p.k_out;
+    const long long ld = IN ? p.ld : (long long)c.heads * c.dim;
+    for (int i = threadIdx.x; i < n * d4; i += kRowThreads) {
+        const int d = 4 * (i % d4), r = i / d4;
+        const size_t at = (size_t)(a.row + from - a.pos + r) * ld + (size_t)h * c.dim;
+        float4* in = reinterpret_cast<float4*>(c.open_row(open, it.seq, h, from + r) + d);
+        if (IN) *in = load_four(src + at, d, c.dim, p.wide);
+        else store_four(out + at, d, c.dim, p.wide, *in);
+    }
+}
+
+template <int NU>
+__global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_kernel(const RowParams p) {
+    __shared__ uint32_t s_top[kRowThreads / 32];
+    lb_pdl_launch_dependents();
+    lb_pdl_wait();
+    const int kv = blockIdx.x & 1, h = blockIdx.x >> 1;
+    bool more = true;
+    for (int n = blockIdx.y; more; n += gridDim.y) {
+        const Item it = item_of(p, n);
+        if (it.seq < 0) return;
+        more = it.more;
+        if (!fits(p.c, it.a)) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.c.status, 7);
+            continue;
+        }
+        if (it.a.count == 0) continue;
+        const int end = it.a.pos + it.a.count, first = it.a.pos / kKvBlock, last = (end - 1) / kKvBlock, b = first + it.block;
+        const bool keep = b >= last - 1 && (b == first || ((b - first) & 1));
+        if ((b + 1) * kKvBlock <= end) {
+            if (kv) append_block<NU, true>(p, it, b, h, keep, s_top);
+            else append_block<NU, false>(p, it, b, h, keep, s_top);
+        } else if (keep) {
+            copy_rows<true>(p, it, b, kv, h);
+        }
+        if (b == first && last - first >= 2) copy_rows<true>(p, it, last - ((last - first) & 1), kv, h);  // (behind the barrier that append_block ends with)
+    }
+}
+
+// four codes times the block's scale
+__device__ __forceinline__ float4 values_of(uint32_t w, float a) {
+    w ^= 0x80808080u;
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + e)) - 8388736.f, a);  // 2^23 + 128
+    return make_float4(f[0], f[1], f[2], f[3]);
+}
+
+template <bool V>
+__device__ __forceinline__ void read_block(const RowParams& p, const Item& it, int b, int h) {
+    const Kv8& c = p.c;
+    const Span a = it.a;
+    const int s = it.seq;
+    const int dims = V ? c.dim_v : c.dim_k;
+    const size_t at = c.head_of(s, h) * c.blocks + b;
+    const uint8_t* codes = (V ? c.v : c.k) + at * kKvBlock * dims;
+    const float scale = __fdiv_rn(__ldg((V ? c.v_top : c.k_top) + at), 127.f);
+    const int units = V ? (dims + 15) / 16 * 32 : dims * 2;
+    for (int u = threadIdx.x; u < units; u += kRowThreads) {
+        const Unit w = unit_of<V>(u);
+        if (4 * w.col >= c.dim) continue;
+        uint32_t n[8];
+        if (V) {
+            uint2 e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = *reinterpret_cast<const uint2*>(codes + value_byte(place_of<V>(w.oct, 0), 4 * w.col + i));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t sel = i | (i + 4) << 4;
+                n[i] = __byte_perm(__byte_perm(e[0].x, e[1].x, sel), __byte_perm(e[2].x, e[3].x, sel), 0x5410);
+                n[4 + i] = __byte_perm(__byte_perm(e[0].y, e[1].y, sel), __byte_perm(e[2].y, e[3].y, sel), 0x5410);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n[i] = *reinterpret_cast<const uint32_t*>(codes + key_byte(place_of<V>(w.oct, i), 4 * w.col, dims));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int pos = b * kKvBlock + place_of<V>(w.oct, i);
+            if (pos < a.pos) continue;
+            float* out = (V ? p.v_out : p.k_out) + ((size_t)(a.row + pos - a.pos) * c.heads + h) * c.dim;
+            store_four(out, 4 * w.col, c.dim, p.wide, values_of(n[i], scale));
         }
     }
 }
 
-// ---- rows out, as the cache holds them --------------------------------------------------------------------------------------------
-
-struct ReadParams {
-    Kv8 c;
-    int rows;
-    const int32_t *starts, *lengths;
-    float *k, *v;  // [rows][heads][dim]
-};
-
-__global__ void __launch_bounds__(kApThreads) lb_kv8_read_kernel(const ReadParams p) {
-    const Kv8& c = p.c;
-    const int s = blockIdx.z, h = blockIdx.y;
-    const Span a = span_of(p.starts, p.lengths, p.rows, s);
-    if (a.count == 0) return;
-    if (!fits(c, a)) {
-        if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) atomicExch(c.status, 7);
-        return;
-    }
-    const int closed = (a.pos + a.count) / kKvBlock * kKvBlock;
-    for (long long i = (long long)blockIdx.x * kApThreads + threadIdx.x; i < (long long)a.count * c.dim; i += (long long)gridDim.x * kApThreads) {
-        const int j = (int)(i / c.dim), d = (int)(i % c.dim), pos = a.pos + j, at = pos % kKvBlock;
-        const size_t out = ((size_t)(a.row + j) * c.heads + h) * c.dim + d;
-        if (pos < closed) {
-            const size_t blk = c.head_of(s, h) * c.blocks + pos / kKvBlock;
-            p.k[out] = __fmul_rn((float)(int8_t)c.k[blk * kKvBlock * c.dim_k + key_byte(at, d, c.dim_k)], __fdiv_rn(c.k_top[blk], 127.f));
-            p.v[out] = __fmul_rn((float)(int8_t)c.v[blk * kKvBlock * c.dim_v + value_byte(at, d)], __fdiv_rn(c.v_top[blk], 127.f));
+__global__ void __launch_bounds__(kRowThreads, 3) lb_kv8_read_kernel(const RowParams p) {
+    lb_pdl_launch_dependents();
+    lb_pdl_wait();
+    const int kv = blockIdx.x & 1, h = blockIdx.x >> 1;
+    bool more = true;
+    for (int n = blockIdx.y; more; n += gridDim.y) {
+        const Item it = item_of(p, n);
+        if (it.seq < 0) return;
+        more = it.more;
+        if (!fits(p.c, it.a)) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.c.status, 7);
+            continue;
+        }
+        if (it.a.count == 0) continue;
+        const int b = it.a.pos / kKvBlock + it.block;
+        if ((b + 1) * kKvBlock > it.a.pos + it.a.count) {
+            copy_rows<false>(p, it, b, kv, h);
         } else {
-            p.k[out] = c.open_row(c.k_open, s, h, pos)[d];
-            p.v[out] = c.open_row(c.v_open, s, h, pos)[d];
+            if (kv) read_block<true>(p, it, b, h);
+            else read_block<false>(p, it, b, h);
         }
     }
 }
@@ -1119,26 +1346,34 @@ static int kv8_ready(loom_b200_ctx* ctx, const loom_b200_kv8* c, int rows, const
     return 0;
 }
 
+// a CTA for each item, as far as the blocks can be bounded here: a sequence's rows touch one more than their 64s, and at most one each
+static dim3 row_grid(const RowParams& p) {
+    long long blocks = p.rows;
+    if (p.starts && blocks > (p.rows + 62LL * p.c.seqs) / kKvBlock + p.c.seqs) blocks = (p.rows + 62LL * p.c.seqs) / kKvBlock + p.c.seqs;
+    if (blocks > 32768) blocks = 32768;
+    return dim3(2 * p.c.heads, (unsigned)blocks);
+}
+
 int loom_b200_kv8_append(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, const int32_t* starts, const int32_t* lengths, const float* k, const float* v, long long ld) {
     if (int rc = kv8_ready(ctx, c, rows, starts, lengths, k, v, "kv8_append")) return rc;
     LB_REQUIRE(ctx, ld >= (long long)c->heads * c->dim, "kv8_append: %lld floats between rows of %d", ld, c->heads * c->dim);
     if (int rc = lb_set_device(ctx)) return rc;
-    AppendParams p{view(c), rows, starts, lengths, k, v, ld};
-    const size_t smem = (size_t)kKvBlock * c->dim * 4;
-    LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_append_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKvBlock * 256 * 4));
-    const int blocks = starts ? (rows + kKvBlock - 2) / kKvBlock + 1 : 1;
-    lb_kv8_append_kernel<<<dim3(blocks < 256 ? blocks : 256, c->heads, c->seqs), kApThreads, smem, ctx->stream>>>(p);
-    LB_CHECK_LAUNCH(ctx, "lb_kv8_append_kernel");
+    const bool wide = c->dim % 4 == 0 && ld % 4 == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
+    const RowParams p{view(c), rows, starts, lengths, k, v, ld, nullptr, nullptr, wide};
+    const dim3 grid = row_grid(p);
+    LB_CUDA(ctx, launch_pdl(ctx, c->dim > 128 ? lb_kv8_append_kernel<2> : lb_kv8_append_kernel<1>, grid, kRowThreads, 0, p));
+    ctx->launches++;
     return 0;
 }
 
 int loom_b200_kv8_read(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, const int32_t* starts, const int32_t* lengths, float* k, float* v) {
     if (int rc = kv8_ready(ctx, c, rows, starts, lengths, k, v, "kv8_read")) return rc;
     if (int rc = lb_set_device(ctx)) return rc;
-    ReadParams p{view(c), rows, starts, lengths, k, v};
-    const long long per = starts ? ((long long)rows * c->dim + kApThreads - 1) / kApThreads : 1;
-    lb_kv8_read_kernel<<<dim3((unsigned)(per < 256 ? per : 256), c->heads, c->seqs), kApThreads, 0, ctx->stream>>>(p);
-    LB_CHECK_LAUNCH(ctx, "lb_kv8_read_kernel");
+    const bool wide = c->dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
+    const RowParams p{view(c), rows, starts, lengths, nullptr, nullptr, 0, k, v, wide};
+    const dim3 grid = row_grid(p);
+    LB_CUDA(ctx, launch_pdl(ctx, lb_kv8_read_kernel, grid, kRowThreads, 0, p));
+    ctx->launches++;
     return 0;
 }
 
