@@ -14,7 +14,9 @@
 //   values  [dimension / 8][dimension % 8 = g][t][16 positions 8 j + 2 t + e, (j, e) in order]: the positions whose scores lane t holds
 //           after the products with the keys
 #include "serving.cuh"
+#include "umma.cuh"
 
+#include <cuda_fp16.h>
 #include <math_constants.h>
 
 #include <cmath>
@@ -419,6 +421,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) lb_kv8_read_kernel(const RowPa
 // for bit.
 constexpr int kAtThreads = 128;
 constexpr int kAtWarps = kAtThreads / 32;
+constexpr int kAtRowsNk = 4;      // the kernel for portions has up to 128 dimensions: a row's results stay in a thread's registers
 constexpr int kAtWideRows = 48;   // rows of a sequence beyond which its tiles are wide
 constexpr int kAtSizes = 8;       // sizes of parts that are tried: 1, 1 + 1/8, 1 + 2/8 and so on of an equal share
 constexpr int kAtOpenFew = 6;     // what an open block costs, in blocks: beside one token's rows (5.8 us, four blocks 3.4 us)
@@ -508,7 +511,8 @@ struct AttendShape {
     static constexpr size_t kSmem = kMerge > (size_t)kSlots * kSlot ? kMerge : (size_t)kSlots * kSlot;
 };
 
-template <int NK, int SETS>
+// WIDE: with wide tiles, for sequences that may have many rows
+template <int NK, int SETS, bool WIDE>
 __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_kv8_attend_kernel(const AttendParams p) {
     using S = AttendShape<NK, SETS>;
     constexpr int RW = S::kRows, NT = 4 * NK, LD = S::kLd, D4 = 8 * NK, RING = S::kRing, STAGES = S::kSlots / 2;
@@ -557,7 +561,8 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
         q.work = 0;
         if (q.a.count > 0 && fits(c, q.a)) {
             const int rows = q.a.count * p.group;
-            q.cost = rows > kAtWideRows ? 2 : 0;  // (all four warps work on it)
+            if (!WIDE && rows > kAtWideRows) return q;  // (the kernel for portions')
+            q.cost = WIDE && rows > kAtWideRows ? 2 : 0;  // (all four warps work on it)
             const int per = q.cost ? S::kTile : RW;
             q.blocks = (q.a.pos + q.a.count - 1) / kKvBlock + 1;
             q.tiles = (rows + per - 1) / per;
@@ -582,7 +587,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
                 continue;
             }
             v += q.work;
-            if (q.work == 0 && q.a.count > 0 && me == 0 && my_size == 0) {
+            if (q.work == 0 && q.a.count > 0 && me == 0 && my_size == 0 && !fits(c, q.a)) {
                 atomicExch(c.status, 7);
 #pragma unroll 1
                 for (long long j = 0; j < (long long)q.a.count * p.q_heads * hd; ++j) p.out[(size_t)q.a.row * p.q_heads * hd + j] = 0.f;
@@ -670,7 +675,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
         }
         if (!each && first + work_at(part_at) >= stop) break;
         const Span& a = sq.a;
-        const bool wide = sq.cost != 0;
+        const bool wide = WIDE && sq.cost != 0;
         const int unit = part_at / cuts, cut = part_at - unit * cuts;
         const int b0 = block_at(cut), b1 = block_at(cut + 1);
         // this part's place among the partial results, and the first one's of its tile
@@ -1240,6 +1245,8 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
 }
 
 
+#include "kv8_rows.cuh"
+
 Kv8 view(const loom_b200_kv8* c) {
     return {c->seqs, c->max_len, c->heads, c->dim, c->blocks, c->dim_k, c->dim_v, c->dim_o, c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->ctx->status_dev};
 }
@@ -1263,15 +1270,33 @@ static cudaError_t launch_pdl(loom_b200_ctx* ctx, void (*kern)(P), dim3 grid, in
 
 constexpr int kAtMostCtasPerSm = 2;
 
-template <int NK, int SETS>
+template <int NK, int SETS, bool WIDE>
 static int launch_attend(loom_b200_ctx* ctx, AttendParams p) {
     using S = AttendShape<NK, SETS>;
     p.ctas = ctx->sm_count * S::kPerSm;
     static_assert(S::kPerSm * (S::kSmem + 6 * 1024) <= 228 * 1024, "shared memory of an SM");
     p.part = (float*)((uint8_t*)p.cnt + (2 * (size_t)ctx->sm_count * kAtMostCtasPerSm + 1) * 4 / 16 * 16 + 16);
     const size_t smem = S::kSmem;
-    LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_attend_kernel<NK, SETS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    LB_CUDA(ctx, launch_pdl(ctx, lb_kv8_attend_kernel<NK, SETS>, dim3(p.ctas), kAtThreads, smem, p));
+    LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_attend_kernel<NK, SETS, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    LB_CUDA(ctx, launch_pdl(ctx, lb_kv8_attend_kernel<NK, SETS, WIDE>, dim3(p.ctas), kAtThreads, smem, p));
+    ctx->launches++;
+    return 0;
+}
+
+// (without the code for wide tiles one token's attention is 5 % faster)
+template <int NK>
+static int launch_few(loom_b200_ctx* ctx, const AttendParams& p, bool few, bool wide) {
+    if (wide) return few ? launch_attend<NK, 1, true>(ctx, p) : launch_attend<NK, 2, true>(ctx, p);
+    return few ? launch_attend<NK, 1, false>(ctx, p) : launch_attend<NK, 2, false>(ctx, p);
+}
+
+template <int NK>
+static int launch_rows(loom_b200_ctx* ctx, AttendParams p) {
+    using S = RowsShape<NK>;
+    p.ctas = 2 * ctx->sm_count;
+    p.part = (float*)((uint8_t*)p.cnt + (2 * (size_t)ctx->sm_count * kAtMostCtasPerSm + 1) * 4 / 16 * 16 + 16);
+    LB_CUDA(ctx, cudaFuncSetAttribute(lb_kv8_rows_kernel<NK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem));
+    LB_CUDA(ctx, launch_pdl(ctx, lb_kv8_rows_kernel<NK>, dim3(p.ctas), kRwThreads, S::kSmem, p));
     ctx->launches++;
     return 0;
 }
@@ -1301,7 +1326,9 @@ int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_
     c->dim_o = (head_dim + 3) / 4 * 4;
     const size_t blocks = (size_t)sequences * kv_heads * c->blocks, open = (size_t)sequences * kv_heads * 2 * kKvBlock * c->dim_o * 4;
     const size_t ctas = (size_t)ctx->sm_count * kAtMostCtasPerSm;
-    c->work_bytes = (2 * ctas + 1) * 4 + 32 + (2 * ctas + 1) * (head_dim > 128 ? AttendShape<8, 1>::kTile : AttendShape<4, 2>::kTile) * ((head_dim + 3) / 4 * 4 + 4) * 4;
+    // counters, then parts: a few rows' of every CTA, or the tiles' of a portion
+    const size_t dims = (head_dim + 31) / 32 * 32, few = (head_dim > 128 ? AttendShape<8, 1>::kTile : AttendShape<4, 2>::kTile) * (size_t)(c->dim_o + 4), many = head_dim > 128 ? 0 : kRwTile * (dims + 2);
+    c->work_bytes = (2 * ctas + 1) * 4 + 32 + (2 * ctas + 1) * (few > many ? few : many) * 4;
     cudaError_t e = cudaSuccess;
     const auto get = [&](void** p, size_t bytes) {
         if (e == cudaSuccess) e = cudaMalloc(p, bytes);
@@ -1404,16 +1431,24 @@ int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, int hea
     p.part_ld = (c->dim + 3) / 4 * 4 + 4;
     // tiles of eight rows a warp where sequences have no more on the average (any number is right with either)
     const bool few = (long long)rows * p.group <= 8LL * (starts ? c->seqs : rows);
-    switch (c->dim_k / 32) {
-        case 1: return few ? launch_attend<1, 1>(ctx, p) : launch_attend<1, 2>(ctx, p);
-        case 2: return few ? launch_attend<2, 1>(ctx, p) : launch_attend<2, 2>(ctx, p);
-        case 3: return few ? launch_attend<3, 1>(ctx, p) : launch_attend<3, 2>(ctx, p);
-        case 4: return few ? launch_attend<4, 1>(ctx, p) : launch_attend<4, 2>(ctx, p);
-        case 5: return launch_attend<5, 1>(ctx, p);
-        case 6: return launch_attend<6, 1>(ctx, p);
-        case 7: return launch_attend<7, 1>(ctx, p);
-        default: return launch_attend<8, 1>(ctx, p);
+    // Sequences of many rows go to the kernel for portions, where the call has two rows a sequence on the average (300 rows of 4 heads at 2900: 66 us
+    // instead of 93; but 5 us are its launch where there are none: 16 sequences of one row 41.6 instead of 36.4 us).
+    const int nk = c->dim_k / 32;
+    const bool portions = nk <= kAtRowsNk && (starts ? rows > 2 * c->seqs && (long long)rows * p.group > kAtWideRows : p.group > kAtWideRows);
+    const bool wide = !portions && (long long)(starts ? rows : 1) * p.group > kAtWideRows;
+    int rc = 0;
+    switch (nk) {
+        case 1: rc = launch_few<1>(ctx, p, few, wide); break;
+        case 2: rc = launch_few<2>(ctx, p, few, wide); break;
+        case 3: rc = launch_few<3>(ctx, p, few, wide); break;
+        case 4: rc = launch_few<4>(ctx, p, few, wide); break;
+        case 5: rc = launch_attend<5, 1, true>(ctx, p); break;
+        case 6: rc = launch_attend<6, 1, true>(ctx, p); break;
+        case 7: rc = launch_attend<7, 1, true>(ctx, p); break;
+        default: rc = launch_attend<8, 1, true>(ctx, p);
     }
+    if (rc || !portions) return rc;
+    return nk == 1 ? launch_rows<1>(ctx, p) : nk == 2 ? launch_rows<2>(ctx, p) : nk == 3 ? launch_rows<3>(ctx, p) : launch_rows<4>(ctx, p);
 }
 
 }  // extern "C"
