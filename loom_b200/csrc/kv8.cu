@@ -1431,8 +1431,8 @@ int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, int hea
     p.part_ld = (c->dim + 3) / 4 * 4 + 4;
     // tiles of eight rows a warp where sequences have no more on the average (any number is right with either)
     const bool few = (long long)rows * p.group <= 8LL * (starts ? c->seqs : rows);
-    // Sequences of many rows go to the kernel for portions, where the call has two rows a sequence on the average (300 rows of 4 heads at 2900: 66 us
-    // instead of 93; but 5 us are its launch where there are none: 16 sequences of one row 41.6 instead of 36.4 us).
+    // Sequences of many rows go to the kernel for portions, where the call has more than two rows a sequence on the average (13 to 512 rows of 4
+    // heads at 2900: 43 to 83 us instead of 125 to 238; but 5 us are its launch where there are none: 16 sequences of one row 41.6 us instead of 36.4).
     const int nk = c->dim_k / 32;
     const bool portions = nk <= kAtRowsNk && (starts ? rows > 2 * c->seqs && (long long)rows * p.group > kAtWideRows : p.group > kAtWideRows);
     const bool wide = !portions && (long long)(starts ? rows : 1) * p.group > kAtWideRows;

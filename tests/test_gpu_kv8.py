@@ -314,6 +314,121 @@ def test_starts_that_do_not_ascend_or_pass_the_rows(ctx):
     c.drop()
 
 
+def check_some(c, rng, call, counts, heads, most=40, scale=0.0):
+    """A call's rows against the plain implementation: the first and last ones of every sequence, and some between them."""
+    q, got = c.attend(rng, call, heads, scale)
+    at = 0
+    for s, n in enumerate(counts):
+        first = len(c.k[s]) - n
+        k, v = kit.held(c.k[s]), kit.held(c.v[s])
+        for j in sorted({0, n - 1, *rng.integers(0, n, min(n, most)).tolist()} if n else {}):
+            want, tol = kit.attend(q[at + j:at + j + 1], k, v, first + j, scale or None)
+            off = np.abs(got[at + j] - want[0])
+            assert (off <= tol[0]).all(), (s, j, n, first, (off / tol[0]).max())
+        at += n
+    return q, got
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim", [(20, 5, 128), (6, 2, 72), (7, 1, 96), (16, 16, 32), (9, 3, 50), (64, 1, 128)])
+@pytest.mark.parametrize("before, count", [(0, 65), (1000, 257), (63, 128), (640, 49), (2900, 300)])
+def test_portions(ctx, heads, kv_heads, dim, before, count):
+    rng = np.random.default_rng(before + count + dim)
+    c = Cache(ctx, 1, before + count, kv_heads, dim)
+    if before:
+        c.append(rng, [before], spread=2.0)
+    call = c.append(rng, [count])
+    check_some(c, rng, call, [count], heads, 12)
+    c.drop()
+
+
+def test_more_tiles_than_ctas(ctx):
+    """Portions of which a CTA takes several, and single rows beside them; again, bit for bit."""
+    rng = np.random.default_rng(20)
+    c = Cache(ctx, 5, 1700, 8, 64)
+    c.append(rng, [100, 0, 37, 64, 200])
+    counts = [1500, 1, 400, 0, 90]
+    call = c.append(rng, counts)
+    q, got = check_some(c, rng, call, counts, 48, 15)
+    for _ in range(3):
+        assert np.array_equal(c.attend(rng, call, 48, q=q)[1], got)
+    c.drop()
+
+
+@pytest.mark.parametrize("dim", [32, 128])
+def test_query_heads_that_are_many(ctx, dim):
+    """One row a sequence, without starts, of more heads than the kernel for few rows takes."""
+    rng = np.random.default_rng(dim)
+    c = Cache(ctx, 4, 700, 1, dim)
+    c.append(rng, [600, 3, 64, 255])
+    call = c.append(rng, [1, 1, 1, 1], step=True)
+    c.check(rng, call, [1, 1, 1, 1], 150)
+
+
+def test_a_portion_with_rows_that_are_not_finite(ctx):
+    """Keys, values and queries; what is not finite reaches the rows that see it, and no others."""
+    rng = np.random.default_rng(21)
+
+    def change(k, v):
+        k[300, 0, 3] = np.nan
+        v[310, 1, 2] = np.inf
+        k[20, 1, 5] = np.inf
+    c = Cache(ctx, 1, 1000, 2, 64)
+    c.append(rng, [650])
+    call = c.append(rng, [330], change=change)  # positions 650 .. 979, blocks 10 .. 15; 960 on are open
+    q = rng.standard_normal((330, 8, 64)).astype(np.float32)
+    q[7, 2, 1] = np.nan
+    _, out = c.attend(rng, call, 8, q=q)
+    bad = ~np.isfinite(out).all(2)
+    want = np.zeros((330, 8), bool)
+    want[7, 2] = True
+    pos = np.arange(330) + 650
+    want[pos >= (650 + 300) // 64 * 64, :4] = True  # a whole block reads as not-a-numbers
+    want[pos >= (650 + 20) // 64 * 64, 4:] = True
+    want[pos >= 960, 4:] = True
+    assert np.array_equal(bad, want), np.argwhere(bad != want)[:5]
+    for h in (0, 3):
+        for j in (0, 100, 240):
+            o, tol = kit.attend(q[j:j + 1], kit.held(c.k[0]), kit.held(c.v[0]), 650 + j)
+            assert (np.abs(out[j, h] - o[0, h]) <= tol[0, h]).all()
+    c.drop()
+
+
+def test_open_rows_that_are_not_finite(ctx):
+    rng = np.random.default_rng(22)
+
+    def change(k, v):
+        k[40, 0, 3] = np.nan
+        v[50, 1, 2] = -np.inf
+    c = Cache(ctx, 1, 200, 2, 64)
+    c.append(rng, [64])
+    call = c.append(rng, [60], change=change)
+    q, out = c.attend(rng, call, 8)
+    bad = ~np.isfinite(out).all(2)
+    want = np.zeros((60, 8), bool)
+    want[40:, :4] = True
+    want[50:, 4:] = True
+    assert np.array_equal(bad, want)
+    for j in (0, 39, 49):
+        o, tol = kit.attend(q[j:j + 1], kit.held(c.k[0]), kit.held(c.v[0]), 64 + j)
+        good = ~bad[j]
+        assert (np.abs(out[j, good] - o[0, good]) <= tol[0, good]).all()
+    c.drop()
+
+
+@pytest.mark.parametrize("spread", [1e-30, 1e-4, 1e4, 1e15])
+def test_portions_of_small_and_large_values(ctx, spread):
+    """Keys by `spread`, queries by its inverse: the same scores, whatever power of two stands in between."""
+    rng = np.random.default_rng(23)
+    c = Cache(ctx, 1, 400, 1, 64)
+    call = c.append(rng, [200], change=lambda k, v: np.multiply(k, np.float32(spread), out=k))
+    q = (rng.standard_normal((200, 4, 64)) / spread).astype(np.float32)
+    _, got = c.attend(rng, call, 4, q=q)
+    for j in (0, 63, 64, 150, 199):
+        o, tol = kit.attend(q[j:j + 1], kit.held(c.k[0]), kit.held(c.v[0]), j)
+        assert (np.abs(got[j] - o[0]) <= tol[0]).all()
+    c.drop()
+
+
 def test_frames_and_repeats():
     """A recorded step replayed with new lengths, beside another frame of the same cache: the same bits as eager calls."""
     rng = np.random.default_rng(11)
