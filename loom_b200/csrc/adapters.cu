@@ -15,7 +15,7 @@
 // to 6912 rows of rank 16, five adapters: 62.8 us, 0.49 of what 197 MB take at the copy's rate -- 8 us to find the tiles, 10 for down x,
 // 3 for its sums, 35 for up h and the rows of base and out at 5 TB/s.  (Asking L2 for rows of x and base some steps ahead: 64 to 69 us; tiles
 // of 64 tokens, which read the adapter less often: 60.7 us, but 28 us instead of 20 for 512 tokens.)  One token 5.0 us, sixteen tokens of as
-// many adapters, 4096 to 14336: 20.9 us.
+// many adapters, 4096 to 14336: 20.0 us.  4096 tokens of rank 64: 108 us, where the adapter's rows come from L2 for every sixteen of them.
 #include "serving.cuh"
 
 #include <cuda_bf16.h>
@@ -33,6 +33,7 @@ constexpr int kAdTile = 16;  // tokens
 
 struct AdapterParams {
     const void *down, *up;
+    size_t down_plane, up_plane;  // bytes from one part of float32 values to the next
     const int* rank;
     const float* scale;
     const int32_t* slot;
@@ -85,48 +86,45 @@ __device__ __forceinline__ void products(float (&d)[4], const uint32_t (&a)[3][4
     mma_bf16(d, a[0][0], a[0][1], a[0][2], a[0][3], b0[0], b1[0]);
 }
 
-// consecutive values of a row of an adapter's matrix, four or eight, as they come
+// Consecutive values of a row of an adapter's matrix, four or eight, as they come: bf16, or the three parts of float32 values, which lie
+// `plane` bytes apart.
 template <bool F32, int N>
 struct Raw {
-    uint32_t w[F32 ? N : N / 2];
+    uint32_t w[F32 ? 3 : 1][N / 2];
 };
 template <bool F32, int N>
-__device__ __forceinline__ void load_raw(const void* base, size_t at, Raw<F32, N>& r) {
-    constexpr int W = F32 ? N : N / 2;
-    const uint8_t* p = static_cast<const uint8_t*>(base) + at * (F32 ? 4 : 2);
-    if (W == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        r.w[0] = v.x;
-        r.w[1] = v.y;
-    } else {
+__device__ __forceinline__ void load_raw(const uint8_t* base, size_t plane, size_t at, Raw<F32, N>& r) {
 #pragma unroll
-        for (int i = 0; i < W; i += 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
-            r.w[i] = v.x;
-            r.w[i + 1] = v.y;
-            r.w[i + 2] = v.z;
-            r.w[i + 3] = v.w;
+    for (int k = 0; k < (F32 ? 3 : 1); ++k) {
+        const uint8_t* p = base + k * plane + at * 2;
+        if (N == 4) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+            r.w[k][0] = v.x;
+            r.w[k][1] = v.y;
+        } else {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+            r.w[k][0] = v.x;
+            r.w[k][1] = v.y;
+            r.w[k][N == 4 ? 0 : 2] = v.z;
+            r.w[k][N == 4 ? 0 : 3] = v.w;
         }
     }
 }
 // the four values from 4 i on as B registers of both pairs
 template <bool F32, int N>
 __device__ __forceinline__ void parts_of(const Raw<F32, N>& r, int i, uint32_t (&b0)[3], uint32_t (&b1)[3]) {
-    if (F32) {
-        split2(__uint_as_float(r.w[F32 ? 4 * i : 0]), __uint_as_float(r.w[F32 ? 4 * i + 1 : 0]), b0);
-        split2(__uint_as_float(r.w[F32 ? 4 * i + 2 : 0]), __uint_as_float(r.w[F32 ? 4 * i + 3 : 0]), b1);
-    } else {
-        b0[0] = r.w[F32 ? 0 : 2 * i];
-        b1[0] = r.w[F32 ? 0 : 2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < (F32 ? 3 : 1); ++k) {
+        b0[k] = r.w[k][2 * i];
+        b1[k] = r.w[k][2 * i + 1];
     }
 }
 
-// CTAs of an SM (three or four with fewer registers: 62 and 107 us for 2999 tokens, 62.8 with two, and more for all other sizes)
-constexpr int ad_per_sm(int tiles, bool f32) { return tiles > 4 && f32 ? 1 : 2; }
+constexpr int kAdPerSm = 2;  // CTAs (three or four with fewer registers each: 62 and 107 us for 2999 tokens, 62.8 with two, and more for all other sizes)
 
-// TILES: ranks of one pass over x / 8
+// TILES: ranks of one pass over x / 8.  Four at most for float32, whose 64 take so two passes: 4096 tokens 172 us, with eight and one CTA an SM 235.
 template <int TILES, bool F32>
-__global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters_kernel(const AdapterParams p) {
+__global__ void __launch_bounds__(kAdThreads, kAdPerSm) lb_adapters_kernel(const AdapterParams p) {
     constexpr int M = kAdTile, KS = kAdWarps, kAdPass = 8 * TILES;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     float* part = reinterpret_cast<float*>(smem_raw);  // [KS][M][kAdPass] down x of this CTA's columns
@@ -236,13 +234,12 @@ __global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters
     const int rank = __ldg(p.rank + group);
     const float scale = __ldg(p.scale + group);
     const int tok0 = s_tok[g], tok1 = s_tok[g + 8];
-    const size_t wsize = F32 ? 4 : 2;
-    constexpr int CH = TILES == 8 || !F32 ? 4 : 2;  // columns of out that a warp takes at a time, in sixteens
-    const uint8_t* up = static_cast<const uint8_t*>(p.up) + (size_t)group * p.rows_pad * p.rank_pad * wsize;
+    constexpr int CH = TILES == 2 && !F32 ? 4 : 2;  // columns of out that a warp takes at a time, in sixteens
+    const uint8_t* up = static_cast<const uint8_t*>(p.up) + (size_t)group * p.rows_pad * p.rank_pad * 2;
     {  // the first of them: the rows of up that they take
         const int c = ((int)crank * KS + warp) * 16 * CH, n = min(16 * CH, p.rows_pad - c);
-        const int bytes = n * p.rank_pad * (int)wsize;
-        for (int i = lane * 128; i < bytes; i += 32 * 128) prefetch_l2(up + (size_t)c * p.rank_pad * wsize + i);
+        for (int k = 0; k < (F32 ? 3 : 1); ++k)
+            for (int i = lane * 128; i < n * p.rank_pad * 2; i += 32 * 128) prefetch_l2(up + k * p.up_plane + (size_t)c * p.rank_pad * 2 + i);
     }
 
     // ---- h = c down x: 32 columns at a time, eight of them a lane ----
@@ -260,7 +257,7 @@ __global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters
             if (k + 3 < p.cols) f.w = __ldg(row + k + 3);
             return f;
         };
-        const uint8_t* down = static_cast<const uint8_t*>(p.down) + (size_t)group * p.rank_pad * p.cols_pad * wsize;
+        const uint8_t* down = static_cast<const uint8_t*>(p.down) + (size_t)group * p.rank_pad * p.cols_pad * 2;
         for (int n0 = 0; n0 < rank; n0 += kAdPass) {
             const int tiles = (min(rank - n0, kAdPass) + 7) / 8, width = 8 * tiles;
             float acc[TILES][4] = {};
@@ -276,7 +273,7 @@ __global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters
                 Raw<F32, 8> w[TILES];
 #pragma unroll
                 for (int n = 0; n < TILES; ++n)
-                    if (n < tiles) load_raw<F32, 8>(down, (size_t)(n0 + 8 * n + g) * p.cols_pad + k, w[n]);
+                    if (n < tiles) load_raw<F32, 8>(down, p.down_plane, (size_t)(n0 + 8 * n + g) * p.cols_pad + k, w[n]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     uint32_t a[3][4], v[3];
@@ -346,32 +343,44 @@ __global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters
                 if (wide && p.base && tok >= 0 && c < p.rows) base[j][z] = __ldcs(reinterpret_cast<const float4*>(p.base + (size_t)tok * p.rows + c));
             }
         float acc[CH][2][4] = {};
-        for (int k0 = 0; k0 < rank; k0 += 16) {
-            Raw<F32, 4> w[CH][2];
+        // KU stretches of 4 KV ranks, lane t the KV from KV t on: every row of up that is there in flight at once
+        constexpr int KV = TILES == 2 ? 4 : 8, KU = TILES == 8 ? 2 : 1;
+        for (int k0 = 0; k0 < rank; k0 += 4 * KV * KU) {
+            Raw<F32, KV> w[KU][CH][2];
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
+            for (int u = 0; u < KU; ++u)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    if (c0 + 16 * j < p.rows_pad) load_raw<F32, 4>(up, (size_t)(c0 + 16 * j + col_a + 2 * n) * p.rank_pad + k0 + 4 * t, w[j][n]);
-            uint32_t a[3][4];
+                for (int j = 0; j < CH; ++j)
 #pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const __nv_bfloat16* from = hs + ((size_t)i * M + g) * hs_ld + k0 + 4 * t;
-                uint2 r0 = *reinterpret_cast<const uint2*>(from), r1 = *reinterpret_cast<const uint2*>(from + 8 * hs_ld);
-                a[i][0] = r0.x;
-                a[i][1] = r1.x;
-                a[i][2] = r0.y;
-                a[i][3] = r1.y;
-            }
+                    for (int n = 0; n < 2; ++n)
+                        if (c0 + 16 * j < p.rows_pad && (u == 0 || k0 + 4 * KV * u < rank))
+                            load_raw<F32, KV>(up, p.up_plane, (size_t)(c0 + 16 * j + col_a + 2 * n) * p.rank_pad + k0 + 4 * KV * u + KV * t, w[u][j][n]);
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
-                if (c0 + 16 * j < p.rows_pad)
+            for (int u = 0; u < KU; ++u) {
+                if (u > 0 && k0 + 4 * KV * u >= rank) break;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        uint32_t b0[3], b1[3];
-                        parts_of<F32, 4>(w[j][n], 0, b0, b1);
-                        products<F32>(acc[j][n], a, b0, b1);
+                for (int e = 0; e < KV / 4; ++e) {
+                    uint32_t a[3][4];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        const __nv_bfloat16* from = hs + ((size_t)i * M + g) * hs_ld + k0 + 4 * KV * u + KV * t + 4 * e;
+                        const uint2 r0 = *reinterpret_cast<const uint2*>(from), r1 = *reinterpret_cast<const uint2*>(from + 8 * hs_ld);
+                        a[i][0] = r0.x;
+                        a[i][1] = r1.x;
+                        a[i][2] = r0.y;
+                        a[i][3] = r1.y;
                     }
+#pragma unroll
+                    for (int j = 0; j < CH; ++j)
+                        if (c0 + 16 * j < p.rows_pad)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) {
+                                uint32_t b0[3], b1[3];
+                                parts_of<F32, KV>(w[u][j][n], e, b0, b1);
+                                products<F32>(acc[j][n], a, b0, b1);
+                            }
+                }
+            }
         }
 #pragma unroll
         for (int j = 0; j < CH; ++j)
@@ -393,16 +402,16 @@ __global__ void __launch_bounds__(kAdThreads, ad_per_sm(TILES, F32)) lb_adapters
     }
 }
 
-// a slot's matrices into their padded places
-template <typename WT>
-__global__ void lb_adapters_put_kernel(const void* __restrict__ src, int src_dtype, int rows, int cols, int rows_pad, int cols_pad, WT* __restrict__ dst) {
+// a slot's matrix into its padded place: bf16, or float32 values in three parts
+__global__ void lb_adapters_put_kernel(const void* __restrict__ src, int src_dtype, int rows, int cols, int rows_pad, int cols_pad, int parts, size_t plane, uint8_t* __restrict__ dst) {
     const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= (size_t)rows_pad * cols_pad) return;
     const int r = (int)(i / cols_pad), c = (int)(i % cols_pad);
     float f = 0.f;
     if (r < rows && c < cols)
         f = src_dtype == LOOM_B200_DTYPE_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(src)[(size_t)r * cols + c]) : static_cast<const float*>(src)[(size_t)r * cols + c];
-    dst[i] = (WT)f;
+    if (parts == 1) reinterpret_cast<__nv_bfloat16*>(dst)[i] = __float2bfloat16_rn(f);
+    for (int k = 0; k < parts && parts > 1; ++k) *reinterpret_cast<unsigned short*>(dst + k * plane + i * 2) = (unsigned short)(__float_as_uint(cut(f)) >> 16);
 }
 __global__ void lb_adapters_meta_kernel(int* rank, float* scale, int r, float s) {
     *rank = r;
@@ -420,7 +429,7 @@ int launch_adapters(loom_b200_ctx* ctx, const AdapterParams& p, int tiles) {
     LB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     // As many CTAs a tile as are there at once.  Clusters of more than eight find their places in a GPC less and less well (256 tokens of
     // two adapters: 12 CTAs a tile 13.9 us, 14 18.6 us), so those leave a quarter free; 16 of 16 fit (16 tokens: 20.9 us, with 13 26.2 us).
-    const int most = ad_per_sm(TILES, F32) * ctx->sm_count;
+    const int most = kAdPerSm * ctx->sm_count;
     int size = most * 7 / 8 / tiles;
     if (size >= kAdMostCtas) size = kAdMostCtas;
     else if (size > 8) size = most * 3 / 4 / tiles > 8 ? most * 3 / 4 / tiles : 8;
@@ -465,10 +474,10 @@ int loom_b200_adapters_create(loom_b200_ctx* ctx, int slots, int rows, int cols,
     a->cols = cols;
     a->max_rank = max_rank;
     a->dtype = dtype;
-    a->rank_pad = (max_rank + 15) / 16 * 16;
+    a->rank_pad = max_rank <= 16 ? 16 : (max_rank + 31) / 32 * 32;  // (what lb_adapters_kernel takes at a time)
     a->cols_pad = (cols + 31) / 32 * 32;
     a->rows_pad = (rows + 15) / 16 * 16;
-    const size_t w = dtype == LOOM_B200_DTYPE_F32 ? 4 : 2;
+    const size_t w = dtype == LOOM_B200_DTYPE_F32 ? 6 : 2;  // (float32 values as three of 16 bits)
     cudaError_t e = cudaMalloc(&a->down, (size_t)slots * a->rank_pad * a->cols_pad * w);
     if (e == cudaSuccess) e = cudaMalloc(&a->up, (size_t)slots * a->rows_pad * a->rank_pad * w);
     if (e == cudaSuccess) e = cudaMalloc((void**)&a->rank, (size_t)slots * 4);
@@ -492,7 +501,7 @@ int loom_b200_adapters_put(loom_b200_ctx* ctx, loom_b200_adapters* a, int slot, 
     LB_REQUIRE(ctx, src_dtype == LOOM_B200_DTYPE_F32 || src_dtype == LOOM_B200_DTYPE_BF16, "adapters_put: dtype %d", src_dtype);
     if (ctx->capturing) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "adapters_put cannot be recorded");
     if (int rc = lb_set_device(ctx)) return rc;
-    const size_t w = a->dtype == LOOM_B200_DTYPE_F32 ? 4 : 2, sw = src_dtype == LOOM_B200_DTYPE_F32 ? 4 : 2;
+    const size_t sw = src_dtype == LOOM_B200_DTYPE_F32 ? 4 : 2;
     for (int m = 0; m < 2 && rank > 0; ++m) {
         const void* src = m ? up : down;
         const int rows = m ? a->rows : rank, cols = m ? rank : a->cols;
@@ -504,10 +513,9 @@ int loom_b200_adapters_put(loom_b200_ctx* ctx, loom_b200_adapters* a, int slot, 
             src = ctx->scratch;
         }
         const size_t total = (size_t)rows_pad * cols_pad;
-        uint8_t* dst = static_cast<uint8_t*>(m ? a->up : a->down) + (size_t)slot * total * w;
+        uint8_t* dst = static_cast<uint8_t*>(m ? a->up : a->down) + (size_t)slot * total * 2;
         const unsigned grid = (unsigned)((total + 255) / 256);
-        if (a->dtype == LOOM_B200_DTYPE_F32) lb_adapters_put_kernel<float><<<grid, 256, 0, ctx->stream>>>(src, src_dtype, rows, cols, rows_pad, cols_pad, (float*)dst);
-        else lb_adapters_put_kernel<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(src, src_dtype, rows, cols, rows_pad, cols_pad, (__nv_bfloat16*)dst);
+        lb_adapters_put_kernel<<<grid, 256, 0, ctx->stream>>>(src, src_dtype, rows, cols, rows_pad, cols_pad, a->dtype == LOOM_B200_DTYPE_F32 ? 3 : 1, (size_t)a->slots * total * 2, dst);
         LB_CHECK_LAUNCH(ctx, "lb_adapters_put_kernel");
     }
     lb_adapters_meta_kernel<<<1, 1, 0, ctx->stream>>>(a->rank + slot, a->scale + slot, rank, scale);
@@ -549,6 +557,8 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
     AdapterParams p;
     p.down = a->down;
     p.up = a->up;
+    p.down_plane = (size_t)a->slots * a->rank_pad * a->cols_pad * 2;
+    p.up_plane = (size_t)a->slots * a->rows_pad * a->rank_pad * 2;
     p.rank = a->rank;
     p.scale = a->scale;
     p.slot = slot;
@@ -567,7 +577,7 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
     p.single = tokens <= 16;
     const int groups = a->slots + 1;
     const int tiles = p.single || tokens <= groups ? tokens : groups + (tokens - groups) / kAdTile;  // at most
-    const auto launch = a->dtype == LOOM_B200_DTYPE_F32 ? a->max_rank <= 16 ? launch_adapters<2, true> : a->max_rank <= 32 ? launch_adapters<4, true> : launch_adapters<8, true>
+    const auto launch = a->dtype == LOOM_B200_DTYPE_F32 ? a->max_rank <= 16 ? launch_adapters<2, true> : launch_adapters<4, true>
                                                         : a->max_rank <= 16 ? launch_adapters<2, false> : a->max_rank <= 32 ? launch_adapters<4, false> : launch_adapters<8, false>;
     return launch(ctx, p, tiles);
 }
