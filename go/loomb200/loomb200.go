@@ -394,6 +394,101 @@ func (dec *Decoder) ReadTokensBatch(batch, n int) ([]int32, error) {
 	return out, dec.ctx.check(rc)
 }
 
+// ---- several requests on one decoder (no counterpart in poly) ----
+
+// SampleParams are one sequence's: Temperature 0 takes the largest logit, TopK 0 and TopP 1 keep all.
+type SampleParams struct {
+	Temperature float32
+	TopK        int32
+	TopP, MinP  float32
+	Uniform     float32 // random number in [0, 1)
+}
+
+// Sample draws the next token of sequence seq, or of every one (-1), from the logits of the last forward; logprobs may be nil.
+func (dec *Decoder) Sample(seq int, params []SampleParams, logprobs []float32) ([]int32, error) {
+	n := len(params)
+	temperature, topP, minP, uniform := make([]float32, n), make([]float32, n), make([]float32, n), make([]float32, n)
+	topK, tokens := make([]int32, n), make([]int32, n)
+	for i, p := range params {
+		temperature[i], topK[i], topP[i], minP[i], uniform[i] = p.Temperature, p.TopK, p.TopP, p.MinP, p.Uniform
+	}
+	rc := C.loom_b200_decoder_sample(dec.d, C.int(seq), f32ptr(temperature), (*C.int32_t)(unsafe.Pointer(&topK[0])), f32ptr(topP), f32ptr(minP),
+		f32ptr(uniform), (*C.int32_t)(unsafe.Pointer(&tokens[0])), f32ptr(logprobs))
+	return tokens, dec.ctx.check(rc)
+}
+
+// Adapters are low-rank adapters of several requests for one matrix.
+type Adapters struct {
+	ctx *Context
+	a   *C.loom_b200_adapters
+}
+
+func (ctx *Context) NewAdapters(slots, rows, cols, maxRank, dtype int) (*Adapters, error) {
+	a := &Adapters{ctx: ctx}
+	if err := ctx.check(C.loom_b200_adapters_create(ctx.c, C.int(slots), C.int(rows), C.int(cols), C.int(maxRank), C.int(dtype), &a.a)); err != nil {
+		return nil, err
+	}
+	return a, nil
+}
+
+// Put fills a slot from down [rank][cols] and up [rows][rank]; rank 0 empties it.
+func (a *Adapters) Put(slot, rank int, scale float32, down, up []float32) error {
+	return a.ctx.check(C.loom_b200_adapters_put(a.ctx.c, a.a, C.int(slot), C.int(rank), C.float(scale), unsafe.Pointer(f32ptr(down)),
+		unsafe.Pointer(f32ptr(up)), DTypeF32, 0))
+}
+
+// Apply adds the adapters of the tokens' slots (int32 in device memory) to base; out may be base.
+func (a *Adapters) Apply(tokens int, slot, x *Buffer, ldx int, base, out *Buffer) error {
+	return a.ctx.check(C.loom_b200_adapters_apply(a.ctx.c, a.a, C.int(tokens), (*C.int32_t)(slot.p), (*C.float)(x.p), C.longlong(ldx),
+		(*C.float)(base.p), (*C.float)(out.p)))
+}
+
+func (a *Adapters) Free() {
+	if a.a != nil {
+		C.loom_b200_adapters_free(a.ctx.c, a.a)
+		a.a = nil
+	}
+}
+
+// KV8 is a cache of keys and values in 8 bits for several sequences; the caller keeps their lengths in device memory.
+type KV8 struct {
+	ctx *Context
+	c   *C.loom_b200_kv8
+}
+
+func (ctx *Context) NewKV8(sequences, maxLen, kvHeads, headDim int) (*KV8, error) {
+	k := &KV8{ctx: ctx}
+	if err := ctx.check(C.loom_b200_kv8_create(ctx.c, C.int(sequences), C.int(maxLen), C.int(kvHeads), C.int(headDim), &k.c)); err != nil {
+		return nil, err
+	}
+	return k, nil
+}
+
+// starts nil: one row each of the first `rows` sequences.
+func startsPtr(starts *Buffer) *C.int32_t {
+	if starts == nil {
+		return nil
+	}
+	return (*C.int32_t)(starts.p)
+}
+
+func (k *KV8) Append(rows int, starts, lengths, keys, values *Buffer, ld int) error {
+	return k.ctx.check(C.loom_b200_kv8_append(k.ctx.c, k.c, C.int(rows), startsPtr(starts), (*C.int32_t)(lengths.p), (*C.float)(keys.p),
+		(*C.float)(values.p), C.longlong(ld)))
+}
+
+func (k *KV8) Attend(rows, heads int, starts, lengths, q *Buffer, ldq int, scale float64, out *Buffer) error {
+	return k.ctx.check(C.loom_b200_kv8_attend(k.ctx.c, k.c, C.int(rows), C.int(heads), startsPtr(starts), (*C.int32_t)(lengths.p), (*C.float)(q.p),
+		C.longlong(ldq), C.double(scale), (*C.float)(out.p)))
+}
+
+func (k *KV8) Free() {
+	if k.c != nil {
+		C.loom_b200_kv8_free(k.ctx.c, k.c)
+		k.c = nil
+	}
+}
+
 // ---- float matrices and layer stacks: decoders whose layers are set one by one (no counterpart in poly) ----
 
 // Element types of a Matrix.
