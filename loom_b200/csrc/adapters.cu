@@ -28,7 +28,7 @@ constexpr int kAdMaxRank = 256;
 constexpr int kAdMaxSlots = 4096;
 constexpr int kAdMostCtas = 16;
 constexpr int kAdGroups = 24 * 1024;  // where the tokens' groups stand while a tile is being found, behind histogram and flags
-constexpr int kAdKept = 4096;         // tokens whose group is kept there
+constexpr int kAdKept = 4096;         // tokens of a launch
 constexpr int kAdTile = 16;  // tokens
 
 struct AdapterParams {
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kAdThreads, kAdPerSm) lb_adapters_kernel(const
         __syncthreads();
     } else {
         int* count = reinterpret_cast<int*>(smem_raw);                                          // [slots + 1]
-        unsigned short* groups = reinterpret_cast<unsigned short*>(smem_raw + kAdGroups);       // [tokens] the first of them, at least
+        unsigned short* groups = reinterpret_cast<unsigned short*>(smem_raw + kAdGroups);       // [tokens]
         uint8_t* valid = smem_raw + kAdGroups - kAdMaxSlots;                                     // [slots]
         for (int i = tid; i <= p.slots; i += kAdThreads) {
             count[i] = 0;
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kAdThreads, kAdPerSm) lb_adapters_kernel(const
         for (int i = tid; i < p.tokens; i += kAdThreads) {
             const int s = group_at(i);
             atomicAdd(&count[s], 1);
-            if (i < kAdKept) groups[i] = (unsigned short)s;
+            groups[i] = (unsigned short)s;
         }
         __syncthreads();
         int before = 0;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kAdThreads, kAdPerSm) lb_adapters_kernel(const
         if (tid < M) s_tok[tid] = -1;
         // the tokens in their order: a stretch of them to every warp, how many of each are the group's, then the tile's
         const int per = ((p.tokens + kAdWarps - 1) / kAdWarps + 31) / 32 * 32, from = warp * per, to = min(p.tokens, from + per);
-        const auto is_mine = [&](int i) { return i < to && (i < kAdKept ? groups[i] : group_at(i)) == group; };
+        const auto is_mine = [&](int i) { return i < to && groups[i] == group; };
         int here = 0;
         for (int i0 = from; i0 < to; i0 += 32) here += __popc(__ballot_sync(0xffffffffu, is_mine(i0 + lane)));
         if (lane == 0) s_warp[warp] = here;
@@ -561,10 +561,6 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
     p.up_plane = (size_t)a->slots * a->rows_pad * a->rank_pad * 2;
     p.rank = a->rank;
     p.scale = a->scale;
-    p.slot = slot;
-    p.x = x;
-    p.base = base;
-    p.out = out;
     p.ldx = ldx;
     p.slots = a->slots;
     p.rows = a->rows;
@@ -572,14 +568,22 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
     p.rank_pad = a->rank_pad;
     p.cols_pad = a->cols_pad;
     p.rows_pad = a->rows_pad;
-    p.tokens = tokens;
     p.copy = base != out;
-    p.single = tokens <= 16;
-    const int groups = a->slots + 1;
-    const int tiles = p.single || tokens <= groups ? tokens : groups + (tokens - groups) / kAdTile;  // at most
     const auto launch = a->dtype == LOOM_B200_DTYPE_F32 ? a->max_rank <= 16 ? launch_adapters<2, true> : launch_adapters<4, true>
                                                         : a->max_rank <= 16 ? launch_adapters<2, false> : a->max_rank <= 32 ? launch_adapters<4, false> : launch_adapters<8, false>;
-    return launch(ctx, p, tiles);
+    // (every CTA reads all slots of its launch: 8192 tokens in one 151 us, in two 131)
+    for (int at = 0; at < tokens; at += kAdKept) {
+        p.tokens = tokens - at < kAdKept ? tokens - at : kAdKept;
+        p.slot = slot + at;
+        p.x = x + (size_t)at * ldx;
+        p.base = base ? base + (size_t)at * a->rows : nullptr;
+        p.out = out + (size_t)at * a->rows;
+        p.single = p.tokens <= 16;
+        const int groups = a->slots + 1;
+        const int tiles = p.single || p.tokens <= groups ? p.tokens : groups + (p.tokens - groups) / kAdTile;  // at most
+        if (int rc = launch(ctx, p, tiles)) return rc;
+    }
+    return 0;
 }
 
 }  // extern "C"

@@ -96,6 +96,18 @@ def test_ranks(ctx, dtype):
         s.check(rng.standard_normal((tokens, 300)).astype(np.float32), np.arange(tokens) % 9, rng.standard_normal((tokens, 90)).astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_tokens_than_a_launch_takes(ctx, dtype):
+    rng = np.random.default_rng(9)
+    a = Set(ctx, rng, 3, 13, 20, [5, 0, 17], dtype)
+    n = 2 * 4096 + 7
+    x, base = rng.standard_normal((n, 20)).astype(np.float32), rng.standard_normal((n, 13)).astype(np.float32)
+    slot = rng.integers(-1, 4, n)
+    a.check(x, slot, base, ldx=23, offset=1)
+    a.check(x, slot, base, in_place=True)
+    a.a.free()
+
+
 def test_a_slot_put_again(ctx):
     rng = np.random.default_rng(4)
     s = Set(ctx, rng, 2, 40, 50, [16, 12], cabi.DTYPE_BF16)

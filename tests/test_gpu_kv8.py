@@ -468,3 +468,44 @@ def test_frames_and_repeats():
         assert all(np.array_equal(a, b) for a, b in zip(*runs))
     finally:
         ctx.close()
+
+
+def test_portions_in_frames():
+    """A recorded call of up to 200 rows, replayed with other starts and lengths: portions, single rows, nothing; the same bits as eager calls."""
+    ctx = loom_b200.Context(0)
+    try:
+        runs = []
+        for recorded in (False, True):
+            rng = np.random.default_rng(13)
+            c = Cache(ctx, 3, 1000, 2, 64)
+            c.append(rng, [300, 0, 64])
+            c.drop()
+            q, out = c.dev(rng.standard_normal((200, 8, 64)).astype(np.float32)), c.dev(np.zeros((200, 8, 64), np.float32))
+            k = c.dev(rng.standard_normal((200, 2, 64)).astype(np.float32))
+            lengths, starts = c.dev(c.lengths()), c.dev(np.zeros(4, np.int32))
+
+            def call():
+                c.kv.append(200, lengths, k, k, starts=starts)
+                c.kv.attend(200, 8, lengths, q, out, starts=starts)
+            frame = None
+            if recorded:
+                ctx.graph_begin()
+                call()
+                frame = ctx.graph_end()
+            held, got = c.lengths(), []
+            for counts in ([150, 49, 1], [1, 1, 1], [0, 0, 0], [0, 200, 0], [13, 12, 170], [200, 0, 0]):
+                ctx.upload(lengths, held)
+                ctx.upload(starts, np.concatenate([[0], np.cumsum(counts)]).astype(np.int32))
+                for _ in range(2):  # (a step again is the same step)
+                    ctx.graph_launch(frame) if recorded else call()
+                got.append(ctx.download(out, (200, 8, 64), np.uint32))
+                held = (held + np.array(counts)).astype(np.int32)
+            ctx.sync()
+            if frame:
+                ctx.graph_free(frame)
+            runs.append(got)
+            c.drop()
+            c.kv.free()
+        assert all(np.array_equal(a, b) for a, b in zip(*runs))
+    finally:
+        ctx.close()

@@ -186,3 +186,60 @@ def test_a_serving_step(ctx):
     finally:
         cache.free()
         adapters.free()
+
+
+def test_two_contexts_at_once():
+    """Two contexts with streams of their own, every call of one beside a call of the other: each has what it has alone.  (Portions begin with a
+    block, so that a call again is the same call.)"""
+    rng = np.random.default_rng(3)
+    kv_heads, heads, dim, seqs, rows, vocab = 2, 8, 64, 4, 260, 40000
+    counts = np.array([200, 1, 59, 0])
+    host = dict(starts=np.concatenate([[0], np.cumsum(counts)]).astype(np.int32), lengths=np.array([128, 700, 0, 64], np.int32),
+                k=rng.standard_normal((rows, kv_heads * dim)).astype(np.float32), q=rng.standard_normal((rows, heads * dim)).astype(np.float32),
+                logits=(4 * rng.standard_normal((8, vocab))).astype(np.float32), u=rng.random(8, np.float32), slot=rng.integers(-1, 2, rows).astype(np.int32))
+    down, up = rng.standard_normal((9, heads * dim)).astype(np.float32), rng.standard_normal((333, 9)).astype(np.float32)
+
+    class One:
+        def __init__(self):
+            self.ctx = ctx = loom_b200.Context(0)
+            self.dev = {n: ctx.to_device(a) for n, a in host.items()}
+            self.kv, self.ad = cabi.KV8(ctx, seqs, 1000, kv_heads, dim), cabi.Adapters(ctx, 2, 333, heads * dim, 9)
+            self.ad.put(0, down, up, 0.25)
+            old = ctx.to_device(np.random.default_rng(4).standard_normal((892, kv_heads * dim)).astype(np.float32))
+            zero, starts = ctx.to_device(np.zeros(seqs, np.int32)), ctx.to_device(np.array([0, 128, 828, 828, 892], np.int32))
+            self.kv.append(892, zero, old, old, starts=starts)
+            self.att, self.out, self.tok, self.lp = (ctx.to_device(np.zeros(n, np.float32)) for n in (rows * heads * dim, rows * 333, 8, 8))
+            ctx.sync()
+            for b in (old, zero, starts):
+                ctx.free(b)
+
+        def calls(self):
+            d = self.dev
+            return [lambda: self.kv.append(rows, d["lengths"], d["k"], d["k"], starts=d["starts"]),
+                    lambda: self.kv.attend(rows, heads, d["lengths"], d["q"], self.att, starts=d["starts"]),
+                    lambda: self.ad.apply(rows, d["slot"], self.att, self.out),
+                    lambda: self.ctx.sample(8, vocab, d["logits"], d["u"], self.tok, logprob=self.lp)]
+
+        def results(self):
+            return [self.ctx.download(b, (n,), np.uint32) for b, n in ((self.att, rows * heads * dim), (self.out, rows * 333), (self.tok, 8), (self.lp, 8))]
+
+        def close(self):
+            self.ctx.sync()
+            self.kv.free()
+            self.ad.free()
+            self.ctx.close()
+    one, two = One(), One()
+    try:
+        for c in one.calls():
+            c()
+        alone = one.results()
+        for _ in range(20):
+            for c, d in zip(one.calls(), two.calls()):
+                c()
+                d()
+        for o in (one, two):
+            assert all(np.array_equal(a, b) for a, b in zip(o.results(), alone))
+            o.ctx.sync()
+    finally:
+        one.close()
+        two.close()
