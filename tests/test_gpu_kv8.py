@@ -429,6 +429,30 @@ def test_portions_of_small_and_large_values(ctx, spread):
     c.drop()
 
 
+def test_one_row_of_several_sequences(ctx):
+    """Starts that go back, so that one row is three sequences' (more blocks than the call's rows can touch where they ascend)."""
+    rng = np.random.default_rng(31)
+    c = Cache(ctx, 6, 200, 2, 32)
+    starts, lengths = c.dev(np.array([0, 1, 0, 1, 0, 1, 1], np.int32)), c.dev(np.zeros(6, np.int32))
+    row = rng.standard_normal((1, 2, 32)).astype(np.float32)
+    c.kv.append(1, lengths, c.dev(row), c.dev(row), starts=starts)
+    for s in range(0, 6, 2):
+        one = np.zeros(7, np.int32)
+        one[s + 1:] = 1
+        got = c.read(c.dev(one), lengths, 1)
+        assert np.array_equal(got[0], row) and np.array_equal(got[1], row), s
+    # a hundred rows three times: blocks that are whole, and open rows
+    k = rng.standard_normal((100, 2, 32)).astype(np.float32)
+    starts = c.dev(np.array([0, 100, 0, 100, 0, 100, 100], np.int32))
+    c.kv.append(100, lengths, c.dev(k), c.dev(-k), starts=starts)
+    for s in range(0, 6, 2):
+        one = np.zeros(7, np.int32)
+        one[s + 1:] = 100
+        got = c.read(c.dev(one), lengths, 100)
+        assert np.array_equal(got[0], kit.held(k, exact=False)) and np.array_equal(got[1], kit.held(-k, exact=False)), s
+    c.drop()
+
+
 def test_frames_and_repeats():
     """A recorded step replayed with new lengths, beside another frame of the same cache: the same bits as eager calls."""
     rng = np.random.default_rng(11)
