@@ -429,6 +429,25 @@ def test_portions_of_small_and_large_values(ctx, spread):
     c.drop()
 
 
+@pytest.mark.parametrize("n, dim", [(300, 64), (700, 32)])
+def test_hundreds_of_sequences(ctx, n, dim):
+    """Single rows, few rows and portions, over more sequences than a CTA's threads look at together."""
+    rng = np.random.default_rng(n)
+    c = Cache(ctx, n, 400, 2, dim)
+    call = c.append(rng, rng.integers(0, 130, n))
+    counts = np.where(rng.random(n) < 0.1, 0, rng.integers(1, 12, n))
+    counts[[5, n // 2, n - 1]] = 100, 40, 70
+    call = c.append(rng, counts)
+    assert call[2] > 2 * n
+    check_some(c, rng, call, counts, 16, 1)
+    c.check_rows(call, counts)
+    counts = np.ones(n, int)
+    counts[7] = 30  # few rows a sequence on the average, and many of one
+    call = c.append(rng, counts)
+    check_some(c, rng, call, counts, 16, 1)
+    c.drop()
+
+
 def test_one_row_of_several_sequences(ctx):
     """Starts that go back, so that one row is three sequences' (more blocks than the call's rows can touch where they ascend)."""
     rng = np.random.default_rng(31)

@@ -56,7 +56,7 @@ def settings(rng, rows):
                 top_p=rng.choice([1.0, 0.99, 0.9, 0.5, 0.05], rows), min_p=rng.choice([0.0, 0.0, 0.01, 0.2], rows))
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 31, 32, 33, 100, 511, 1025, 4096, 8191, 8192, 8193, 16385, 32003, 65537, 128256, 131073, 250001])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 5, 31, 32, 33, 100, 511, 1025, 4096, 8191, 8192, 8193, 16385, 32003, 65537, 128256, 131073, 250001, 655360])
 def test_sizes(ctx, vocab):
     rng = np.random.default_rng(vocab)
     rows = 12 if vocab < 50000 else 5
