@@ -15,7 +15,7 @@
 // to 6912 rows of rank 16, five adapters: 62.8 us, 0.49 of what 197 MB take at the copy's rate -- 8 us to find the tiles, 10 for down x,
 // 3 for its sums, 35 for up h and the rows of base and out at 5 TB/s.  (Asking L2 for rows of x and base some steps ahead: 64 to 69 us; tiles
 // of 64 tokens, which read the adapter less often: 60.7 us, but 28 us instead of 20 for 512 tokens.)  One token 5.0 us, sixteen tokens of as
-// many adapters, 4096 to 14336: 20.0 us.  4096 tokens of rank 64: 108 us, where the adapter's rows come from L2 for every sixteen of them.
+// many adapters, 4096 to 14336: 19.8 us.  4096 tokens of rank 64: 108 us, where the adapter's rows come from L2 for every sixteen of them.
 #include "serving.cuh"
 
 #include <cuda_bf16.h>
@@ -428,10 +428,11 @@ int launch_adapters(loom_b200_ctx* ctx, const AdapterParams& p, int tiles) {
     LB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(front + (size_t)3 * M * (kAdMaxRank + 4) * 2)));
     LB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     // As many CTAs a tile as are there at once.  Clusters of more than eight find their places in a GPC less and less well (256 tokens of
-    // two adapters: 12 CTAs a tile 13.9 us, 14 18.6 us), so those leave a quarter free; 16 of 16 fit (16 tokens: 20.9 us, with 13 26.2 us).
+    // two adapters: 12 CTAs a tile 13.9 us, 14 18.6 us), so those leave a quarter free; 14 clusters of 16 still fit (16 tokens of rank 16, 4096 to
+    // 14336: 13.9 us by 16 CTAs each, 11.6 by 12, 12.0 by 8; 14 tokens 8.5, 10.8 and 11.8 us; with sixteen warps a CTA no better).
     const int most = kAdPerSm * ctx->sm_count;
     int size = most * 7 / 8 / tiles;
-    if (size >= kAdMostCtas) size = kAdMostCtas;
+    if (size >= kAdMostCtas) size = tiles <= 14 ? kAdMostCtas : 12;
     else if (size > 8) size = most * 3 / 4 / tiles > 8 ? most * 3 / 4 / tiles : 8;
     else if (size < 4) size = most / tiles > 4 ? 4 : most / tiles > 0 ? most / tiles : 1;
     cudaLaunchConfig_t cfg = {};
