@@ -75,8 +75,8 @@ __device__ __forceinline__ int value_byte(int p, int d) { return (d >> 3) * 512 
 // A code is the float32 product where that is further than 2^-10 from a half (its error is below 2^-16) and the float64 arithmetic
 // elsewhere, one value in five hundred: conversions and float64 take sixteen values a clock of an SM.
 //
-// Bound: memory; for few rows, latencies.  About 8000 rows of eight heads of 128 in 8 sequences: append 18.5 us, read 11.8 us (81 MB
-// each way, 4.4 and 6.9 TB/s); one row of each of 64 sequences: 6.7 and 4.9 us.  A CTA for each head: with two, four and all eight heads
+// Bound: memory; for few rows, latencies.  5000 rows of eight heads of 128 in 8 sequences: append 18.5 us, read 11.8 us (52 MB
+// each way, 2.8 and 4.4 TB/s: waves of CTAs, each its loads, its largest value and its stores one behind the other); one row of each of 64 sequences: 6.7 and 4.9 us.  A CTA for each head: with two, four and all eight heads
 // a CTA the append takes 28, 38 and 66 us; runs of two to eight blocks a CTA 21 to 40 us.
 constexpr int kRowThreads = 256;
 

@@ -19,8 +19,8 @@
 // Work is a list: sequences, KV heads, tiles, parts of a tile's blocks, every CTA its place and those a grid further on.  Parts are put together
 // by twos, so that results repeat bit for bit.
 //
-// Bound: a block costs two CTAs of an SM 2.7 us, of which the tensor pipe has about 2 (S takes 94 clocks for sixteen dimensions of 64 positions: its
-// operand A, 4 KB of shared memory for so few columns).  300 rows of 20 heads over 5 of 128 dimensions at position 2900: 63 us (without these
+// Bound: a block costs two CTAs of an SM 2.7 us: weights 0.8 and 0.5, results 0.5, waiting for S 0.5 (its MMAs come 94 clocks apart, with an operand A
+// of 4 KB of shared memory for 64 columns), the tensor pipe counted as active 14 % and issue slots 33 % of the kernel.  300 rows of 20 heads over 5 of 128 dimensions at position 2900: 63 us (without these
 // tiles, on integer instructions, 93 us; with them on integer digits 89 us; with one set of warps for both kinds of work 66 us), of which 12 are the list and
 // the queries, 28 the blocks, 15 the parts' joining; 2048 rows at 8000: 755 us (1690), 2048 from the start 135 us (354).
 constexpr int kRwThreads = 256;
