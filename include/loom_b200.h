@@ -527,9 +527,10 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
  * The caller keeps the lengths: every call takes the device array lengths [sequences], the positions that each sequence holds in front of
  * this call's rows, and starts [sequences + 1]: rows starts[s] .. starts[s+1]-1 belong to sequence s and have the positions
  * lengths[s], lengths[s] + 1, ... (no rows: the sequence takes no part); rows behind starts[sequences] are left as they are.  starts NULL: one row each
- * of the first `rows` sequences, a decode step.  A sequence is cut back by giving a smaller length, not further than to the beginning of the block in
- * front of the one its last position lies in.  Rows that a sequence has no room for are not taken (attention: zeros), which loom_b200_sync
- * reports as LOOM_B200_ERR_INVALID. */
+ * of the first `rows` sequences, a decode step.  A sequence is cut back by giving a smaller length, as often as wanted.  Of the block that its last
+ * position lies in, and of the one in front of that, the float32 rows are there, and a block cut into goes on from them; cut back further, or into a block
+ * whose float32 rows an append of two blocks further on has replaced since, it goes on from that block's rows as they are held in 8 bits.  Rows that a
+ * sequence has no room for are not taken (attention: zeros), which loom_b200_sync reports as LOOM_B200_ERR_INVALID. */
 typedef struct loom_b200_kv8 loom_b200_kv8;
 int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_heads, int head_dim, loom_b200_kv8** out);
 void loom_b200_kv8_free(loom_b200_ctx* ctx, loom_b200_kv8* cache);

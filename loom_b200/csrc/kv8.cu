@@ -4,7 +4,9 @@
 // a = largest |x| of the block's 64 rows of that head, code = round(x * 127 / a) half away from zero (the arithmetic of the activation
 // quantizer: float64 quotient and product), value = code * a / 127.  A block with a value that is not finite reads as not-a-numbers.
 // The positions behind the last whole block are held in float32 as they came; of the block in front of them the float32 rows stay too, so
-// a sequence may be cut back into it and go on from there.
+// a sequence may be cut back into it and go on from there.  There are two places for such rows, for blocks of even and of odd numbers, and a
+// note of which blocks' they are: cut back further, or into a block whose place another one has taken since, a sequence goes on from that
+// block's rows as the codes have them (it was whole before another one could take its place).
 //
 // Codes lie as the tensor core's B operands want them, so that a warp's load of 16 bytes a lane is 512 consecutive bytes and needs no
 // shared memory on its way (lane = 4 g + t):
@@ -27,6 +29,7 @@ struct Kv8 {
     int seqs, max_len, heads, dim, blocks, dim_k, dim_v, dim_o;
     uint8_t *k, *v;
     float *k_top, *v_top, *k_open, *v_open;
+    int* placed;  // [seqs][heads][keys, values][2] the even and the odd block whose rows are in the open places, -1: none
     int* status;
 
     __host__ __device__ size_t head_of(int s, int h) const { return (size_t)s * heads + h; }
@@ -302,6 +305,22 @@ __device__ __forceinline__ void copy_rows(const RowParams& p, const Item& it, in
     }
 }
 
+// Rows of block b in front of position `end` from its codes into its open place, which holds another block's: the sequence was cut back to there.
+template <bool V>
+__device__ __forceinline__ void restore_rows(const Kv8& c, int s, int h, int b, int end) {
+    const int dims = V ? c.dim_v : c.dim_k, n = end - b * kKvBlock;
+    const size_t at = c.head_of(s, h) * c.blocks + b;
+    const uint8_t* codes = (V ? c.v : c.k) + at * kKvBlock * dims;
+    const float scale = __fdiv_rn((V ? c.v_top : c.k_top)[at], 127.f);
+    float* open = c.open_row(V ? c.v_open : c.k_open, s, h, b * kKvBlock);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n * c.dim; i += kRowThreads) {
+        const int r = i / c.dim, d = i - r * c.dim;
+        open[(size_t)r * c.dim_o + d] = __fmul_rn((float)(int8_t)codes[V ? value_byte(r, d) : key_byte(r, d, dims)], scale);
+    }
+    __syncthreads();
+}
+
 template <int NU>
 __global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_kernel(const RowParams p) {
     __shared__ uint32_t s_top[kRowThreads / 32];
@@ -320,13 +339,27 @@ __global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_ke
         if (it.a.count == 0) continue;
         const int end = it.a.pos + it.a.count, first = it.a.pos / kKvBlock, last = (end - 1) / kKvBlock, b = first + it.block;
         const bool keep = b >= last - 1 && (b == first || ((b - first) & 1));
-        if ((b + 1) * kKvBlock <= end) {
+        // The first block's CTA alone reads and writes the note of its head's places.
+        int* placed = p.c.placed + (p.c.head_of(it.seq, h) * 2 + kv) * 2;
+        const int there = b == first && it.a.pos % kKvBlock ? placed[first & 1] : first;
+        const bool whole = (b + 1) * kKvBlock <= end;
+        if (!whole && keep) copy_rows<true>(p, it, b, kv, h);
+        if (there >= 0 && there != first && first < p.c.blocks) {  // (a last block that is no whole one has no codes)
+            if (kv) restore_rows<true>(p.c, it.seq, h, first, it.a.pos);
+            else restore_rows<false>(p.c, it.seq, h, first, it.a.pos);
+        }
+        if (whole) {
             if (kv) append_block<NU, true>(p, it, b, h, keep, s_top);
             else append_block<NU, false>(p, it, b, h, keep, s_top);
-        } else if (keep) {
-            copy_rows<true>(p, it, b, kv, h);
         }
         if (b == first && last - first >= 2) copy_rows<true>(p, it, last - ((last - first) & 1), kv, h);  // (behind the barrier that append_block ends with)
+        if (b == first) {
+            __syncthreads();  // (everyone has read it)
+            if (threadIdx.x == 0) {
+                placed[last & 1] = last;
+                if (last > first) placed[last - 1 & 1] = last - 1;
+            }
+        }
     }
 }
 
@@ -1252,7 +1285,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
 #include "kv8_rows.cuh"
 
 Kv8 view(const loom_b200_kv8* c) {
-    return {c->seqs, c->max_len, c->heads, c->dim, c->blocks, c->dim_k, c->dim_v, c->dim_o, c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->ctx->status_dev};
+    return {c->seqs, c->max_len, c->heads, c->dim, c->blocks, c->dim_k, c->dim_v, c->dim_o, c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->placed, c->ctx->status_dev};
 }
 
 }  // namespace
@@ -1343,7 +1376,9 @@ int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_
     get((void**)&c->v_top, blocks * 4);
     get((void**)&c->k_open, open);
     get((void**)&c->v_open, open);
+    get((void**)&c->placed, (size_t)sequences * kv_heads * 4 * sizeof(int));
     get(&c->work, c->work_bytes);
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->placed, 0xff, (size_t)sequences * kv_heads * 4 * sizeof(int), ctx->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(c->work, 0, c->work_bytes, ctx->stream);
     if (e == cudaSuccess) e = cudaMemsetAsync(c->k_open, 0, open, ctx->stream);  // (what rounds a row's dimensions up stays zero)
     if (e == cudaSuccess) e = cudaMemsetAsync(c->v_open, 0, open, ctx->stream);
@@ -1361,7 +1396,7 @@ void loom_b200_kv8_free(loom_b200_ctx* ctx, loom_b200_kv8* c) {
         cudaSetDevice(ctx->device);
         cudaStreamSynchronize(ctx->stream);
     }
-    void* ptrs[] = {c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->work};
+    void* ptrs[] = {c->k, c->v, c->k_top, c->v_top, c->k_open, c->v_open, c->placed, c->work};
     for (void* p : ptrs)
         if (p) cudaFree(p);
     delete c;

@@ -13,6 +13,7 @@ struct loom_b200_kv8 {
     uint8_t *k = nullptr, *v = nullptr;      // [seqs][heads][blocks][64 * dim_k or dim_v]
     float *k_top = nullptr, *v_top = nullptr;  // [seqs][heads][blocks] largest |x|
     float *k_open = nullptr, *v_open = nullptr;  // [seqs][heads][2][64][dim_o]: rows of the open block and of the one in front, by the block's parity
+    int* placed = nullptr;        // [seqs][heads][keys, values][2] which blocks those are
     void* work = nullptr;         // partial results of attention that several CTAs share, and arrival counters (zero between launches)
     size_t work_bytes = 0;
 };
