@@ -9,7 +9,8 @@
 //            least); of those the ones with w_i >= min_p
 //   token    the first kept one, by index, whose weight and that of the kept ones in front of it exceed u times the kept weight
 // T <= 0 is the first largest logit.  Weights are integers, round(w 2^S) with S such that a whole row's sum stays below 2^62: sums do not
-// depend on their order then, and are within vocab * 2^-S of the real ones (S = 44 for 128,256 tokens: 7e-9 of the largest weight).
+// depend on their order then.  They are within vocab * 2^-S of the largest weight (S = 44 for 128,256 tokens: 7e-9) and 2^-32 of themselves of the
+// real ones, the latter from the weights beyond four temperatures.
 //
 // One cluster of CTAs per row, each with a slice of the row in shared memory, so the row is read once and by one launch.  What is kept
 // ends at a place in the order, a (logit, index) pair.  A place is found from a histogram -- of counts for top-k, of weights for
@@ -24,8 +25,10 @@
 //   whole   the same with exact weights, bins divided further by the bits of the values down to a single value, whose ties go by index: long
 //           stretches of equal or nearly equal logits, top-p next to 1
 //
-// Weights near the largest are exp2 of a double by a table of 32 entries and a polynomial (P. T. P. Tang, Table-driven implementation of the
-// exponential function, ACM TOMS 15, 1989), error 2^-48; the many others take a float32 exponential of a distance that is exact.
+// Weights are exp2 by a table and a polynomial (P. T. P. Tang, Table-driven implementation of the exponential function, ACM TOMS 15, 1989): near the
+// largest in doubles, 32 entries, error 2^-48; the many others by 512 entries of 63 bits, a float32 polynomial of what is left and one integer
+// product, of a distance that is exact.  (A float32 exponential, 2^-22 of a weight, moved the borders of 128,256 tokens of nearly equal weight by
+// thousandths of one.  64 rows of 128,256: 91 us with that, 98 so, 103 with 32 entries and what they leave in pairs of floats.)
 //
 // Bound: latencies one behind the other, 1.2 to 2 us for an exchange over the cluster; the reads are 5 of the 82 us that 64 rows of 128,256
 // take, a row of 32,000 by temperature, top-k and top-p takes 25 us.  So a row goes over as many CTAs as give 2048 logits each while there
@@ -67,6 +70,7 @@ using u64 = unsigned long long;
 
 struct __align__(16) SampleShared {  // (the slice behind it is written sixteen bytes at a time)
     double exp2_32[32];      // 2^(j/32)
+    u64 exp2_512[512];       // 2^(62 + j/512)
     u64 mass[kSpBins];       // bins of weights; running sums over this CTA's share of finer ones; with cand, values on their way to the first CTA
     u64 cand[kSpCap];        // values on their way, their weights
     union {
@@ -88,7 +92,6 @@ struct __align__(16) SampleShared {  // (the slice behind it is written sixteen 
     float wf[kSpWarps];
     unsigned wcount[kSpWarps];
     unsigned n_cand;
-    int flag;
 };
 // (declared again wherever it is used, so that the compiler knows the accesses for shared ones)
 #define LB_SAMPLE_SHARED                                       \
@@ -165,6 +168,7 @@ struct Row {
     float inv_hi, inv_lo;  // log2(e) / temperature as two floats
     float bin_scale;
     float far;     // no weight beyond it: 48 temperatures
+    float least;   // nor below this power of two: half of 2^-S
     int bits;
 
     __device__ __forceinline__ double distance(float l) const { return ((double)l - (double)top) * inv_t; }
@@ -188,8 +192,10 @@ struct Row {
         e = __hiloint2double(__double2hiint(e) + ((n >> 5) + bits) * (1 << 20), __double2loint(e));
         return __double2ull_rn(e);
     }
-    // Beyond four temperatures a float32 exponential will do: its error, 2^-21 of the value, is 2^-27 of the largest weight, and the sums
-    // that a choice hangs on are off by a few 10^-9 of it.  The distance itself is the exact difference, as two floats.
+    // Beyond four temperatures: y + z = log2 of the weight, the 512ths of y by the table, 2^r - 1 of the rest (|r| <= 2^-10) as a float32 polynomial.
+    // That is taken in 2^-32ths (the sums with 1.5 2^n have them as their low bits: no conversions): 2^-33 of the weight, and 2^-35 each from the
+    // roundings of r and of the polynomial's last two steps, 2^-32 together; what equal values share of it adds up.  The distance itself is the exact
+    // difference, as two floats.
     __device__ __forceinline__ u64 weight(float l) const {
         const float far_l = l - top;
         const float y = far_l * inv_hi;
@@ -198,13 +204,17 @@ struct Row {
             if (top == CUDART_INF_F || l == -CUDART_INF_F) return 0;
             return weight_at(distance(l));
         }
-        if (!(y > -62.f)) return 0;
+        if (!(y > least)) return 0;
         const float back = far_l - l, rest = (l - (far_l - back)) - (top + back);
         const float z = fmaf(rest, inv_hi, fmaf(far_l, inv_lo, fmaf(far_l, inv_hi, -y)));
-        const float k = y + 12582912.f;  // 1.5 2^23: its low bits are y rounded
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((y - (k - 12582912.f)) + z));
-        return __float2ull_rn(__int_as_float(__float_as_int(e) + (__float_as_int(k) - 0x4b400000 + bits) * (1 << 23)));
+        constexpr float kWhole = 24576.f, kPart = 0.0029296875f;  // 1.5 2^14 and 1.5 2^-9
+        const float k = y + kWhole, r = (y - (k - kWhole)) + z;
+        const float x = fmaf(fmaf(fmaf(0.055504109f, r, 0.24022651f), r, 0.69314718f), r, kPart);  // powers of ln 2 over factorials
+        LB_SAMPLE_SHARED;
+        const unsigned n = __float_as_uint(k);
+        const u64 t = s.exp2_512[n & 511];
+        const u64 w = t + (u64)((long long)(int)(t >> 32) * (__float_as_int(x) - 0x3b400000));  // (the table's top half will do: 2^-41 of the weight)
+        return ((w >> (61 - bits + (0x46c00000 >> 9) - (int)(n >> 9))) + 1) >> 1;  // (a shift of 62 at most, since y > least)
     }
     __device__ __forceinline__ int bin(float l) const {
         const int b = (int)((top - l) * bin_scale);  // (not a number, from equal infinities: 0)
@@ -314,7 +324,6 @@ __device__ __noinline__ Found find_bin(const Cluster c, bool mass, u64 limit, in
     if (c.rank == owner) {
         if (threadIdx.x == 0) {
             s.cand[0] = share - 1;  // (nothing reaches it: the last bin; does not happen with limits up to the total)
-            s.flag = 0;
         }
         __syncthreads();
         for (int b = threadIdx.x; b < share; b += kSpThreads) {
@@ -898,7 +907,10 @@ __global__ void __launch_bounds__(kSpThreads, 2) lb_sample_kernel(const SamplePa
     const unsigned rank = lb_cluster_rank();
     const int first = (int)rank * p.slice, n = max(0, min(p.slice, p.vocab - first));
     lb_cluster_arrive();  // (waited for in front of the first access to another CTA's memory)
-    if (tid < 32) s.exp2_32[tid] = exp2((double)tid / 32);
+    static_assert(kSpThreads == 512, "a thread for each entry");
+    const double entry = exp2((double)tid / 512);
+    s.exp2_512[tid] = __double2ull_rn(entry * 4611686018427387904.0);
+    if (tid % 16 == 0) s.exp2_32[tid / 16] = entry;
     lb_pdl_launch_dependents();
     lb_pdl_wait();
     const float* __restrict__ src = p.logits + (size_t)r * p.stride + first;
@@ -958,6 +970,7 @@ __global__ void __launch_bounds__(kSpThreads, 2) lb_sample_kernel(const SamplePa
     Row row;
     row.top = value_of_key(best_key);
     row.bits = p.bits;
+    row.least = (float)(-1 - p.bits);
     if (row.top == -CUDART_INF_F) {  // nothing to choose
         if (rank == 0 && tid == 0) {
             p.tokens[r] = -1;
