@@ -404,9 +404,24 @@ type SampleParams struct {
 	Uniform     float32 // random number in [0, 1)
 }
 
-// Sample draws the next token of sequence seq, or of every one (-1), from the logits of the last forward; logprobs may be nil.
+// wrongLength is the error of a slice that the library would read or write past its end.
+func wrongLength(who, what string, got, want int) error {
+	return &Error{int(C.LOOM_B200_ERR_INVALID), fmt.Sprintf("%s: %d %s, %d wanted", who, got, what, want)}
+}
+
+// Sample draws the next token of sequence seq, or of every one (-1), from the logits of the last forward: params has an entry for each of
+// them, and logprobs has room for as many or is nil.
 func (dec *Decoder) Sample(seq int, params []SampleParams, logprobs []float32) ([]int32, error) {
-	n := len(params)
+	n := 1
+	if seq < 0 {
+		n = int(C.loom_b200_decoder_batch(dec.d))
+	}
+	if n < 1 || len(params) != n {
+		return nil, wrongLength("Sample", "settings", len(params), n)
+	}
+	if logprobs != nil && len(logprobs) != n {
+		return nil, wrongLength("Sample", "log probabilities", len(logprobs), n)
+	}
 	temperature, topP, minP, uniform := make([]float32, n), make([]float32, n), make([]float32, n), make([]float32, n)
 	topK, tokens := make([]int32, n), make([]int32, n)
 	for i, p := range params {
@@ -433,14 +448,28 @@ func (ctx *Context) NewAdapters(slots, rows, cols, maxRank, dtype int) (*Adapter
 
 // Put fills a slot from down [rank][cols] and up [rows][rank]; rank 0 empties it.
 func (a *Adapters) Put(slot, rank int, scale float32, down, up []float32) error {
+	var rows, cols C.int
+	if err := a.ctx.check(C.loom_b200_adapters_info(a.a, nil, &rows, &cols, nil, nil)); err != nil {
+		return err
+	}
+	if rank > 0 && len(down) != rank*int(cols) {
+		return wrongLength("Put", "values of down", len(down), rank*int(cols))
+	}
+	if rank > 0 && len(up) != rank*int(rows) {
+		return wrongLength("Put", "values of up", len(up), rank*int(rows))
+	}
 	return a.ctx.check(C.loom_b200_adapters_put(a.ctx.c, a.a, C.int(slot), C.int(rank), C.float(scale), unsafe.Pointer(f32ptr(down)),
 		unsafe.Pointer(f32ptr(up)), DTypeF32, 0))
 }
 
-// Apply adds the adapters of the tokens' slots (int32 in device memory) to base; out may be base.
+// Apply adds the adapters of the tokens' slots (int32 in device memory) to base (nil: to zeros); out may be base.
 func (a *Adapters) Apply(tokens int, slot, x *Buffer, ldx int, base, out *Buffer) error {
+	var b *C.float
+	if base != nil {
+		b = (*C.float)(base.p)
+	}
 	return a.ctx.check(C.loom_b200_adapters_apply(a.ctx.c, a.a, C.int(tokens), (*C.int32_t)(slot.p), (*C.float)(x.p), C.longlong(ldx),
-		(*C.float)(base.p), (*C.float)(out.p)))
+		b, (*C.float)(out.p)))
 }
 
 func (a *Adapters) Free() {
