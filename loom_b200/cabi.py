@@ -6,6 +6,7 @@ If the shared library is missing the import of `lib()` raises: there is no fallb
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 
 import numpy as np
@@ -532,6 +533,31 @@ def to_bf16(a: np.ndarray) -> np.ndarray:
     return ((u + 0x7FFF + ((u >> 16) & 1)) >> 16).astype(np.uint16)
 
 
+def _values(a, dtype, device: int, who: str):
+    """A matrix's values for the library: (array or tensor, its type's code, whether it is on the device).  The type is the array's own; a `dtype`
+    that is given has to be that."""
+    if hasattr(a, "data_ptr"):
+        kind, on_device = str(a.dtype).rsplit(".", 1)[-1], bool(a.is_cuda)
+        if kind not in DTYPES:
+            raise ValueError("%s: a tensor of %s (float32 or bfloat16)" % (who, kind))
+        if on_device and a.device.index != device:
+            raise ValueError("%s: a tensor on device %s for a context on device %d" % (who, a.device.index, device))
+        if on_device and not a.is_contiguous():  # (a copy would be made on another stream than the library's)
+            raise ValueError("%s: a tensor with strides %s" % (who, tuple(a.stride())))
+        a, code = a.contiguous(), DTYPES[kind]
+    else:
+        a, on_device = np.ascontiguousarray(a), False
+        if a.dtype == np.uint16:
+            code = DTYPE_BF16
+        elif a.dtype.kind == "f":
+            a, code = a.astype(np.float32, copy=False), DTYPE_F32
+        else:
+            raise ValueError("%s: an array of %s (floats, or uint16 bit patterns of bfloat16)" % (who, a.dtype))
+    if dtype is not None and dtype != code:
+        raise ValueError("%s: dtype %s for values of dtype %s" % (who, dtype, code))
+    return a, code, on_device
+
+
 class Matrix:
     """bf16 or float32 matrices of one shape (`groups` of them) in the library's blocked layout."""
 
@@ -542,13 +568,13 @@ class Matrix:
         ctx._check(lib().loom_b200_matrix_create(ctx.h, rows, cols, groups, dtype, C.byref(h)))
         self.h = h
 
-    def put(self, src, dtype: int = DTYPE_F32, row0: int = 0, group: int = 0, rows: int | None = None):
-        """Rows row0 ... of a group from a host array (float32, or uint16 bit patterns with DTYPE_BF16) or a device tensor."""
-        on_device = hasattr(src, "data_ptr")
-        if not on_device:
-            src = np.ascontiguousarray(src)
+    def put(self, src, dtype: int | None = None, row0: int = 0, group: int = 0, rows: int | None = None):
+        """Rows row0 ... of a group from an array (floats, or uint16 bit patterns of bfloat16) or a tensor, on the device written before this call."""
+        src, code, on_device = _values(src, dtype, self.ctx.device, "Matrix.put")
         n = rows if rows is not None else src.shape[0]
-        self.ctx._check(lib().loom_b200_matrix_put(self.ctx.h, self.h, group, row0, n, _ptr(src), dtype, 1 if on_device else 0))
+        if math.prod(src.shape) < n * self.cols:
+            raise ValueError("Matrix.put: %d rows of %d out of %s" % (n, self.cols, tuple(src.shape)))
+        self.ctx._check(lib().loom_b200_matrix_put(self.ctx.h, self.h, group, row0, n, _ptr(src), code, 1 if on_device else 0))
         return self
 
     def free(self):
@@ -573,15 +599,21 @@ class Adapters:
         ctx._check(lib().loom_b200_adapters_create(ctx.h, slots, rows, cols, max_rank, dtype, C.byref(h)))
         self.h = h
 
-    def put(self, slot: int, down, up, scale: float = 1.0, dtype: int = DTYPE_F32):
-        """down [rank, cols] and up [rows, rank]: host arrays (float32, or uint16 bit patterns with DTYPE_BF16) or device tensors; None
-        for both empties the slot."""
-        rank, on_device = 0 if down is None else down.shape[0], hasattr(down, "data_ptr")
-        if rank and not on_device:
-            down, up = np.ascontiguousarray(down), np.ascontiguousarray(up)
-        if rank and (tuple(down.shape) != (rank, self.cols) or tuple(up.shape) != (self.rows, rank)):
-            raise ValueError("adapter of %s and %s for a matrix %dx%d" % (tuple(down.shape), tuple(up.shape), self.rows, self.cols))
-        self.ctx._check(lib().loom_b200_adapters_put(self.ctx.h, self.h, slot, rank, float(scale), _ptr(down), _ptr(up), dtype, 1 if on_device else 0))
+    def put(self, slot: int, down, up, scale: float = 1.0, dtype: int | None = None):
+        """down [rank, cols] and up [rows, rank], both of one type and in one place: arrays (floats, or uint16 bit patterns of bfloat16) or tensors, on the
+        device written before this call; None for both, or a rank of 0, empties the slot."""
+        if (down is None) != (up is None):
+            raise ValueError("Adapters.put: one matrix of two")
+        rank, code, on_device = 0 if down is None else down.shape[0], DTYPE_F32, False
+        if rank:
+            down, code, on_device = _values(down, dtype, self.ctx.device, "Adapters.put")
+            up, of_up, there = _values(up, dtype, self.ctx.device, "Adapters.put")
+            if (of_up, there) != (code, on_device):
+                raise ValueError("Adapters.put: matrices of two types, or in two places")
+            if tuple(down.shape) != (rank, self.cols) or tuple(up.shape) != (self.rows, rank):
+                raise ValueError("adapter of %s and %s for a matrix %dx%d" % (tuple(down.shape), tuple(up.shape), self.rows, self.cols))
+        self.ctx._check(lib().loom_b200_adapters_put(self.ctx.h, self.h, slot, rank, float(scale), _ptr(down) if rank else None, _ptr(up) if rank else None, code,
+                                                     1 if on_device else 0))
 
     def apply(self, tokens, slot, x, out, base=None, ldx=None):
         """out[t] = base[t] + scale up (down x[t]) with the adapter in slot[t] (device buffers; base may be out)."""
