@@ -498,8 +498,9 @@ int loom_b200_decoder_extend(loom_b200_decoder* dec, const int32_t* tokens, int 
 int loom_b200_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logits, long long stride, const float* temperature,
                      const int32_t* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* tokens, float* logprob);
 
-/* The same for a decoder, from the logits that its last forward left on the device: of one sequence (seq), or of every one (seq -1; all need a
- * prompt behind them).  Host arrays, one entry for each of them; the tokens are the caller's to feed to the next forward, extend or step_batch. */
+/* The same for a decoder, from the logits that its last forward left on the device: of one sequence (seq), or of every one (seq -1).  Each needs
+ * a forward that ended at the position it is at: one that has been cut back or uploaded since is refused (LOOM_B200_ERR_INVALID).  Host
+ * arrays, one entry for each of them; the tokens are the caller's to feed to the next forward, extend or step_batch. */
 int loom_b200_decoder_sample(loom_b200_decoder* dec, int seq, const float* temperature, const int32_t* top_k, const float* top_p,
                              const float* min_p, const float* uniform, int32_t* tokens, float* logprob);
 

@@ -77,6 +77,7 @@ struct loom_b200_decoder {
     float* logits_all = nullptr;
     int* cur_tok = nullptr;             // the current token of the selected lane (tok when there is one sequence)
     std::vector<int> kv_offsets;        // host mirror of every lane's position
+    std::vector<int> logits_at;         // the position behind which every lane's row of logits stands, -1: none
     int* h_tok_all = nullptr;           // pinned [batch]
     cudaEvent_t read_done[kReadEvents] = {};  // pieces of a logits row on their way to the host; passes of several sequences
     cudaStream_t read_stream = nullptr;  // several sequences: a pass's logits cross the bus beside the next pass
@@ -716,6 +717,7 @@ int dec_extend(loom_b200_decoder* dec, const int32_t* tokens, int n, const int32
     loom_b200_ctx* ctx = dec->ctx;
     const size_t V = (size_t)dec->d.vocab;
     LB_REQUIRE(ctx, dec->kv_offset + n <= dec->d.max_seq_len, "decoder_forward: %d positions exceed MaxSeqLen %d", dec->kv_offset + n, dec->d.max_seq_len);
+    dec->logits_at[dec->lane] = -1;
     const bool want_last = n_want > 0 && want[n_want - 1] == n - 1;
     if (dec->stack && n > 1) {
         const int cap = std::min(n, kStackBlock);
@@ -730,7 +732,7 @@ int dec_extend(loom_b200_decoder* dec, const int32_t* tokens, int n, const int32
             if (int rc = dec_stack_block(dec, M, dec->kv_offset + s0, s0 + M == n, local.data() + w, w1 - w, logits_host ? logits_host + (size_t)w * V : nullptr)) return rc;
             w = w1;
         }
-        dec->kv_offset += n;
+        dec->logits_at[dec->lane] = dec->kv_offset += n;
         return 0;
     }
     if (n == 1) {
@@ -761,7 +763,7 @@ int dec_extend(loom_b200_decoder* dec, const int32_t* tokens, int n, const int32
         if (int rc = dec_gather_logits(dec, dec->logits)) return rc;
         if (int rc = dec_read_logits(dec, logits_host + (size_t)(n_want - 1) * V)) return rc;
     }
-    dec->kv_offset += n;
+    dec->logits_at[dec->lane] = dec->kv_offset += n;
     return 0;
 }
 
@@ -789,6 +791,7 @@ static int dec_finish_create(loom_b200_decoder* dec, loom_b200_decoder** out) {
     A((void**)&dec->tok_all, sizeof(int));
     A((void**)&dec->out_tokens_all, (size_t)dec->out_cap * sizeof(int));
     dec->kv_offsets.assign(1, 0);
+    dec->logits_at.assign(1, -1);
     dec_point_at_lane(dec, 0);
     if (dec->tp_world > 1) {
         A((void**)&dec->tp_stats, 2 * kChunkTokens * sizeof(double));
@@ -1049,6 +1052,7 @@ int loom_b200_decoder_reset(loom_b200_decoder* dec) {
     if (ctx->capturing) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "decoder_reset cannot be recorded");
     if (int rc = lb_set_device(ctx)) return rc;
     dec->kv_offset = 0;
+    dec->logits_at[dec->lane] = -1;
     LB_CUDA(ctx, cudaMemsetAsync(dec->pos, 0, sizeof(int), ctx->stream));
     LB_CUDA(ctx, cudaMemsetAsync(dec->step, 0, sizeof(int), ctx->stream));
     return 0;
@@ -1107,12 +1111,14 @@ int loom_b200_decoder_continue(loom_b200_decoder* dec, int steps) {
     LB_REQUIRE(ctx, dec->kv_offset + steps <= dec->d.max_seq_len, "decoder_continue: %d positions exceed MaxSeqLen %d", dec->kv_offset + steps, dec->d.max_seq_len);
     if (ctx->capturing) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "decoder_continue cannot be recorded");
     if (int rc = lb_set_device(ctx)) return rc;
+    if (steps == 0) return 0;
+    dec->logits_at[dec->lane] = -1;
     for (int i = 0; i < steps; ++i) {
         if (!dec->fused_tail)
             if (int rc = lb_launch_argmax_advance(ctx, dec->logits, dec->d.vocab, dec->tok, dec->out_tokens, dec->out_cap, dec->step, nullptr)) return rc;
         if (int rc = dec_step(dec, false)) return rc;
     }
-    dec->kv_offset += steps;
+    dec->logits_at[dec->lane] = dec->kv_offset += steps;
     return 0;
 }
 
@@ -1159,6 +1165,7 @@ int loom_b200_decoder_set_batch(loom_b200_decoder* dec, int batch) {
     if (e != cudaSuccess) return lb_fail(ctx, LOOM_B200_ERR_CUDA, "decoder_set_batch: %s", cudaGetErrorString(e));
     dec->batch = batch;
     dec->kv_offsets.assign(B, 0);
+    dec->logits_at.assign(B, -1);
     dec_drop_graph(dec);
     dec_point_at_lane(dec, 0);
     return 0;
@@ -1218,9 +1225,10 @@ int loom_b200_decoder_step_batch(loom_b200_decoder* dec, const int32_t* tokens, 
         return 0;
     };
     const int per = dec_pass_lanes(dec);
+    dec->logits_at.assign(B, -1);
     for (int l0 = 0; l0 < B; l0 += per)
         if (int rc = beside ? dec_forward_lanes(dec, l0, std::min(per, B - l0), rows_done) : dec_forward_lanes(dec, l0, std::min(per, B - l0))) return rc;
-    for (int i = 0; i < B; ++i) dec->kv_offsets[i] += 1;
+    for (int i = 0; i < B; ++i) dec->logits_at[i] = dec->kv_offsets[i] += 1;
     dec->kv_offset = dec->kv_offsets[dec->lane];
     if (beside) {
         const size_t row = (size_t)dec->d.vocab * 4;
@@ -1256,8 +1264,11 @@ int loom_b200_decoder_sample(loom_b200_decoder* dec, int seq, const float* tempe
     LB_REQUIRE(ctx, uniform && tokens, "decoder_sample: NULL buffer");
     if (ctx->capturing) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "decoder_sample takes host buffers and cannot be recorded");
     const int first = seq < 0 ? 0 : seq, n = seq < 0 ? dec->batch : 1;
-    for (int i = first; i < first + n; ++i)
-        LB_REQUIRE(ctx, (i == dec->lane ? dec->kv_offset : dec->kv_offsets[i]) > 0, "decoder_sample: sequence %d has no prompt behind it", i);
+    for (int i = first; i < first + n; ++i) {
+        const int at = i == dec->lane ? dec->kv_offset : dec->kv_offsets[i];
+        LB_REQUIRE(ctx, at > 0, "decoder_sample: sequence %d has no prompt behind it", i);
+        LB_REQUIRE(ctx, dec->logits_at[i] == at, "decoder_sample: sequence %d has no logits of its position %d (cut back, uploaded or not forwarded to it): forward a token first", i, at);
+    }
     if (int rc = lb_set_device(ctx)) return rc;
     if (n > dec->draw_cap) {
         if (dec->draw) cudaFree(dec->draw);
@@ -1294,11 +1305,13 @@ int loom_b200_decoder_continue_batch(loom_b200_decoder* dec, int steps) {
     if (int rc = lb_set_device(ctx)) return rc;
     if (int rc = dec_batch_ready(dec, steps, "decoder_continue_batch")) return rc;
     const int B = dec->batch;
+    if (steps == 0) return 0;
     const int per = dec_pass_lanes(dec);
+    dec->logits_at.assign(B, -1);
     for (int s = 0; s < steps; ++s)
         for (int l0 = 0; l0 < B; l0 += per)
             if (int rc = dec_forward_lanes(dec, l0, std::min(per, B - l0))) return rc;
-    for (int i = 0; i < B; ++i) dec->kv_offsets[i] += steps;
+    for (int i = 0; i < B; ++i) dec->logits_at[i] = dec->kv_offsets[i] += steps;
     dec->kv_offset = dec->kv_offsets[dec->lane];
     return 0;
 }
@@ -1384,6 +1397,7 @@ int loom_b200_decoder_upload_cache(loom_b200_decoder* dec, int block, int kv_off
         }
     }
     dec->kv_offset = kv_offset;
+    dec->logits_at[dec->lane] = -1;
     LB_CUDA(ctx, cudaMemcpy(dec->pos, &kv_offset, sizeof(int), cudaMemcpyHostToDevice));
     return 0;
 }
@@ -1413,6 +1427,7 @@ int loom_b200_decoder_generate(loom_b200_decoder* dec, const int32_t* prompt, in
     if (int rc = dec_check_ready(dec)) return rc;
     using clk = std::chrono::steady_clock;
     dec->kv_offset = 0;  // Generate starts with Transformer.Reset
+    dec->logits_at[dec->lane] = -1;
     auto t0 = clk::now();
     // prefill: a one-token prompt still starts a fresh sequence
     if (n_prompt == 1) {
@@ -1445,7 +1460,7 @@ int loom_b200_decoder_generate(loom_b200_decoder* dec, const int32_t* prompt, in
     cudaEventElapsedTime(&ms, e0, e1);
     cudaEventDestroy(e0);
     cudaEventDestroy(e1);
-    dec->kv_offset += max_new;
+    dec->logits_at[dec->lane] = dec->kv_offset += max_new;
     if (metrics) {
         metrics->prefill_seconds = std::chrono::duration<double>(t1 - t0).count();
         metrics->decode_seconds = std::chrono::duration<double>(t2 - t1).count();
