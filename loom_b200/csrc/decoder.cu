@@ -69,6 +69,7 @@ struct loom_b200_decoder {
     // appends it to the output ring, advances the position and gathers the next embedding row, so a step is
     // {blocks, head} and needs no argmax, position or embedding launch
     bool fused_tail = false;
+    int x_lane = -1;  // the sequence of which x holds that row, -1: of none
     // independent sequences ("lanes"): `batch` KV rings per block and one position, current token, output ring and logits
     // row per sequence.  The single-sequence calls act on the selected lane: pos, step, out_tokens, logits and cur_tok
     // point into the arrays below at that lane.
@@ -717,7 +718,7 @@ int dec_extend(loom_b200_decoder* dec, const int32_t* tokens, int n, const int32
     loom_b200_ctx* ctx = dec->ctx;
     const size_t V = (size_t)dec->d.vocab;
     LB_REQUIRE(ctx, dec->kv_offset + n <= dec->d.max_seq_len, "decoder_forward: %d positions exceed MaxSeqLen %d", dec->kv_offset + n, dec->d.max_seq_len);
-    dec->logits_at[dec->lane] = -1;
+    dec->logits_at[dec->lane] = dec->x_lane = -1;
     const bool want_last = n_want > 0 && want[n_want - 1] == n - 1;
     if (dec->stack && n > 1) {
         const int cap = std::min(n, kStackBlock);
@@ -764,6 +765,7 @@ int dec_extend(loom_b200_decoder* dec, const int32_t* tokens, int n, const int32
         if (int rc = dec_read_logits(dec, logits_host + (size_t)(n_want - 1) * V)) return rc;
     }
     dec->logits_at[dec->lane] = dec->kv_offset += n;
+    dec->x_lane = dec->lane;
     return 0;
 }
 
@@ -1018,6 +1020,7 @@ int loom_b200_decoder_set_embeddings(loom_b200_decoder* dec, const float* emb_de
     if (int rc = lb_set_device(ctx)) return rc;
     dec_drop_graph(dec);
     dec->emb = emb_dev;
+    dec->x_lane = -1;
     dec->fused_tail = dec_tail_possible(dec, emb_dev);
     const int H = dec->d.hidden;
     std::vector<float> ones(H, 1.0f);
@@ -1041,6 +1044,7 @@ int loom_b200_decoder_set_lm_head_ternary(loom_b200_decoder* dec, const loom_b20
     }
     dec_drop_graph(dec);
     dec->head_tern = head;
+    dec->x_lane = -1;
     // the greedy step folded into the fp32 head's tail does not exist for this head: argmax, position and embedding are launches again
     dec->fused_tail = head == nullptr && dec_tail_possible(dec, dec->emb);
     return 0;
@@ -1113,12 +1117,16 @@ int loom_b200_decoder_continue(loom_b200_decoder* dec, int steps) {
     if (int rc = lb_set_device(ctx)) return rc;
     if (steps == 0) return 0;
     dec->logits_at[dec->lane] = -1;
+    if (dec->fused_tail && !dec->stack && dec->x_lane != dec->lane)  // another sequence's pass, or several sequences', came between
+        if (int rc = lb_launch_embed(ctx, dec->emb, dec->d.vocab, dec->d.hidden, dec->cur_tok, 1, dec->x)) return rc;
+    dec->x_lane = -1;
     for (int i = 0; i < steps; ++i) {
         if (!dec->fused_tail)
             if (int rc = lb_launch_argmax_advance(ctx, dec->logits, dec->d.vocab, dec->tok, dec->out_tokens, dec->out_cap, dec->step, nullptr)) return rc;
         if (int rc = dec_step(dec, false)) return rc;
     }
     dec->logits_at[dec->lane] = dec->kv_offset += steps;
+    dec->x_lane = dec->lane;
     return 0;
 }
 
@@ -1166,6 +1174,7 @@ int loom_b200_decoder_set_batch(loom_b200_decoder* dec, int batch) {
     dec->batch = batch;
     dec->kv_offsets.assign(B, 0);
     dec->logits_at.assign(B, -1);
+    dec->x_lane = -1;
     dec_drop_graph(dec);
     dec_point_at_lane(dec, 0);
     return 0;
@@ -1226,6 +1235,7 @@ int loom_b200_decoder_step_batch(loom_b200_decoder* dec, const int32_t* tokens, 
     };
     const int per = dec_pass_lanes(dec);
     dec->logits_at.assign(B, -1);
+    dec->x_lane = -1;
     for (int l0 = 0; l0 < B; l0 += per)
         if (int rc = beside ? dec_forward_lanes(dec, l0, std::min(per, B - l0), rows_done) : dec_forward_lanes(dec, l0, std::min(per, B - l0))) return rc;
     for (int i = 0; i < B; ++i) dec->logits_at[i] = dec->kv_offsets[i] += 1;
@@ -1308,6 +1318,7 @@ int loom_b200_decoder_continue_batch(loom_b200_decoder* dec, int steps) {
     if (steps == 0) return 0;
     const int per = dec_pass_lanes(dec);
     dec->logits_at.assign(B, -1);
+    dec->x_lane = -1;
     for (int s = 0; s < steps; ++s)
         for (int l0 = 0; l0 < B; l0 += per)
             if (int rc = dec_forward_lanes(dec, l0, std::min(per, B - l0))) return rc;
@@ -1356,6 +1367,7 @@ int loom_b200_decoder_linears_frame(loom_b200_decoder* dec) {
     if (int rc = dec_check_ready(dec)) return rc;
     LB_REQUIRE(ctx, dec->tp_world == 1, "decoder_linears_frame: not available under a tensor-parallel group");
     if (int rc = lb_set_device(ctx)) return rc;
+    dec->x_lane = -1;
     return dec_forward_chunk(dec, 1, dec->decode_splits, false, 0, true);
 }
 
@@ -1427,7 +1439,7 @@ int loom_b200_decoder_generate(loom_b200_decoder* dec, const int32_t* prompt, in
     if (int rc = dec_check_ready(dec)) return rc;
     using clk = std::chrono::steady_clock;
     dec->kv_offset = 0;  // Generate starts with Transformer.Reset
-    dec->logits_at[dec->lane] = -1;
+    dec->logits_at[dec->lane] = dec->x_lane = -1;
     auto t0 = clk::now();
     // prefill: a one-token prompt still starts a fresh sequence
     if (n_prompt == 1) {
@@ -1461,6 +1473,7 @@ int loom_b200_decoder_generate(loom_b200_decoder* dec, const int32_t* prompt, in
     cudaEventDestroy(e0);
     cudaEventDestroy(e1);
     dec->logits_at[dec->lane] = dec->kv_offset += max_new;
+    dec->x_lane = dec->lane;
     if (metrics) {
         metrics->prefill_seconds = std::chrono::duration<double>(t1 - t0).count();
         metrics->decode_seconds = std::chrono::duration<double>(t2 - t1).count();
