@@ -35,7 +35,7 @@ constexpr int kRwFixed = 4;     // what a part costs beside its blocks, in block
 constexpr int kRwLevel = 2;
 constexpr int kRwLeast = 4;     // blocks of a part, at least (13 rows of 4 heads at 2900: 43 us; with 3 the same, with 6 45 us, with 13 55 us)
 constexpr float kRwWeight = 16384.f;
-constexpr float kRwLag = 20.f;  // a row's results are scaled anew where a block's largest score is so far above theirs, as a power of two
+constexpr float kRwLag = 8.f;  // a row's results are scaled anew where a block's largest score is so far above theirs, as a power of two (by as much may they overflow sooner)
 
 template <int NK>
 struct RowsShape {
@@ -626,7 +626,9 @@ __global__ void __launch_bounds__(kRwThreads, 2) lb_kv8_rows_kernel(const Attend
                     most_y = fmaxf(most_y, sc[i]);
                     odd += sc[i] * 0.f;  // (not a number, from one)
                 }
-                const float inv = most_y > 1e-33f ? __fdiv_rn(kRwWeight, most_y) : 0.f;
+                // (from 2^-112 down the weights get smaller with the values: a larger factor would overflow)
+                most_y = fmaxf(most_y, 0x1p-112f);
+                const float inv = __fdiv_rn(kRwWeight, most_y);
 #pragma unroll
                 for (int i = 0; i < kKvBlock; ++i) sc[i] *= inv;
                 put_weights(0);
