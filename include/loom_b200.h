@@ -521,7 +521,7 @@ void loom_b200_adapters_free(loom_b200_ctx* ctx, loom_b200_adapters* a);
 int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, int tokens, const int32_t* slot, const float* x, long long ldx,
                              const float* base, float* out);
 
-/* A cache of keys and values in 8 bits for `sequences` sequences of up to max_len positions, head_dim <= 256.  Positions go by blocks of
+/* A cache of keys and values in 8 bits for `sequences` (<= 4096) sequences of up to max_len (<= 2^29) positions, head_dim <= 256.  Positions go by blocks of
  * 64: a whole block is held as int8 codes with one scale for each KV head, for keys and for values (largest |x| / 127; codes rounded half
  * away from zero, as loom_b200_quantize_activation does); the positions behind a sequence's last whole block are held as they came.  A
  * block with a value that is not finite reads as not-a-numbers.

@@ -115,6 +115,7 @@ int lb_status_result(loom_b200_ctx* ctx) {
     *ctx->status_host = 0;
     LB_CUDA(ctx, cudaMemsetAsync(ctx->status_dev, 0, sizeof(int), ctx->stream));
     if (code == 7) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "rows for positions that an 8-bit cache does not have; they were not taken");
+    if (code == 8) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "attention over an 8-bit cache with more work than a call takes: sequences that share rows; it was not done");
     static const char* what[] = {"", "a shared-memory tile copy did not complete", "",
                                  "the tensor-core pipeline of the GEMM stalled", "", "a tensor-parallel peer did not answer",
                                  "self-test: a flag that nothing sets"};

@@ -465,6 +465,11 @@ constexpr int kAtOpenFew = 6;     // what an open block costs, in blocks: beside
 constexpr int kAtOpenWide = 3;    // and beside a wide tile's
 constexpr int kAtOpenRows = 16;   // rows that go through the open block together
 
+// Work is counted in 31 bits; a call with more than they hold (sequences that share rows, as no others can) is not done at all.
+constexpr double kAtMostWork = 2147483648.0 - 1024;
+constexpr int kAtTooMuch = 8;  // the status then
+__device__ __forceinline__ unsigned add_work(unsigned a, unsigned b) { return a + min(b, ~a); }
+
 struct AttendParams {
     Kv8 c;
     int rows, q_heads, group, ctas;
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
                 if (q.work) v += c.heads * q.tiles * ((((unsigned)q.load << q.cost) + size - 1) / size);
                 continue;
             }
-            v += q.work;
+            v = add_work(v, q.work);
             if (q.work == 0 && q.a.count > 0 && me == 0 && my_size == 0 && !fits(c, q.a)) {
                 atomicExch(c.status, 7);
 #pragma unroll 1
@@ -631,13 +636,17 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
             }
         }
 #pragma unroll
-        for (int o = kAtSizes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int o = kAtSizes; o < 32; o <<= 1) v = add_work(v, __shfl_xor_sync(0xffffffffu, v, o));
         __syncthreads();
         if (lane < kAtSizes) s_scan[warp][lane] = v;
         __syncthreads();
-        v = s_scan[0][my_size] + s_scan[1][my_size] + s_scan[2][my_size] + s_scan[3][my_size];
+        v = add_work(add_work(s_scan[0][my_size], s_scan[1][my_size]), add_work(s_scan[2][my_size], s_scan[3][my_size]));
         if (pass == 0) {
             total = v;
+            if (total >> 31) {
+                if (me == 0 && tid == 0) atomicExch(c.status, kAtTooMuch);
+                return;
+            }
             share = total / p.ctas + 1;
             size = max((unsigned)kAtWarps, share + (unsigned)((unsigned long long)share * my_size / kAtSizes));
         } else {
@@ -1339,6 +1348,7 @@ static int launch_rows(loom_b200_ctx* ctx, AttendParams p) {
 }
 
 constexpr int kKvMaxSeqs = 4096;
+constexpr int kKvMaxLen = 1 << 29;  // (a tile's load times its parts, of which there are no more than CTAs, in 32 bits)
 
 extern "C" {
 
@@ -1347,8 +1357,8 @@ int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_
     LB_REQUIRE(ctx, out != nullptr, "kv8_create: out is NULL");
     *out = nullptr;
     LB_REQUIRE(ctx, sequences > 0 && max_len > 0 && kv_heads > 0 && head_dim > 0, "kv8_create: %d sequences of %d positions, %d KV heads of %d", sequences, max_len, kv_heads, head_dim);
-    if (sequences > kKvMaxSeqs || kv_heads > 65535 || head_dim > 256 || max_len > (1 << 30))
-        return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_create: %d sequences (%d at most), %d positions, %d KV heads of %d (256 at most)", sequences, kKvMaxSeqs, max_len, kv_heads, head_dim);
+    if (sequences > kKvMaxSeqs || kv_heads > 65535 || head_dim > 256 || max_len > kKvMaxLen)
+        return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_create: %d sequences (%d at most), %d positions (%d at most), %d KV heads of %d (256 at most)", sequences, kKvMaxSeqs, max_len, kKvMaxLen, kv_heads, head_dim);
     if (ctx->capturing) return lb_fail(ctx, LOOM_B200_ERR_INVALID, "kv8_create cannot be recorded");
     if (int rc = lb_set_device(ctx)) return rc;
     auto* c = new loom_b200_kv8();
@@ -1456,9 +1466,12 @@ int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, int hea
     LB_REQUIRE(ctx, (long long)rows * p.group < (1 << 30), "kv8_attend: %d rows of %d heads", rows, heads);
     if (p.group > 32768) return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_attend: %d query heads a KV head, 32768 at most", p.group);
     p.group_inv = p.group > 1 ? (unsigned)((4294967296ull + p.group - 1) / p.group) : 0u;
-    // the list of work is counted in 32 bits: blocks of tiles of eight rows, as if every sequence were full
-    if ((double)c->heads * (c->blocks + 1) * ((double)rows * p.group / 8 + 8.0 * c->seqs) >= 4294967296.0)
+    // the list of work is counted in 31 bits: blocks of tiles of eight rows, as if every sequence were full and had an open block
+    if ((double)c->heads * (c->blocks + 1 + kAtOpenFew) * ((double)rows * p.group / 8 + 8.0 * c->seqs) >= kAtMostWork)
         return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_attend: %d rows of %d heads over sequences of up to %d positions: fewer rows a call", rows, heads, c->max_len);
+    // and so are a portion's tiles, should every sequence have every row
+    if ((double)c->heads * c->seqs * ((double)rows * p.group / kRwTile + 1) >= kAtMostWork)
+        return lb_fail(ctx, LOOM_B200_ERR_UNSUPPORTED, "kv8_attend: %d rows of %d heads for %d sequences: fewer rows a call", rows, heads, c->seqs);
     if (int rc = lb_set_device(ctx)) return rc;
     p.starts = starts;
     p.lengths = lengths;

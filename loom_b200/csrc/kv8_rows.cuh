@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(kRwThreads, 2) lb_kv8_rows_kernel(const Attend
         lb_mbar_init(&s_bar[3], kRwHalf / 32);
         lb_fence_mbar_init();
     }
-    // blocks of a part: the size of those tried for which rounds of parts times their length is least
+    // blocks of a part: the size of those tried for which rounds of parts times their length is least (more work than 32 bits hold, by sequences that
+    // share rows, gives a share beyond every sequence's blocks: parts are tiles then, which 31 bits do hold)
     const int my_size = lane % kRwSizes;
     unsigned size = 0, most = 0, parts = 0;
 #pragma unroll 1
@@ -167,11 +168,11 @@ __global__ void __launch_bounds__(kRwThreads, 2) lb_kv8_rows_kernel(const Attend
 #pragma unroll 1
         for (int i = warp * (32 / kRwSizes) + lane / kRwSizes; i < c.seqs; i += kRwThreads / kRwSizes) {
             const Seq q = seq_of(i);
-            v += c.heads * q.tiles * (pass == 0 ? (unsigned)q.blocks : (q.blocks + size - 1) / size);
+            v = add_work(v, c.heads * q.tiles * (pass == 0 ? (unsigned)q.blocks : (q.blocks + size - 1) / size));
             longest = max(longest, (unsigned)q.blocks);
         }
 #pragma unroll
-        for (int o = kRwSizes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int o = kRwSizes; o < 32; o <<= 1) v = add_work(v, __shfl_xor_sync(0xffffffffu, v, o));
         longest = __reduce_max_sync(0xffffffffu, longest);
         __syncthreads();
         if (lane < kRwSizes) s_scan[warp][lane] = v;
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(kRwThreads, 2) lb_kv8_rows_kernel(const Attend
         __syncthreads();
         v = 0;
 #pragma unroll
-        for (int w = 0; w < kRwWarps; ++w) v += s_scan[w][my_size];
+        for (int w = 0; w < kRwWarps; ++w) v = add_work(v, s_scan[w][my_size]);
         if (pass == 0) {
 #pragma unroll
             for (int w = 0; w < kRwWarps; ++w) most = max(most, s_most[w]);
