@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
     __shared__ float s_f[2][kAtOpenRows];            // factors of a row's piece and of its open block
     __shared__ int s_span[kAtThreads][3];            // the first sequences' rows
     __shared__ unsigned s_scan[kAtWarps][kAtSizes], s_at;
-    __shared__ int s_seq, s_last;
+    __shared__ int s_seq, s_last, s_misfit;
     __shared__ __align__(8) uint64_t s_bar;  // copies of parts
     uint32_t bar_phase = 0;
     const Kv8& c = p.c;
@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
     if (tid == 0) {
         lb_mbar_init(&s_bar, 1);
         lb_fence_mbar_init();
+        s_misfit = 0;
     }
     for (int i = tid; i < min(c.seqs, kAtThreads); i += kAtThreads) {
         const Span a = span_of(p.starts, p.lengths, p.rows, i);
@@ -629,11 +630,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
                 continue;
             }
             v = add_work(v, q.work);
-            if (q.work == 0 && q.a.count > 0 && me == 0 && my_size == 0 && !fits(c, q.a)) {
-                atomicExch(c.status, 7);
-#pragma unroll 1
-                for (long long j = 0; j < (long long)q.a.count * p.q_heads * hd; ++j) p.out[(size_t)q.a.row * p.q_heads * hd + j] = 0.f;
-            }
+            if (q.work == 0 && q.a.count > 0 && !fits(c, q.a)) s_misfit = 1;
         }
 #pragma unroll
         for (int o = kAtSizes; o < 32; o <<= 1) v = add_work(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -654,6 +651,18 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
             each = fits_in != 0;
             size = __shfl_sync(0xffffffffu, size, each ? __ffs(fits_in) - 1 : 0);
             if (!each) size = (share + 7) / 8 * 8;  // (parts of a cut tile are half of it at least, which their places in p.part go by)
+        }
+    }
+    if (s_misfit) {  // rows that have no room: zeros, by all CTAs
+        if (me == 0 && tid == 0) atomicExch(c.status, 7);
+#pragma unroll 1
+        for (int i = 0; i < c.seqs; ++i) {
+            const Span a = span_of(p.starts, p.lengths, p.rows, i);
+            if (fits(c, a)) continue;
+            const size_t n = (size_t)a.count * p.q_heads * hd;
+            float* to = p.out + (size_t)a.row * p.q_heads * hd;
+#pragma unroll 1
+            for (size_t j = (size_t)me * kAtThreads + tid; j < n; j += (size_t)p.ctas * kAtThreads) to[j] = 0.f;
         }
     }
     const auto parts_of = [&](const Seq& q) { return (int)((((unsigned)q.load << q.cost) + size - 1) / size); };  // of a tile
