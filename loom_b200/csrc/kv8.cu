@@ -58,6 +58,9 @@ __device__ __forceinline__ Span span_of(const int32_t* __restrict__ starts, cons
 // whether the sequence has room for them
 __device__ __forceinline__ bool fits(const Kv8& c, const Span& a) { return a.pos >= 0 && a.pos <= c.max_len && a.count <= c.max_len - a.pos; }
 
+// Rows that are not taken are said in the status word, unless a wait that ran out stands there: that one spoils other results too.
+__device__ __forceinline__ void say_not_taken(int* status, int code) { atomicCAS(status, 0, code); }
+
 // byte of a key's dimension d at place p of its block; of a value's
 __device__ __forceinline__ int key_byte(int p, int d, int dim_k) {
     const int c = d >> 6, whole = dim_k >> 6;
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_ke
         if (it.seq < 0) return;
         more = it.more;
         if (!fits(p.c, it.a)) {
-            if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.c.status, 7);
+            if (blockIdx.x == 0 && threadIdx.x == 0) say_not_taken(p.c.status, 7);
             continue;
         }
         if (it.a.count == 0) continue;
@@ -420,7 +423,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) lb_kv8_read_kernel(const RowPa
         if (it.seq < 0) return;
         more = it.more;
         if (!fits(p.c, it.a)) {
-            if (blockIdx.x == 0 && threadIdx.x == 0) atomicExch(p.c.status, 7);
+            if (blockIdx.x == 0 && threadIdx.x == 0) say_not_taken(p.c.status, 7);
             continue;
         }
         if (it.a.count == 0) continue;
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
         if (pass == 0) {
             total = v;
             if (total >> 31) {
-                if (me == 0 && tid == 0) atomicExch(c.status, kAtTooMuch);
+                if (me == 0 && tid == 0) say_not_taken(c.status, kAtTooMuch);
                 return;
             }
             share = total / p.ctas + 1;
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__(kAtThreads, AttendShape<NK, SETS>::kPerSm) lb_
         }
     }
     if (s_misfit) {  // rows that have no room: zeros, by all CTAs
-        if (me == 0 && tid == 0) atomicExch(c.status, 7);
+        if (me == 0 && tid == 0) say_not_taken(c.status, 7);
 #pragma unroll 1
         for (int i = 0; i < c.seqs; ++i) {
             const Span a = span_of(p.starts, p.lengths, p.rows, i);
