@@ -463,6 +463,7 @@ constexpr int kAtThreads = 128;
 constexpr int kAtWarps = kAtThreads / 32;
 constexpr int kAtRowsNk = 4;      // the kernel for portions has up to 128 dimensions: a row's results stay in a thread's registers
 constexpr int kAtWideRows = 48;   // rows of a sequence beyond which its tiles are wide
+constexpr int kAtPortionRows = 256;  // rows of a KV head's group, in a call, beyond which the kernel for portions looks for some
 constexpr int kAtSizes = 8;       // sizes of parts that are tried: 1, 1 + 1/8, 1 + 2/8 and so on of an equal share
 constexpr int kAtOpenFew = 6;     // what an open block costs, in blocks: beside one token's rows (5.8 us, four blocks 3.4 us)
 constexpr int kAtOpenWide = 3;    // and beside a wide tile's
@@ -1495,10 +1496,13 @@ int loom_b200_kv8_attend(loom_b200_ctx* ctx, loom_b200_kv8* c, int rows, int hea
     p.part_ld = (c->dim + 3) / 4 * 4 + 4;
     // tiles of eight rows a warp where sequences have no more on the average (any number is right with either)
     const bool few = (long long)rows * p.group <= 8LL * (starts ? c->seqs : rows);
-    // Sequences of many rows go to the kernel for portions, where the call has more than two rows a sequence on the average (13 to 512 rows of 4
-    // heads at 2900: 43 to 83 us instead of 125 to 238; but 5 us are its launch where there are none: 16 sequences of one row 41.6 us instead of 36.4).
+    // Sequences of many rows go to the kernel for portions, where the call has more than two rows a sequence on the average, or more than 256 rows
+    // of a KV head's group: which sequences have them is on the device, and a cache may have many that take no part.  13 to 512 rows of 4 heads at
+    // 2900: 43 to 83 us instead of 125 to 238; 200 rows of one of 256 sequences 71 instead of 118, 512 of them 97 instead of 351.  Its launch where there are
+    // none takes up to 5 us: 16 sequences of one row 41.6 us instead of 36.4, 128 of one at 1000 97 instead of 91.
     const int nk = c->dim_k / 32;
-    const bool portions = nk <= kAtRowsNk && (starts ? rows > 2 * c->seqs && (long long)rows * p.group > kAtWideRows : p.group > kAtWideRows);
+    const long long group_rows = (long long)rows * p.group;
+    const bool portions = nk <= kAtRowsNk && (starts ? group_rows > kAtWideRows && (rows > 2 * c->seqs || group_rows > kAtPortionRows) : p.group > kAtWideRows);
     const bool wide = !portions && (long long)(starts ? rows : 1) * p.group > kAtWideRows;
     int rc = 0;
     switch (nk) {
