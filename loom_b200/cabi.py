@@ -207,6 +207,29 @@ def _ptr(x):
     raise TypeError(type(x))
 
 
+_KINDS = {}  # torch's types of 32-bit numbers, once a tensor has come: whether they are floats
+
+
+def _dev(x, floats: bool):
+    """Device address of a buffer of 32-bit numbers: an address, None, or a tensor on a GPU that holds such numbers one behind the other."""
+    if x is None or isinstance(x, int):
+        return x
+    try:
+        if x.is_cuda and _KINDS[x.dtype] is floats and x.is_contiguous():
+            return x.data_ptr()
+    except (AttributeError, KeyError):
+        if hasattr(x, "data_ptr") and not _KINDS:
+            import torch
+
+            _KINDS.update({torch.float32: True, torch.int32: False})
+            return _dev(x, floats)
+    if not getattr(x, "is_cuda", False):
+        raise TypeError("a buffer on the device is wanted, not %s" % type(x).__name__)
+    if _KINDS.get(x.dtype) is not floats:
+        raise TypeError("a buffer of %s is wanted, not of %s" % ("float32" if floats else "int32", x.dtype))
+    raise ValueError("a tensor with strides %s" % (tuple(x.stride()),))
+
+
 class Weight:
     """A packed ternary matrix resident in HBM (GPUWeights[key] + GPUScaleValues[key])."""
 
@@ -390,8 +413,8 @@ class Context:
 
     def sample(self, rows, vocab, logits, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None, stride=None):
         """The next token of every row of logits (device buffers; one entry a row in every array)."""
-        self._check(lib().loom_b200_sample(self.h, rows, vocab, _ptr(logits), vocab if stride is None else stride, _ptr(temperature), _ptr(top_k), _ptr(top_p),
-                                           _ptr(min_p), _ptr(uniform), _ptr(tokens), _ptr(logprob)))
+        self._check(lib().loom_b200_sample(self.h, rows, vocab, _dev(logits, True), vocab if stride is None else stride, _dev(temperature, True), _dev(top_k, False),
+                                           _dev(top_p, True), _dev(min_p, True), _dev(uniform, True), _dev(tokens, False), _dev(logprob, True)))
 
     # ---- tensor parallelism: one process per GPU, one context per process ----
     @staticmethod
@@ -617,7 +640,8 @@ class Adapters:
 
     def apply(self, tokens, slot, x, out, base=None, ldx=None):
         """out[t] = base[t] + scale up (down x[t]) with the adapter in slot[t] (device buffers; base may be out)."""
-        self.ctx._check(lib().loom_b200_adapters_apply(self.ctx.h, self.h, tokens, _ptr(slot), _ptr(x), self.cols if ldx is None else ldx, _ptr(base), _ptr(out)))
+        self.ctx._check(lib().loom_b200_adapters_apply(self.ctx.h, self.h, tokens, _dev(slot, False), _dev(x, True), self.cols if ldx is None else ldx, _dev(base, True),
+                                                        _dev(out, True)))
 
     def free(self):
         if self.h:
@@ -647,16 +671,17 @@ class KV8:
         self.h = h
 
     def append(self, rows, lengths, k, v, starts=None, ld=None):
-        self.ctx._check(lib().loom_b200_kv8_append(self.ctx.h, self.h, rows, _ptr(starts), _ptr(lengths), _ptr(k), _ptr(v), self.kv_heads * self.head_dim if ld is None else ld))
+        self.ctx._check(lib().loom_b200_kv8_append(self.ctx.h, self.h, rows, _dev(starts, False), _dev(lengths, False), _dev(k, True), _dev(v, True),
+                                                    self.kv_heads * self.head_dim if ld is None else ld))
 
     def read(self, rows, lengths, k, v, starts=None):
         """The rows of that append as the cache holds them, into k and v."""
-        self.ctx._check(lib().loom_b200_kv8_read(self.ctx.h, self.h, rows, _ptr(starts), _ptr(lengths), _ptr(k), _ptr(v)))
+        self.ctx._check(lib().loom_b200_kv8_read(self.ctx.h, self.h, rows, _dev(starts, False), _dev(lengths, False), _dev(k, True), _dev(v, True)))
 
     def attend(self, rows, heads, lengths, q, out, starts=None, scale=0.0, ldq=None):
         """Causal attention of the rows that an append with the same starts and lengths has added."""
-        self.ctx._check(lib().loom_b200_kv8_attend(self.ctx.h, self.h, rows, heads, _ptr(starts), _ptr(lengths), _ptr(q), heads * self.head_dim if ldq is None else ldq,
-                                                   float(scale), _ptr(out)))
+        self.ctx._check(lib().loom_b200_kv8_attend(self.ctx.h, self.h, rows, heads, _dev(starts, False), _dev(lengths, False), _dev(q, True),
+                                                    heads * self.head_dim if ldq is None else ldq, float(scale), _dev(out, True)))
 
     def free(self):
         if self.h:
