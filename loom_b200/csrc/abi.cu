@@ -26,6 +26,7 @@ int lb_fail(loom_b200_ctx* ctx, int code, const char* fmt, ...) {
         std::lock_guard<std::mutex> lk(g_err_mu);
         g_global_error = buf;
     }
+    if (code == LOOM_B200_ERR_CUDA) (void)cudaGetLastError();  // (said here; the next launch's check must not find it again)
     return code;
 }
 
