@@ -335,6 +335,9 @@ __global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_ke
         const Item it = item_of(p, n);
         if (it.seq < 0) return;
         more = it.more;
+        // The first block's CTA alone reads and writes the note of its head's places.  (Read ahead of what the sequence's length decides.)
+        const auto placed = [&](int i) -> int* { return p.c.placed + (p.c.head_of(it.seq, h) * 2 + kv) * 2 + i; };
+        const int2 were = *reinterpret_cast<const int2*>(placed(0));
         if (!fits(p.c, it.a)) {
             if (blockIdx.x == 0 && threadIdx.x == 0) say_not_taken(p.c.status, 7);
             continue;
@@ -342,12 +345,10 @@ __global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_ke
         if (it.a.count == 0) continue;
         const int end = it.a.pos + it.a.count, first = it.a.pos / kKvBlock, last = (end - 1) / kKvBlock, b = first + it.block;
         const bool keep = b >= last - 1 && (b == first || ((b - first) & 1));
-        // The first block's CTA alone reads and writes the note of its head's places.
-        int* placed = p.c.placed + (p.c.head_of(it.seq, h) * 2 + kv) * 2;
-        const int there = b == first && it.a.pos % kKvBlock ? placed[first & 1] : first;
+        const int there = it.a.pos % kKvBlock == 0 ? first : first & 1 ? were.y : were.x;
         const bool whole = (b + 1) * kKvBlock <= end;
         if (!whole && keep) copy_rows<true>(p, it, b, kv, h);
-        if (there >= 0 && there != first && first < p.c.blocks) {  // (a last block that is no whole one has no codes)
+        if (b == first && there >= 0 && there != first && first < p.c.blocks) {  // (a last block that is no whole one has no codes)
             if (kv) restore_rows<true>(p.c, it.seq, h, first, it.a.pos);
             else restore_rows<false>(p.c, it.seq, h, first, it.a.pos);
         }
@@ -357,11 +358,8 @@ __global__ void __launch_bounds__(kRowThreads, NU == 1 ? 4 : 2) lb_kv8_append_ke
         }
         if (b == first && last - first >= 2) copy_rows<true>(p, it, last - ((last - first) & 1), kv, h);  // (behind the barrier that append_block ends with)
         if (b == first) {
-            __syncthreads();  // (everyone has read it)
-            if (threadIdx.x == 0) {
-                placed[last & 1] = last;
-                if (last > first) placed[last - 1 & 1] = last - 1;
-            }
+            if (last == first) __syncthreads();  // (everyone has read it; one of several blocks is whole and has ended with a barrier)
+            if (threadIdx.x < 2 && (threadIdx.x == 0 || last > first)) *placed(last - threadIdx.x & 1) = last - threadIdx.x;
         }
     }
 }
