@@ -489,10 +489,10 @@ int loom_b200_decoder_extend(loom_b200_decoder* dec, const int32_t* tokens, int 
  * min-p, from random numbers that the caller gives.  Per row, arrays [rows], each but `uniform` may be NULL (= 1, 0, 1, 0):
  *   order  larger logits first, equal ones by index; weight w_i = exp((l_i - largest) / temperature)
  *   kept   the first top_k (0 or less: all); of those the shortest run from the front that holds top_p of their weight (1 or more: all;
- *          one token at least); of those the ones with w_i >= min_p (0 or less: all)
+ *          one token at least); of those the ones with w_i >= min_p (0 or less: all; above 1: as 1)
  *   token  the first kept one by index at which the kept weight up to it exceeds uniform (0 <= uniform < 1; else the last one, or the
  *          first) times all of it
- * temperature 0 or less: the first largest logit.  Not-a-numbers and minus infinity are never chosen; plus infinities share alike; a row
+ * temperature 0 or less, or not a number: the first largest logit.  Not-a-numbers and minus infinity are never chosen; plus infinities share alike; a row
  * with nothing to choose gives -1.  logprob [rows] or NULL: logarithm of the chosen token's share of the kept weight (not a number for -1).
  * Sums are integers and repeat bit for bit.  vocab <= 655,360. */
 int loom_b200_sample(loom_b200_ctx* ctx, int rows, int vocab, const float* logits, long long stride, const float* temperature,
@@ -531,7 +531,8 @@ int loom_b200_adapters_apply(loom_b200_ctx* ctx, const loom_b200_adapters* a, in
  * of the first `rows` sequences, a decode step.  A sequence is cut back by giving a smaller length, as often as wanted.  Of the block that its last
  * position lies in, and of the one in front of that, the float32 rows are there, and a block cut into goes on from them; cut back further, or into a block
  * whose float32 rows an append of two blocks further on has replaced since, it goes on from that block's rows as they are held in 8 bits.  Rows that a
- * sequence has no room for are not taken (attention: zeros), which loom_b200_sync reports as LOOM_B200_ERR_INVALID. */
+ * sequence has no room for are not taken (attention: zeros), which loom_b200_sync reports as LOOM_B200_ERR_INVALID; so it does where starts that go
+ * back give many sequences the same rows, more than attention can count (it leaves out as it is then). */
 typedef struct loom_b200_kv8 loom_b200_kv8;
 int loom_b200_kv8_create(loom_b200_ctx* ctx, int sequences, int max_len, int kv_heads, int head_dim, loom_b200_kv8** out);
 void loom_b200_kv8_free(loom_b200_ctx* ctx, loom_b200_kv8* cache);

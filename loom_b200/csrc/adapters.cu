@@ -429,7 +429,8 @@ int launch_adapters(loom_b200_ctx* ctx, const AdapterParams& p, int tiles) {
     LB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     // As many CTAs a tile as are there at once.  Clusters of more than eight find their places in a GPC less and less well (256 tokens of
     // two adapters: 12 CTAs a tile 13.9 us, 14 18.6 us), so those leave a quarter free; 14 clusters of 16 still fit (16 tokens of rank 16, 4096 to
-    // 14336: 13.9 us by 16 CTAs each, 11.6 by 12, 12.0 by 8; 14 tokens 8.5, 10.8 and 11.8 us; with sixteen warps a CTA no better).
+    // 14336: 13.9 us by 16 CTAs each, 11.6 by 12, 12.0 by 8; 14 tokens 8.5, 10.8 and 11.8 us; with sixteen warps a CTA no better).  Both are measured on one
+    // division of the SMs into GPCs; any size is right on any other.
     const int most = kAdPerSm * ctx->sm_count;
     int size = most * 7 / 8 / tiles;
     if (size >= kAdMostCtas) size = tiles <= 14 ? kAdMostCtas : 12;

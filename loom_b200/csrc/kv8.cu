@@ -81,8 +81,8 @@ __device__ __forceinline__ int value_byte(int p, int d) { return (d >> 3) * 512 
 // A code is the float32 product where that is further than 2^-10 from a half (its error is below 2^-16) and the float64 arithmetic
 // elsewhere, one value in five hundred: conversions and float64 take sixteen values a clock of an SM.
 //
-// Bound: memory; for few rows, latencies.  5000 rows of eight heads of 128 in 8 sequences: append 18.5 us, read 11.8 us (52 MB
-// each way, 2.8 and 4.4 TB/s: waves of CTAs, each its loads, its largest value and its stores one behind the other); one row of each of 64 sequences: 6.7 and 4.9 us.  A CTA for each head: with two, four and all eight heads
+// Bound: memory; for few rows, latencies.  4944 rows of eight heads of 128 in 8 sequences: append 18.7 us, read 10.8 us (52 MB
+// each way, 2.8 and 4.8 TB/s: waves of CTAs, each its loads, its largest value and its stores one behind the other); one row of each of 64 sequences: 7.4 and 6.1 us.  A CTA for each head: with two, four and all eight heads
 // a CTA the append takes 28, 38 and 66 us; runs of two to eight blocks a CTA 21 to 40 us.
 constexpr int kRowThreads = 256;
 
@@ -455,8 +455,8 @@ __global__ void __launch_bounds__(kRowThreads, 3) lb_kv8_read_kernel(const RowPa
 // for bit.
 //
 // Bound: the codes' way from memory, 5.4 TB/s while it lasts, behind the list and the queries (4 us) and in front of open blocks and joining.  One
-// row of 32 heads over 8 of 128 dimensions at position 131,071: 65.9 us, 49 of them the blocks; 16 sequences at about 4000: 36.4 us; 20 heads over 5 at
-// 1040: 13.7 us.
+// row of 32 heads over 8 of 128 dimensions at position 131,071: 67.5 us, 49 of them the blocks; 16 sequences of 2554 positions on the average: 36.9 us; 20
+// heads over 5 at 1040: 14.1 us.
 constexpr int kAtThreads = 128;
 constexpr int kAtWarps = kAtThreads / 32;
 constexpr int kAtRowsNk = 4;      // the kernel for portions has up to 128 dimensions: a row's results stay in a thread's registers

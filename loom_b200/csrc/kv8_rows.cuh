@@ -20,7 +20,7 @@
 // by twos, so that results repeat bit for bit.
 //
 // Bound: a block costs two CTAs of an SM 2.7 us: weights 0.8 and 0.5, results 0.5, waiting for S 0.5 (its MMAs come 94 clocks apart, with an operand A
-// of 4 KB of shared memory for 64 columns), the tensor pipe counted as active 14 % and issue slots 33 % of the kernel.  300 rows of 20 heads over 5 of 128 dimensions at position 2900: 63 us (without these
+// of 4 KB of shared memory for 64 columns), the tensor pipe counted as active 14 % and issue slots 33 % of the kernel.  300 rows of 20 heads over 5 of 128 dimensions at position 2900: 63.6 us (without these
 // tiles, on integer instructions, 93 us; with them on integer digits 89 us; with one set of warps for both kinds of work 66 us), of which 12 are the list and
 // the queries, 28 the blocks, 15 the parts' joining; 2048 rows at 8000: 755 us (1690), 2048 from the start 135 us (354).
 constexpr int kRwThreads = 256;

@@ -6,7 +6,7 @@
 //            and all others 0
 //   order    larger logit first, equal ones by index
 //   kept     the first k of the order; of those the shortest run from the front whose weight is at least p times theirs (one token at
-//            least); of those the ones with w_i >= min_p
+//            least); of those the ones with w_i >= min_p (above 1: as 1)
 //   token    the first kept one, by index, whose weight and that of the kept ones in front of it exceed u times the kept weight
 // T <= 0 is the first largest logit.  Weights are integers, round(w 2^S) with S such that a whole row's sum stays below 2^62: sums do not
 // depend on their order then.  They are within vocab * 2^-S of the largest weight (S = 44 for 128,256 tokens: 7e-9) and 2^-32 of themselves of the
@@ -30,10 +30,10 @@
 // product, of a distance that is exact.  (A float32 exponential, 2^-22 of a weight, moved the borders of 128,256 tokens of nearly equal weight by
 // thousandths of one.  64 rows of 128,256: 91 us with that, 98 so, 103 with 32 entries and what they leave in pairs of floats.)
 //
-// Bound: latencies one behind the other, 1.2 to 2 us for an exchange over the cluster; the reads are 5 of the 82 us that 64 rows of 128,256
+// Bound: latencies one behind the other, 1.2 to 2 us for an exchange over the cluster; the reads are 5 of the 92 to 98 us that 64 rows of 128,256
 // take, a row of 32,000 by temperature, top-k and top-p takes 25 us.  So a row goes over as many CTAs as give 2048 logits each while there
 // are SMs for them, and 16,384 each beyond (the CTAs of a row wait for one another, four rows share an SM's time); where every CTA read all bins
-// instead of a share of them, 64 rows took 98 us.
+// instead of a share of them, 64 rows took 16 us more.
 #include "common.cuh"
 
 #include <math_constants.h>
