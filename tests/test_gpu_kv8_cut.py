@@ -151,3 +151,32 @@ def test_cuts_in_a_recorded_frame():
         ctx.graph_free(frame)
     finally:
         ctx.close()
+
+
+def test_a_cut_into_a_block_that_is_not_finite(ctx):
+    """Its rows are gone: what they go on from reads as not-a-numbers, in that head and side alone, until the block begins anew."""
+    rng = np.random.default_rng(3)
+    kv, zero = cabi.KV8(ctx, 1, 400, 2, 32), ctx.to_device(np.zeros(1, np.int32))
+    k, v = (rng.standard_normal((330, 2, 32)).astype(np.float32) for _ in "kv")
+    k[70, 1, 5] = np.inf
+
+    def append(kk, vv, at):
+        starts, lengths = ctx.to_device(np.array([0, len(kk)], np.int32)), ctx.to_device(np.array([at], np.int32))
+        kv.append(len(kk), lengths, ctx.to_device(kk), ctx.to_device(vv), starts=starts)
+
+    def held(n):
+        out = [ctx.to_device(np.zeros((n, 2, 32), np.float32)) for _ in "kv"]
+        kv.read(n, zero, *out, starts=ctx.to_device(np.array([0, n], np.int32)))
+        return [ctx.download(o, (n, 2, 32), np.float32) for o in out]
+    append(k, v, 0)
+    append(k[90:91], v[90:91], 90)  # block 1, whose place block 5 has: 64 .. 89 from the codes
+    got_k, got_v = held(91)
+    assert np.isnan(got_k[64:90, 1]).all() and np.isfinite(got_k[:, 0]).all() and np.isfinite(got_k[:64]).all() and np.isfinite(got_v).all()
+    assert np.array_equal(got_k[90], k[90]) and np.array_equal(got_v[90], v[90])
+    assert np.array_equal(got_k[64:90, 0], kit.held(k, exact=False)[64:90, 0])
+    fresh = rng.standard_normal((70, 2, 32)).astype(np.float32)
+    append(fresh, fresh, 64)  # cut to the block's beginning
+    got_k, _ = held(134)
+    assert np.array_equal(got_k[64:], kit.held(np.concatenate([k[:64], fresh]), exact=False)[64:])
+    ctx.sync()
+    kv.free()
